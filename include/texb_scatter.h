@@ -406,6 +406,33 @@ int texb_scatter_mean_max_backward(const float* g_mean, const float* g_max,
                                    float* g_in, int64_t n, int channel,
                                    int64_t num_segments, void* stream);
 
+/* ---- rows of a table by token ------------------------------------------------
+ * The lookup that feeds token or voxel ids into a model, and the gradient of its
+ * table: texb_scatter_sum's reduction with the tokens as segment ids, dense over
+ * the table.  No counterpart in the reference.
+ *   tokens     : n ids of id_bytes (4 or 8) bytes each, any order;
+ *   dtype      : TEXB_FLOAT32, TEXB_BFLOAT16 or TEXB_FLOAT16, of weight / g and of
+ *                out / g_weight alike; rows of `dim` values, contiguous;
+ *   forward    : out[t, :] = scale * weight[tokens[t], :], widened to fp32, scaled,
+ *                rounded once (scale 1 copies the values as they are);
+ *   backward   : g_weight[v, :] = scale * (sum of the rows t of g with tokens[t] = v),
+ *                summed in fp32 (error-free additions for fp32 rows) and rounded
+ *                once; every row of g_weight[vocab, dim] is written, rows without a
+ *                token with 0.  Tokens equal to padding_idx (-1: none) take no part.
+ *                No floating-point atomics: bit-reproducible run to run.
+ * A token outside [0, vocab) reads nothing: its output row is 0, it takes no part
+ * in the gradient, and it is counted (texb_device_status, bad_indices).
+ * Limits: n and vocab < 2^31 - 65536. */
+#define TEXB_FLOAT32 0
+#define TEXB_BFLOAT16 1
+#define TEXB_FLOAT16 2
+int texb_embedding_forward(const void* tokens, int id_bytes, int64_t n, const void* weight, int dtype,
+                           int64_t vocab, int dim, float scale, void* out, void* stream);
+size_t texb_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int dim);
+int texb_embedding_backward(const void* tokens, int id_bytes, int64_t n, const void* g, int dtype,
+                            int64_t vocab, int dim, float scale, int64_t padding_idx, void* g_weight,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- peer buffers for the multi-GPU driver ---------------------------------------
  * One process per GPU; a caller that wants every GPU to hold the whole result of a
  * sharded reduction lets each GPU write its shard into a buffer the other processes

@@ -82,6 +82,12 @@ _SIGNATURES = {
     "texb_scatter_mean_max_backward": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                                   _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int64,
                                                   _c.c_void_p]),
+    "texb_embedding_forward": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_int64,
+                                          _c.c_int, _c.c_float, _c.c_void_p, _c.c_void_p]),
+    "texb_embedding_backward_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int64, _c.c_int]),
+    "texb_embedding_backward": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_int64,
+                                           _c.c_int, _c.c_float, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_size_t,
+                                           _c.c_void_p]),
 }
 
 OP_SUM, OP_MEAN, OP_MAX = 0, 1, 2

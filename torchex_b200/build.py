@@ -6,7 +6,7 @@ libraries this builds) writes
 * ``torchex_b200/lib/libtexb_scatter.so`` -- the kernels behind the plain C ABI of
   ``include/texb_scatter.h`` (nvcc; no torch dependency), and
 * ``torchex_b200/lib/scatter_ext*.so`` -- the torch extension module ``scatter_ext``
-  (g++ against the installed torch; ``csrc/scatter_ext_binding.cpp``), which binds that
+  (g++ against the installed torch; ``csrc/*_binding.cpp``), which binds that
   C ABI to tensors the way TorchEx's own ``scatter_ext`` does.
 
 Each ``.cu`` file is compiled to its own object (in parallel, and only when it or a
@@ -30,13 +30,15 @@ OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libtexb_scatter.so")
 HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "texb_scatter.h")
 SOURCES = ["abi.cu", "segment_reduce.cu", "reduce_unit_sum.cu", "reduce_unit_sum_plain.cu", "reduce_unit_max.cu",
-           "reduce_unit_sum_max.cu", "segment_small.cu", "segment_plan.cu", "segment_backward.cu", "peer_copy.cu"]
+           "reduce_unit_sum_max.cu", "segment_small.cu", "segment_plan.cu", "segment_backward.cu", "peer_copy.cu",
+           "embedding.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
 ]
 EXT_NAME = "scatter_ext"
-EXT_SOURCE = os.path.join(CSRC, "scatter_ext_binding.cpp")
+EXT_SOURCES = [os.path.join(CSRC, f) for f in ("scatter_ext_binding.cpp", "token_ops_binding.cpp")]
+EXT_HEADER = os.path.join(CSRC, "binding.h")
 EXT_PATH = os.path.join(LIB_DIR, EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
@@ -97,7 +99,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def extension_is_stale() -> bool:
     # the module links the library dynamically: only its own source and the ABI header matter
-    return _newer(EXT_PATH, [EXT_SOURCE, HEADER])
+    return _newer(EXT_PATH, EXT_SOURCES + [EXT_HEADER, HEADER])
 
 
 def build_extension(force: bool = False) -> str:
@@ -110,15 +112,23 @@ def build_extension(force: bool = False) -> str:
     from torch.utils import cpp_extension as ce
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda_home = ce.CUDA_HOME or "/usr/local/cuda"
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    gxx = shutil.which("g++") or "g++"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-DTORCH_EXTENSION_NAME={EXT_NAME}",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
     for inc in ce.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda_home, "include"),
                                      os.path.dirname(HEADER)]:
-        cmd += ["-isystem", inc]
-    cmd += [EXT_SOURCE, "-o", EXT_PATH, f"-L{torch_lib}", f"-L{LIB_DIR}", "-ltexb_scatter",
-            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
-            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
+        flags += ["-isystem", inc]
+    objs, jobs = [], []
+    for src in EXT_SOURCES:
+        obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-4] + ".o")
+        objs.append(obj)
+        if force or _newer(obj, [src, EXT_HEADER, HEADER]):
+            jobs.append([gxx, *flags, "-c", "-o", obj, src])
+    with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, len(jobs))) as pool:
+        list(pool.map(lambda j: _run(j, "g++ " + os.path.basename(j[-1])), jobs))
+    cmd = [gxx, "-shared", *objs, "-o", EXT_PATH, f"-L{torch_lib}", f"-L{LIB_DIR}", "-ltexb_scatter",
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     _run(cmd, "g++ scatter_ext")
     return EXT_PATH
 

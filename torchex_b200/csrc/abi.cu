@@ -56,6 +56,11 @@ int peer_pull_impl(const void* const*, void* const*, const size_t*, int, void* c
                    cudaStream_t);
 int mean_from_sum_impl(const float*, const int32_t*, int64_t, int, float*, cudaStream_t);
 
+int embedding_forward_impl(const void*, int, int64_t, const void*, int, int64_t, int, float, void*, cudaStream_t);
+size_t embedding_backward_workspace_bytes_impl(int64_t, int64_t, int);
+int embedding_backward_impl(const void*, int, int64_t, const void*, int, int64_t, int, float, int64_t, void*, void*,
+                            size_t, cudaStream_t);
+
 namespace {
 thread_local char t_error[512] = "";
 
@@ -153,7 +158,7 @@ using namespace texb;
 
 extern "C" {
 
-int texb_version(void) { return 202; }
+int texb_version(void) { return 203; }
 
 const char* texb_last_error(void) { return t_error; }
 
@@ -393,6 +398,21 @@ int texb_peer_pull_mean(const void* const* srcs, void* const* dsts, void* const*
 int texb_mean_from_sum(const float* sums, const int32_t* counts, int64_t num_segments, int channel, float* out,
                        void* stream) {
   return mean_from_sum_impl(sums, counts, num_segments, channel, out, static_cast<cudaStream_t>(stream));
+}
+
+int texb_embedding_forward(const void* tokens, int id_bytes, int64_t n, const void* weight, int dtype, int64_t vocab,
+                           int dim, float scale, void* out, void* stream) {
+  return embedding_forward_impl(tokens, id_bytes, n, weight, dtype, vocab, dim, scale, out,
+                                static_cast<cudaStream_t>(stream));
+}
+size_t texb_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int dim) {
+  return embedding_backward_workspace_bytes_impl(n, vocab, dim);
+}
+int texb_embedding_backward(const void* tokens, int id_bytes, int64_t n, const void* g, int dtype, int64_t vocab,
+                            int dim, float scale, int64_t padding_idx, void* g_weight, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  return embedding_backward_impl(tokens, id_bytes, n, g, dtype, vocab, dim, scale, padding_idx, g_weight, workspace,
+                                 workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

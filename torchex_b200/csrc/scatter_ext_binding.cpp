@@ -16,37 +16,14 @@
 // allocates the outputs, picks the kernel path and launches -- a single trip from
 // Python per reduction.
 
-#include <torch/extension.h>
-
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
+#include "binding.h"
 
 #include <tuple>
 #include <vector>
 
-#include "texb_scatter.h"
+using namespace texb_binding;
 
 namespace {
-
-#define TEXB_CHECK_CUDA(x) TORCH_CHECK((x).device().is_cuda(), #x, " must be a CUDAtensor ")
-#define TEXB_CHECK_CONTIGUOUS(x) TORCH_CHECK((x).is_contiguous(), #x, " must be contiguous ")
-#define TEXB_CHECK_INPUT(x) \
-  TEXB_CHECK_CUDA(x);       \
-  TEXB_CHECK_CONTIGUOUS(x)
-#define TEXB_CHECK_DTYPE(x, t) \
-  TORCH_CHECK((x).scalar_type() == (t), #x, " must have dtype ", (t), ", got ", (x).scalar_type())
-
-void check_status(int status, const char* what) {
-  TORCH_CHECK(status == TEXB_OK, what, " failed with status ", status, ": ", texb_last_error());
-}
-
-void* stream_of(const at::Tensor& t) {
-  return static_cast<void*>(at::cuda::getCurrentCUDAStream(t.get_device()).stream());
-}
-
-at::Tensor scratch(size_t bytes, const at::Tensor& like) {
-  return at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, like.options().dtype(at::kByte));
-}
 
 // ---- the reference's three functions ------------------------------------------------
 
@@ -116,42 +93,6 @@ void get_pre_sum_gpu(at::Tensor unq_inv, at::Tensor preSum) {
 }
 
 // ---- plan-based operators ---------------------------------------------------------------
-
-struct Plan {
-  at::Tensor sid;      // int32 [n]: segment id at each segment-sorted position
-  at::Tensor perm;     // int32 [n]: feats row at that position; undefined when the ids arrived sorted
-  at::Tensor offsets;  // int32 [m + 1]: TorchEx's preSum
-  at::Tensor balance;  // int32 [K + 1]: cost-balanced cut points of the sorted rows
-  int64_t num_total = 0, num_segments = 0;
-  int64_t max_cnt = -1;    // rows of the largest segment, -1 while the host does not know it
-  bool has_empty = true;   // false only once the host knows that every segment has rows
-  bool settled = false;    // the host has synchronised with the stream since the arrays were built
-  bool no_split = false;   // every cut of the balance table is a segment start (short segments only)
-  struct Scratch {
-    int64_t channels;
-    int slot;  // 0: single calls; k: the k-th reduction of a sequence; -1: the two-output operator
-    void* stream;
-    at::Tensor buffer;
-  };
-  std::vector<Scratch> scratch_cache;  // one buffer per (channel count, operator kind, stream)
-
-  int flags() const {
-    return (has_empty || num_total == 0 ? TEXB_PLAN_HAS_EMPTY : 0) | (settled ? TEXB_PLAN_SETTLED : 0) |
-           (no_split ? TEXB_PLAN_NO_SPLIT : 0);
-  }
-  const int32_t* perm_ptr() const { return perm.defined() ? perm.data_ptr<int>() : nullptr; }
-
-  // Calls on one stream are ordered, so they can share a buffer; another stream gets its own.
-  at::Tensor& workspace(int64_t channels, int slot, void* stream, size_t bytes) {
-    for (auto& s : scratch_cache)
-      if (s.channels == channels && s.slot == slot && s.stream == stream) {
-        if (size_t(s.buffer.numel()) < bytes) s.buffer = scratch(bytes, sid);
-        return s.buffer;
-      }
-    scratch_cache.push_back({channels, slot, stream, scratch(bytes, sid)});
-    return scratch_cache.back().buffer;
-  }
-};
 
 Plan make_plan(at::Tensor sid, c10::optional<at::Tensor> perm, at::Tensor offsets, at::Tensor balance,
                int64_t num_segments, bool has_empty, int64_t max_cnt, bool settled) {
@@ -469,4 +410,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mean_max_backward", &mean_max_backward);
   m.def("segment_rank", &segment_rank);
   m.def("abi_version", &texb_version);
+  register_token_ops(m);
 }

@@ -1,4 +1,5 @@
-"""The compiled torch extension ``scatter_ext`` (``csrc/scatter_ext_binding.cpp``).
+"""The compiled torch extension ``scatter_ext`` (``csrc/scatter_ext_binding.cpp`` and the
+other binding files beside it).
 
 TorchEx's operators import a native module of that name
 (torchex/operator_py/scatter_op.py:4) exposing ``sum(feats, preSum, out,
@@ -49,6 +50,8 @@ reduce_sequence = getattr(native, "reduce_sequence", None)
 broadcast_back = native.broadcast_back
 mean_max_backward = native.mean_max_backward
 segment_rank = native.segment_rank
+embedding_forward = native.embedding_forward
+embedding_backward = native.embedding_backward
 abi_version = native.abi_version
 
 
