@@ -720,6 +720,15 @@ int plan_balance_impl(const int32_t* sid, int64_t n, int32_t* table, int table_l
   return check_launch("balance_table_kernel");
 }
 
+// The stable radix sort alone: keys[n] in [0, bound) -> the sorted keys and the position each came from.
+int sort_keys_impl(const int32_t* keys, int64_t n, int64_t bound, int32_t* keys_out, int32_t* perm_out, void* workspace,
+                   size_t workspace_bytes, cudaStream_t stream) {
+  const SortWorkspace sw = carve_sort_workspace(workspace, n);
+  if (!workspace || workspace_bytes < sw.bytes)
+    return fail(TEXB_ERR_WORKSPACE, "sort workspace: need %zu bytes, got %zu", sw.bytes, workspace_bytes);
+  return run_sort<int32_t>(keys, n, bound, keys_out, perm_out, sw, stream);
+}
+
 // Plan entries found outside their range by segment_rank_kernel (a segment id outside
 // [0, num_segments), a perm entry outside [0, n)): the entry is skipped and counted
 // (sticky; part of texb_device_status) instead of being used as an address.

@@ -174,20 +174,22 @@ int segment_reduce_static_impl(int op, const float* feats, const int32_t* sid, c
 
 int small_bad_indices_impl(int* count);  // segment_small.cu
 int plan_bad_indices_impl(int* count);   // segment_plan.cu
-int embedding_bad_tokens_impl(int* count);  // embedding.cu
+int lookup_bad_tokens_impl(int* count);      // embedding.cu
+int table_grad_bad_tokens_impl(int* count);  // embedding_backward.cu
 
 int device_status_impl(int* wait_timeouts, int* bad_indices) {
-  int v = 0, w = 0, w_small = 0, w_plan = 0, w_tokens = 0;
+  int v = 0, w = 0, w_small = 0, w_plan = 0, w_lookup = 0, w_table = 0;
   int st = reduce_counters_sum(&v, &w);
   if (st == TEXB_OK) st = reduce_counters_sum_plain(&v, &w);
   if (st == TEXB_OK) st = reduce_counters_max(&v, &w);
   if (st == TEXB_OK) st = reduce_counters_sum_max(&v, &w);
   if (st == TEXB_OK) st = small_bad_indices_impl(&w_small);
   if (st == TEXB_OK) st = plan_bad_indices_impl(&w_plan);
-  if (st == TEXB_OK) st = embedding_bad_tokens_impl(&w_tokens);
+  if (st == TEXB_OK) st = lookup_bad_tokens_impl(&w_lookup);
+  if (st == TEXB_OK) st = table_grad_bad_tokens_impl(&w_table);
   if (st != TEXB_OK) return st;
   if (wait_timeouts) *wait_timeouts = v;
-  if (bad_indices) *bad_indices = w + w_small + w_plan + w_tokens;
+  if (bad_indices) *bad_indices = w + w_small + w_plan + w_lookup + w_table;
   return TEXB_OK;
 }
 
