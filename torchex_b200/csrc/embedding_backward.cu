@@ -72,9 +72,27 @@ struct SortLayout {  // shared memory of a sorting CTA, in bytes
   static constexpr int kCounts = 0;                                       // uint16 [kSortWarps][kMaxBins]
   static constexpr int kTotals = kCounts + kSortWarps * kMaxBins * 2;     // uint32 [kMaxCluster][kMaxBins]
   static constexpr int kBase = kTotals + kMaxCluster * kMaxBins * 4;      // uint32 [kMaxBins]
-  static constexpr int kScan = kBase + kMaxBins * 4;                      // uint32 [32]
+  static constexpr int kStart = kBase + kMaxBins * 4;                     // uint32 [kMaxBins]
+  static constexpr int kScan = kStart + kMaxBins * 4;                     // uint32 [32]
   static constexpr int kItems = kScan + 128;                              // uint2 [items of the CTA]
 };
+
+// Sum of `v` over the threads before this one.  All threads of the CTA call it; values beyond the first
+// 512 threads must be 0 (only their sum over 16 warps is needed).
+__device__ __forceinline__ uint32_t exclusive_scan(uint32_t v, uint32_t* scan) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t incl = v;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();  // the last call's readers are done
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  uint32_t before = incl - v;
+  for (int w = 0; w < min(warp, kMaxBins / 32); ++w) before += scan[w];
+  return before;
+}
 
 // Cluster 0 sorts; CTAs of the other clusters clear the rows of the table without a token.
 // items: tokens per thread (a power of two); digit_bits * passes covers the keys 0 .. vocab.
@@ -98,7 +116,12 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
 #pragma unroll 4
       for (int i = threadIdx.x; i < n; i += kSortThreads) {
         const int64_t key = key_of<IdT>(tokens[i], vocab, padding, false);
-        if (key >= lo && key < hi) atomicOr(&marks[(key - lo) >> 5], 1u << ((key - lo) & 31));
+        if (key >= lo && key < hi) {
+          // a frequent token is marked once, not by a queue of atomics on one word
+          volatile uint32_t* word = &marks[(key - lo) >> 5];
+          const uint32_t bit = 1u << ((key - lo) & 31);
+          if (!(*word & bit)) atomicOr(&marks[(key - lo) >> 5], bit);
+        }
       }
       __syncthreads();
       for (int64_t v = lo + threadIdx.x / lanes; v < hi; v += kSortThreads / lanes)
@@ -113,6 +136,7 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
   uint16_t(*counts)[kMaxBins] = reinterpret_cast<uint16_t(*)[kMaxBins]>(smem + SortLayout::kCounts);
   uint32_t(*totals)[kMaxBins] = reinterpret_cast<uint32_t(*)[kMaxBins]>(smem + SortLayout::kTotals);
   uint32_t* base = reinterpret_cast<uint32_t*>(smem + SortLayout::kBase);
+  uint32_t* local_start = reinterpret_cast<uint32_t*>(smem + SortLayout::kStart);
   uint32_t* scan = reinterpret_cast<uint32_t*>(smem + SortLayout::kScan);
   uint2* buffer = reinterpret_cast<uint2*>(smem + SortLayout::kItems);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -122,6 +146,7 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
   const int bins = 1 << digit_bits;
   const int mine = warp * items * 32 + lane;  // place of item 0 of this lane in the CTA's share
   const uint32_t before_me = (1u << lane) - 1u;
+  const int share = max(0, min(per_cta, n - rank * per_cta));  // tokens of this CTA: all but the last ones have per_cta
 
   uint2 item[kMaxItems];  // (key, position)
 #pragma unroll
@@ -138,7 +163,7 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
 #pragma unroll
     for (int k = 0; k < kMaxItems; ++k) {
       if (k < items) {
-        const bool valid = rank * per_cta + mine + k * 32 < n;
+        const bool valid = mine + k * 32 < share;
         const uint32_t d = (item[k].x >> shift) & (bins - 1);
         uint32_t peers = __ballot_sync(0xffffffffu, valid);
         for (int b = 0; b < digit_bits; ++b) {
@@ -156,8 +181,8 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
     __syncthreads();
     // counts become prefixes over the CTA's warps; the CTA's totals go to every CTA of the cluster
     const int d = threadIdx.x;
+    uint32_t run = 0u;
     if (d < bins) {
-      uint32_t run = 0u;
 #pragma unroll 8
       for (int w = 0; w < kSortWarps; ++w) {
         const uint32_t c = counts[w][d];
@@ -166,6 +191,23 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
       }
       for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(&totals[rank][d], r)[0] = run;
     }
+    uint32_t start = exclusive_scan(run, scan);
+    if (d < bins) local_start[d] = start;
+    __syncthreads();
+    // The share is first put into digit order in this CTA's own memory (nobody writes into it before
+    // the next cluster barrier), so that the stores into the other CTAs' memory run along consecutive
+    // words: 8-byte stores to scattered places of the cluster took 25 of a pass's 32 us at 131 072 tokens.
+#pragma unroll
+    for (int k = 0; k < kMaxItems; ++k) {
+      if (k < items && mine + k * 32 < share) {
+        const uint32_t dg = (item[k].x >> shift) & (bins - 1);
+        buffer[local_start[dg] + counts[warp][dg] + order[k]] = item[k];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMaxItems; ++k)
+      if (k < items && k * kSortThreads + int(threadIdx.x) < share) item[k] = buffer[k * kSortThreads + threadIdx.x];
     cluster.sync();
     // place of this CTA's first item of each digit: all items of smaller digits, and those of this
     // digit in earlier CTAs
@@ -177,24 +219,14 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
         all += t;
       }
     }
-    uint32_t incl = all;
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
-    }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    if (d < bins) {
-      uint32_t smaller = incl - all;
-      for (int w = 0; w < warp; ++w) smaller += scan[w];
-      base[d] = smaller + earlier;
-    }
+    start = exclusive_scan(all, scan);
+    if (d < bins) base[d] = start + earlier - local_start[d];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kMaxItems; ++k) {
-      if (k < items && rank * per_cta + mine + k * 32 < n) {
-        const uint32_t dg = (item[k].x >> shift) & (bins - 1);
-        const uint32_t to = base[dg] + counts[warp][dg] + order[k];  // < n <= ranks * per_cta
+      const int at = k * kSortThreads + int(threadIdx.x);  // place in the CTA's digit order
+      if (k < items && at < share) {
+        const uint32_t to = base[(item[k].x >> shift) & (bins - 1)] + uint32_t(at);  // < n <= ranks * per_cta
         cluster.map_shared_rank(buffer, to >> shift_cta)[to & (per_cta - 1)] = item[k];
       }
     }
@@ -203,7 +235,7 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
     // for the others' reads before it ends
 #pragma unroll
     for (int k = 0; k < kMaxItems; ++k)
-      if (k < items && rank * per_cta + mine + k * 32 < n) item[k] = buffer[mine + k * 32];
+      if (k < items && mine + k * 32 < share) item[k] = buffer[mine + k * 32];
   }
 #pragma unroll
   for (int k = 0; k < kMaxItems; ++k) {
@@ -277,13 +309,15 @@ struct Sum {  // running sum of one column
 };
 
 // A lane holds kBlocks accesses of BYTES bytes of a chunk of columns: eight values, whatever the
-// width of the access.
+// width of the access.  Its ring in shared memory holds kStages batches of kBatch rows, 384 bytes.
+constexpr int kSumThreads = 128;
 template <typename T, int BYTES>
 struct Shape {
   static constexpr int kVec = BYTES / int(sizeof(T));
   static constexpr int kBlocks = 8 / kVec;
   static constexpr int kColumns = 8;
-  static constexpr int kInFlight = 32 / (kBlocks * (BYTES >= 4 ? BYTES / 4 : 1));  // rows of g in flight: 32 registers
+  static constexpr int kStages = 3;
+  static constexpr int kBatch = 16 / int(sizeof(T));
 };
 
 struct Tiles {
@@ -353,150 +387,207 @@ __device__ __forceinline__ void store_row(const Tiles& t, T* g_weight, int64_t v
   }
 }
 
-// One group of lanes per (tile, chunk of columns).
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// One access of a row of g into the lane's ring.  Rows of an odd number of 16-bit values have no
+// 4-byte alignment to copy by, and go through registers.
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(kThreads)
+__device__ __forceinline__ void fetch(Chunk<T, BYTES>* to, const T* from) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_address(to)), "l"(from) : "memory");
+  } else if constexpr (BYTES == 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_address(to)), "l"(from) : "memory");
+  } else {
+    *to = load_chunk_once<T, BYTES>(from);
+  }
+}
+
+// One group of lanes per (tile, chunk of columns).  The rows of g go through a ring in shared memory,
+// three batches deep, in which every lane reads only what it copied itself -- so the copies need no
+// barrier, and a run's end does not hold back the loads behind it.  Walking the rows of a batch is a
+// loop, not unrolled: eight copies of the code that closes a run (division of the work between row and
+// slot, stores) overflowed the instruction cache, and took 27 us instead of 9 for 16 384 rows of 1024.
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(kSumThreads)
 sum_tiles_kernel(const T* __restrict__ g, const int32_t* __restrict__ sid, const int32_t* __restrict__ perm, Tiles t,
                  T* __restrict__ g_weight) {
   using S = Shape<T, BYTES>;
+  using Access = Chunk<T, BYTES>;
+  __shared__ Access ring[S::kStages][S::kBatch][S::kBlocks][kSumThreads];
   const int lane = threadIdx.x & (t.lanes - 1);
-  const int64_t tile = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / t.lanes;
+  const int64_t tile = (int64_t(blockIdx.x) * kSumThreads + threadIdx.x) / t.lanes;
   const int64_t begin = tile * t.tile;
   if (begin >= t.n) return;
   const int end = int(min(int64_t(t.n), begin + t.tile));
   const int vectors = t.dim / S::kVec;
   const int first = blockIdx.y * t.lanes * S::kBlocks + lane;
+  const int vocab = int(t.vocab);
   const int before = begin > 0 ? __ldg(sid + begin - 1) : -1;
-  const int after = end < t.n ? __ldg(sid + end) : -1;
+
+  // Keys and rows of a batch; positions behind the tile or without a table row have row -1.
+  int next_key[S::kBatch], next_row[S::kBatch];
+  auto load_places = [&](int p0) {
+#pragma unroll
+    for (int u = 0; u < S::kBatch; ++u) {
+      next_key[u] = p0 + u < end ? __ldg(sid + p0 + u) : vocab;
+      next_row[u] = p0 + u < end ? __ldg(perm + p0 + u) : -1;
+    }
+  };
+  auto fetch_batch = [&](int stage) {
+#pragma unroll
+    for (int u = 0; u < S::kBatch; ++u) {
+      if (next_key[u] < vocab) {
+        const T* row = g + int64_t(next_row[u]) * t.dim;
+#pragma unroll
+        for (int b = 0; b < S::kBlocks; ++b) {
+          const int i = first + b * t.lanes;
+          if (i < vectors) fetch<T, BYTES>(&ring[stage][u][b][threadIdx.x], row + int64_t(i) * S::kVec);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int p_load = int(begin);
+#pragma unroll
+  for (int st = 0; st < S::kStages - 1; ++st) {
+    load_places(p_load);
+    fetch_batch(st);
+    p_load += S::kBatch;
+  }
+  load_places(p_load);
+
   int run = __ldg(sid + begin);
   bool from_left = before == run;
   Sum<T> acc[S::kColumns];
 #pragma unroll
   for (int k = 0; k < S::kColumns; ++k) acc[k].clear();
-  for (int p0 = int(begin); p0 < end; p0 += S::kInFlight) {
-    int key[S::kInFlight];
-    int row[S::kInFlight];
-    Chunk<T, BYTES> c[S::kInFlight][S::kBlocks];
+  int stage = 0, load_stage = S::kStages - 1;
+  for (int p0 = int(begin); p0 < end && run < vocab; p0 += S::kBatch) {
+    fetch_batch(load_stage);
+    p_load += S::kBatch;
+    load_places(p_load);
+    load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+#pragma unroll 1
+    for (int u = 0; u < S::kBatch && p0 + u < end; ++u) {
+      const int key = __ldg(sid + p0 + u);
+      if (key != run) {  // the run before this position ends inside the tile
+        if (from_left) store_slot<T, BYTES>(t, 2 * tile, first, acc);
+        else store_row<T, BYTES>(t, g_weight, run, first, acc);
 #pragma unroll
-    for (int u = 0; u < S::kInFlight; ++u) {
-      key[u] = p0 + u < end ? __ldg(sid + p0 + u) : INT_MAX;
-      row[u] = p0 + u < end ? __ldg(perm + p0 + u) : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < S::kInFlight; ++u) {
+        for (int k = 0; k < S::kColumns; ++k) acc[k].clear();
+        run = key;
+        from_left = false;
+        if (run >= vocab) break;
+      }
 #pragma unroll
       for (int b = 0; b < S::kBlocks; ++b) {
-        const int i = first + b * t.lanes;
-        if (key[u] < t.vocab && i < vectors) c[u][b] = load_chunk_once<T, BYTES>(g + int64_t(row[u]) * t.dim + i * S::kVec);
+        const Access c = ring[stage][u][b][threadIdx.x];
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) acc[b * S::kVec + e].add(widen<T>(c.v[e]));
       }
     }
-#pragma unroll
-    for (int u = 0; u < S::kInFlight; ++u) {
-      if (p0 + u < end) {
-        if (key[u] != run) {  // the run before this position ends inside the tile
-          if (run < t.vocab) {
-            if (from_left) store_slot<T, BYTES>(t, 2 * tile, first, acc);
-            else store_row<T, BYTES>(t, g_weight, run, first, acc);
-          }
-#pragma unroll
-          for (int k = 0; k < S::kColumns; ++k) acc[k].clear();
-          run = key[u];
-          from_left = false;
-        }
-        if (run < t.vocab) {
-#pragma unroll
-          for (int b = 0; b < S::kBlocks; ++b)
-#pragma unroll
-            for (int e = 0; e < S::kVec; ++e) acc[b * S::kVec + e].add(widen<T>(c[u][b].v[e]));
-        }
-      }
-    }
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
   }
-  if (run >= t.vocab) return;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (run >= vocab) return;
   if (from_left) store_slot<T, BYTES>(t, 2 * tile, first, acc);
-  else if (after == run) store_slot<T, BYTES>(t, 2 * tile + 1, first, acc);
+  else if (end < t.n && __ldg(sid + end) == run) store_slot<T, BYTES>(t, 2 * tile + 1, first, acc);
   else store_row<T, BYTES>(t, g_weight, run, first, acc);
 }
 
 // Runs that cross tile boundaries.  One group of lanes per (boundary, chunk); only the first
 // boundary of a run has work.  Runs of more than kShortChain tiles are added by the whole CTA.
 constexpr int kShortChain = 8;
+constexpr int kJoinThreads = 128;
 
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kJoinThreads)
 join_runs_kernel(const int32_t* __restrict__ sid, Tiles t, T* __restrict__ g_weight) {
   using S = Shape<T, BYTES>;
-  __shared__ float s_part[kThreads * S::kColumns * Sum<T>::kPlanes];
-  __shared__ int64_t s_long[kThreads];  // boundary of the long run that a group met, or -1
-  const int lane = threadIdx.x & (t.lanes - 1), group = threadIdx.x / t.lanes, groups = kThreads / t.lanes;
-  const int64_t tiles = (int64_t(t.n) + t.tile - 1) / t.tile;
-  const int64_t boundary = int64_t(blockIdx.x) * groups + group + 1;  // between tiles boundary - 1 and boundary
+  __shared__ float s_part[kJoinThreads * S::kColumns * Sum<T>::kPlanes];
+  __shared__ int s_long[kJoinThreads], s_longs;  // boundaries where a long run begins
+  const int lane = threadIdx.x & (t.lanes - 1), group = threadIdx.x / t.lanes, groups = kJoinThreads / t.lanes;
+  const int tiles = int((int64_t(t.n) + t.tile - 1) / t.tile);
+  const int boundary = int(blockIdx.x) * groups + group + 1;  // between tiles boundary - 1 and boundary
   const int first = blockIdx.y * t.lanes * S::kBlocks + lane;
+  if (threadIdx.x == 0) s_longs = 0;
+  __syncthreads();
+  auto key_at = [&](int64_t tile) { return __ldg(sid + tile * t.tile); };
   Sum<T> acc[S::kColumns];
-  bool starts = false, is_long = false;
-  int v = 0;
-  if (boundary < tiles) {
-    const int64_t p = boundary * t.tile;
-    v = __ldg(sid + p);
-    starts = v < t.vocab && __ldg(sid + p - 1) == v && !(p - t.tile > 0 && __ldg(sid + p - t.tile - 1) == v);
-    is_long = starts && boundary + kShortChain < tiles && __ldg(sid + p + int64_t(kShortChain) * t.tile) == v;
-  }
-  if (lane == 0) s_long[group] = is_long ? boundary : -1;
-  if (starts && !is_long) {
 #pragma unroll
-    for (int k = 0; k < S::kColumns; ++k) acc[k].clear();
-    add_slot<T, BYTES>(t, 2 * (boundary - 1) + 1, first, acc);
-    for (int64_t b = boundary; b < tiles && __ldg(sid + b * t.tile) == v; ++b) add_slot<T, BYTES>(t, 2 * b, first, acc);
-    store_row<T, BYTES>(t, g_weight, v, first, acc);
-  }
-  if (!__syncthreads_or(is_long)) return;
-  for (int q = 0; q < groups; ++q) {
-    const int64_t b0 = s_long[q];
-    if (b0 < 0) continue;
-    const int u = __ldg(sid + b0 * t.tile);
-    int64_t lo = b0, hi = tiles;  // tiles lo .. hi - 1: the run reaches lo, not hi
-    while (hi - lo > 1) {
-      const int64_t mid = lo + (hi - lo) / 2;
-      if (__ldg(sid + mid * t.tile) == u) lo = mid; else hi = mid;
+  for (int k = 0; k < S::kColumns; ++k) acc[k].clear();
+  if (boundary < tiles) {
+    const int64_t p = int64_t(boundary) * t.tile;
+    const int v = __ldg(sid + p), left = __ldg(sid + p - 1);
+    const int before = p > t.tile ? __ldg(sid + p - t.tile - 1) : -1;
+    int more = 0;  // tiles behind this one that the run reaches, up to kShortChain
+#pragma unroll
+    for (int k = 1; k <= kShortChain; ++k) more += boundary + k < tiles && key_at(boundary + k) == v;
+    if (v < t.vocab && left == v && before != v) {
+      if (more == kShortChain) {
+        if (lane == 0) s_long[atomicAdd(&s_longs, 1)] = boundary;
+      } else {
+        add_slot<T, BYTES>(t, 2 * int64_t(boundary - 1) + 1, first, acc);
+        for (int k = 0; k <= more; ++k) add_slot<T, BYTES>(t, 2 * int64_t(boundary + k), first, acc);
+        store_row<T, BYTES>(t, g_weight, v, first, acc);
+      }
     }
-    // group k adds an even, consecutive share of the run's parts; the shares are then added in order
+  }
+  __syncthreads();
+  const int longs = s_longs;
+  for (int q = 0; q < longs; ++q) {  // in any order: each is a row of its own
+    const int b0 = s_long[q];
+    const int u = key_at(b0);
+    int64_t lo = b0, hi = tiles;  // the run reaches tile lo, not hi
+    while (hi - lo > 1) {         // kJoinThreads probes at a time
+      const int64_t step = (hi - lo + kJoinThreads - 1) / kJoinThreads, at = lo + step * (threadIdx.x + 1);
+      const int reached = __syncthreads_count(at < hi && key_at(at) == u);
+      hi = min(hi, lo + step * (reached + 1));
+      lo += step * reached;
+    }
+    // group k adds an even, consecutive share of the run's parts; the shares are added pairwise
     const int64_t count = hi - b0, from = b0 + count * group / groups, to = b0 + count * (group + 1) / groups;
 #pragma unroll
     for (int k = 0; k < S::kColumns; ++k) acc[k].clear();
-    if (group == 0) add_slot<T, BYTES>(t, 2 * (b0 - 1) + 1, first, acc);
+    if (group == 0) add_slot<T, BYTES>(t, 2 * int64_t(b0 - 1) + 1, first, acc);
 #pragma unroll 4
     for (int64_t b = from; b < to; ++b) add_slot<T, BYTES>(t, 2 * b, first, acc);
+    for (int half = groups / 2; half > 0; half /= 2) {
+      if (group >= half && group < 2 * half) {
 #pragma unroll
-    for (int k = 0; k < S::kColumns; ++k) {
-      s_part[k * kThreads + threadIdx.x] = acc[k].s;
-      if constexpr (Sum<T>::kExact) s_part[(S::kColumns + k) * kThreads + threadIdx.x] = acc[k].c;
-    }
-    __syncthreads();
-    if (group == 0) {
-      for (int o = 1; o < groups; ++o) {
+        for (int k = 0; k < S::kColumns; ++k) {
+          s_part[k * kJoinThreads + threadIdx.x] = acc[k].s;
+          if constexpr (Sum<T>::kExact) s_part[(S::kColumns + k) * kJoinThreads + threadIdx.x] = acc[k].c;
+        }
+      }
+      __syncthreads();
+      if (group < half) {
+        const int other = threadIdx.x + half * t.lanes;
 #pragma unroll
         for (int k = 0; k < S::kColumns; ++k) {
           Sum<T> part;
-          part.s = s_part[k * kThreads + o * t.lanes + lane];
+          part.s = s_part[k * kJoinThreads + other];
           part.c = 0.f;
-          if constexpr (Sum<T>::kExact) part.c = s_part[(S::kColumns + k) * kThreads + o * t.lanes + lane];
+          if constexpr (Sum<T>::kExact) part.c = s_part[(S::kColumns + k) * kJoinThreads + other];
           acc[k].add(part);
         }
       }
-      store_row<T, BYTES>(t, g_weight, u, first, acc);
+      __syncthreads();
     }
-    __syncthreads();
+    if (group == 0) store_row<T, BYTES>(t, g_weight, u, first, acc);
   }
 }
 
 // ---- launches --------------------------------------------------------------------------------
 
-// Positions of a tile: 128 where that still gives every warp slot of the GPU (148 SMs x 32) a tile,
-// less for fewer tokens, down to 8.  Larger tiles mean fewer partial sums through HBM (two fp32
-// rows per tile), smaller ones more rows in flight.
-inline int tile_positions(int64_t n, int64_t groups_per_row) {
+// Positions of a tile: 128 where that still gives some 380 threads per SM a tile, less for fewer
+// tokens or narrower rows, down to 8.  Larger tiles mean fewer partial sums through HBM (up to two
+// fp32 rows per tile), smaller ones more rows in flight.
+inline int tile_positions(int64_t n, int dim) {
+  const int64_t threads = ceil_div(dim, 8);  // eight values per lane
   int tile = 128;
-  while (tile > 8 && ceil_div(n, tile) * groups_per_row < 148 * 32) tile /= 2;
+  while (tile > 8 && ceil_div(n, tile) * threads < 148 * 384) tile /= 2;
   return tile;
 }
 
@@ -508,7 +599,6 @@ struct Workspace {
   int tile;
 };
 
-// A chunk of columns is 256 values (32 lanes of eight); the slots hold whole rows.
 Workspace carve(void* ws, int64_t n, int dim, int dtype) {
   Workspace w;
   const uintptr_t base = align_up(reinterpret_cast<uintptr_t>(ws), 256);
@@ -516,7 +606,7 @@ Workspace carve(void* ws, int64_t n, int dim, int dtype) {
   const bool on_chip = n <= kMaxSorted;
   size_t at = 0;
   auto take = [&](size_t bytes) { void* p = reinterpret_cast<void*>(base + at); at += align_up(bytes, 256); return p; };
-  w.tile = tile_positions(n, ceil_div(dim, 256));
+  w.tile = tile_positions(n, dim);
   w.sid = static_cast<int32_t*>(take(rows));
   w.perm = static_cast<int32_t*>(take(rows));
   w.keys = static_cast<int32_t*>(take(on_chip ? 0 : rows));
@@ -606,12 +696,13 @@ int launch_sums(const T* g, const Workspace& w, int64_t n, int64_t vocab, int di
   t.slots = w.slots;
   t.slot_words = int64_t(dim) * Sum<T>::kPlanes;
   const int64_t tiles = ceil_div(n, w.tile);
-  const dim3 grid(unsigned(ceil_div(tiles, kThreads / t.lanes)), unsigned(ceil_div(vectors, t.lanes * S::kBlocks)));
+  static_assert(kSumThreads == kJoinThreads, "one grid for both kernels");
+  const dim3 grid(unsigned(ceil_div(tiles, kSumThreads / t.lanes)), unsigned(ceil_div(vectors, t.lanes * S::kBlocks)));
   if (grid.y > 65535u) return fail(TEXB_ERR_UNSUPPORTED, "embedding: rows of %d values are too wide", dim);
-  sum_tiles_kernel<T, BYTES><<<grid, kThreads, 0, stream>>>(g, w.sid, w.perm, t, g_weight);
+  sum_tiles_kernel<T, BYTES><<<grid, kSumThreads, 0, stream>>>(g, w.sid, w.perm, t, g_weight);
   const int st = check_launch("sum_tiles_kernel");
   if (st != TEXB_OK || tiles == 1) return st;
-  join_runs_kernel<T, BYTES><<<grid, kThreads, 0, stream>>>(w.sid, t, g_weight);
+  join_runs_kernel<T, BYTES><<<grid, kJoinThreads, 0, stream>>>(w.sid, t, g_weight);
   return check_launch("join_runs_kernel");
 }
 
