@@ -216,4 +216,7 @@ def test_gradient_only_where_it_is_wanted():
         embedding(tok, w.detach().double())
     with pytest.raises(RuntimeError, match="CUDAtensor"):
         embedding(tok, torch.zeros(4, 4))
-    assert math.isfinite(float(embedding(tok, w).sum()))
+    out = embedding(tok, w).sum()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out, w, create_graph=True)
+    assert math.isfinite(out.item())

@@ -26,6 +26,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "embedding.cuh"
 
 namespace cg = cooperative_groups;
@@ -50,11 +52,20 @@ __device__ __forceinline__ uint32_t key_of(IdT token, int64_t vocab, int64_t pad
 
 // ---- clearing rows ------------------------------------------------------------------------
 
-// Row v of a table of rows of `row_words` words of type W, cleared by `lanes` lanes.
+// Row v of a table of rows of `row_words` words of type W, cleared by `lanes` lanes: 16 bytes at a time
+// between the words in front of the first 16-byte boundary and those behind the last.
 template <typename W>
 __device__ __forceinline__ void clear_row(W* table, int64_t v, int64_t row_words, int lane, int lanes) {
   W* row = table + v * row_words;
-  for (int64_t i = lane; i < row_words; i += lanes) row[i] = W{};
+  constexpr int kPer = 16 / int(sizeof(W));
+  const int64_t head = min(row_words, int64_t((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int64_t(sizeof(W)));
+  const int64_t wide = (row_words - head) / kPer;
+  uint4* body = reinterpret_cast<uint4*>(row + head);
+  for (int64_t i = lane; i < wide; i += lanes) body[i] = uint4{};
+  if constexpr (kPer > 1) {
+    for (int64_t i = lane; i < head; i += lanes) row[i] = W{};
+    for (int64_t i = head + wide * kPer + lane; i < row_words; i += lanes) row[i] = W{};
+  }
 }
 
 // ---- sort of up to 131 072 tokens, and the zero rows, in one launch ------------------------------
@@ -105,27 +116,41 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = int(cluster.num_blocks());
 
-  if (int(blockIdx.x) >= ranks) {  // ---- clear: an even share of the table's rows
+  if (int(blockIdx.x) >= ranks) {
+    // ---- clear: every cluster has an even share of the table's rows, every CTA of it a part of the
+    // share.  The CTAs divide the tokens, and mark those of the share in the memory of the CTA that has
+    // the row (each CTA reading all tokens took 30 us for 131 072).
+    constexpr int kScan = 8;
     uint32_t* marks = reinterpret_cast<uint32_t*>(smem);
-    const int64_t workers = int64_t(gridDim.x) - ranks, worker = int64_t(blockIdx.x) - ranks;
-    const int64_t end = vocab * (worker + 1) / workers;
-    for (int64_t lo = vocab * worker / workers; lo < end; lo += kMarkBits) {
-      const int64_t hi = min(end, lo + kMarkBits);
-      for (int i = threadIdx.x; i < int((hi - lo + 31) / 32); i += kSortThreads) marks[i] = 0u;
-      __syncthreads();
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n; i += kSortThreads) {
-        const int64_t key = key_of<IdT>(tokens[i], vocab, padding, false);
-        if (key >= lo && key < hi) {
-          // a frequent token is marked once, not by a queue of atomics on one word
-          volatile uint32_t* word = &marks[(key - lo) >> 5];
-          const uint32_t bit = 1u << ((key - lo) & 31);
-          if (!(*word & bit)) atomicOr(&marks[(key - lo) >> 5], bit);
+    const int64_t shares = gridDim.x / ranks - 1, which = blockIdx.x / ranks - 1;
+    const int me = int(cluster.block_rank());
+    const int64_t end = vocab * (which + 1) / shares;
+    for (int64_t lo = vocab * which / shares; lo < end; lo += ranks * kMarkBits) {
+      const int64_t hi = min(end, lo + ranks * kMarkBits);
+      const int64_t part = (hi - lo + ranks - 1) / ranks;  // rows of a CTA, at most kMarkBits
+      for (int i = threadIdx.x; i < int((part + 31) / 32); i += kSortThreads) marks[i] = 0u;
+      cluster.sync();
+      for (int i0 = me * kSortThreads + threadIdx.x; i0 < n; i0 += ranks * kSortThreads * kScan) {
+        IdT token[kScan];  // all loads of a batch before the first mark
+#pragma unroll
+        for (int k = 0; k < kScan; ++k)
+          if (i0 + k * ranks * kSortThreads < n) token[k] = __ldg(tokens + i0 + k * ranks * kSortThreads);
+#pragma unroll
+        for (int k = 0; k < kScan; ++k) {
+          if (i0 + k * ranks * kSortThreads >= n) break;
+          const int64_t key = key_of<IdT>(token[k], vocab, padding, false);
+          if (key >= lo && key < hi) {
+            const int owner = int((key - lo) / part), place = int((key - lo) - owner * part);
+            volatile uint32_t* word = cluster.map_shared_rank(marks + (place >> 5), owner);
+            // a frequent token is marked once, not by a queue of atomics on one word
+            if (!(*word >> (place & 31) & 1u)) atomicOr(const_cast<uint32_t*>(word), 1u << (place & 31));
+          }
         }
       }
-      __syncthreads();
-      for (int64_t v = lo + threadIdx.x / lanes; v < hi; v += kSortThreads / lanes)
-        if (!(marks[(v - lo) >> 5] >> ((v - lo) & 31) & 1u)) clear_row(table, v, row_words, threadIdx.x & (lanes - 1), lanes);
+      cluster.sync();  // all marks are there; and, behind it, nobody touches another CTA's memory before the next round's first barrier
+      const int64_t first = lo + me * part, last = min(hi, first + part);
+      for (int64_t v = first + threadIdx.x / lanes; v < last; v += kSortThreads / lanes)
+        if (!(marks[(v - first) >> 5] >> ((v - first) & 31) & 1u)) clear_row(table, v, row_words, threadIdx.x & (lanes - 1), lanes);
       __syncthreads();
     }
     return;
@@ -165,10 +190,12 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
       if (k < items) {
         const bool valid = mine + k * 32 < share;
         const uint32_t d = (item[k].x >> shift) & (bins - 1);
-        uint32_t peers = __ballot_sync(0xffffffffu, valid);
-        for (int b = 0; b < digit_bits; ++b) {
-          const uint32_t ones = __ballot_sync(0xffffffffu, (d >> b) & 1u);
-          peers &= ((d >> b) & 1u) ? ones : ~ones;
+        uint32_t peers = __ballot_sync(0xffffffffu, valid);  // match.any took 1.6 times as long as nine ballots
+#pragma unroll
+        for (int b = 0; b < kMaxDigitBits; ++b) {
+          const bool one = (d >> b) & 1u;
+          const uint32_t ones = __ballot_sync(0xffffffffu, one);
+          peers &= one ? ones : ~ones;
         }
         uint32_t seen = 0u;
         if (valid) seen = counts[warp][d];
@@ -617,6 +644,31 @@ Workspace carve(void* ws, int64_t n, int dim, int dtype) {
   return w;
 }
 
+// Clusters of `ranks` CTAs of the kernel that fit the current device at once; asked once per device
+// and shape (the query takes longer than a launch).
+template <typename K>
+int resident_clusters(K kernel, const cudaLaunchConfig_t& cfg, int ranks, int items) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][kMaxCluster + 1][kMaxItems + 1];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) device = -1;
+  if (device >= 0) {
+    const int v = known[device][ranks][items].load(std::memory_order_relaxed);
+    if (v > 0) return v;
+  }
+  // the largest shared memory that any shape asks for: the attribute stays with the kernel
+  constexpr int kMost = SortLayout::kItems + kSortThreads * kMaxItems * int(sizeof(uint2));
+  static_assert(kMost >= kMarkBits / 8 + 8, "the marks fit as well");
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return 0;
+  int count = 0;
+  if (cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess || count < 2) {
+    (void)cudaGetLastError();
+    count = 2;
+  }
+  if (device >= 0) known[device][ranks][items].store(count, std::memory_order_relaxed);
+  return count;
+}
+
 template <typename IdT, typename W>
 int launch_sort_and_clear(const IdT* tokens, int64_t n, int64_t vocab, int64_t padding, const Workspace& w, W* table,
                           int64_t row_words, cudaStream_t stream) {
@@ -629,17 +681,12 @@ int launch_sort_and_clear(const IdT* tokens, int64_t n, int64_t vocab, int64_t p
   const int passes = n > 1 ? int(ceil_div(bits, kMaxDigitBits)) : 0;
   const int digit_bits = passes ? int(ceil_div(bits, passes)) : 1;
   const int lanes = lanes_of(row_words);
-  // clearing CTAs: at least 64 KB of table each, one per SM at most
-  int64_t workers = ceil_div(vocab * row_words * int64_t(sizeof(W)), 65536);
-  workers = workers < 1 ? 1 : workers > 148 - ranks ? 148 - ranks : workers;
   size_t smem = SortLayout::kItems + size_t(kSortThreads) * items * sizeof(uint2);
-  const size_t marks = size_t((ceil_div(vocab, workers) < kMarkBits ? ceil_div(vocab, workers) : kMarkBits) / 8 + 8);
+  const size_t marks = size_t((vocab < kMarkBits ? vocab : kMarkBits) / 8 + 8);
   if (smem < marks) smem = marks;
+  cudaError_t e = cudaSuccess;
   auto kernel = sort_and_clear_kernel<IdT, W>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "sort_and_clear_kernel: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(ranks + align_up(size_t(workers), size_t(ranks))));
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -649,6 +696,17 @@ int launch_sort_and_clear(const IdT* tokens, int64_t n, int64_t vocab, int64_t p
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  // Clearing CTAs: at least 64 KB of table each, and no more than run beside the sort at once -- a
+  // cluster that had to wait for a free one doubled the time (239 us instead of 105 for 0.7 GB).
+  int64_t workers = ceil_div(vocab * row_words * int64_t(sizeof(W)), 65536);
+  cfg.gridDim = dim3(unsigned(ranks) * 2);
+  const int clusters = resident_clusters(kernel, cfg, ranks, items);
+  if (clusters == 0) return check_launch("sort_and_clear_kernel");
+  const int64_t room = int64_t(clusters - 1) * ranks;
+  workers = workers < 1 ? 1 : workers;
+  workers = int64_t(align_up(size_t(workers), size_t(ranks)));
+  if (workers > room) workers = room;
+  cfg.gridDim = dim3(unsigned(ranks + workers));
   e = cudaLaunchKernelEx(&cfg, kernel, tokens, int(n), vocab, padding, items, digit_bits, passes, w.sid, w.perm, table,
                          row_words, lanes);
   if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "sort_and_clear_kernel: %s", cudaGetErrorString(e));

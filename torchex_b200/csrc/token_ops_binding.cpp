@@ -63,10 +63,37 @@ at::Tensor embedding_backward(const at::Tensor& tokens_in, const at::Tensor& g_i
   return out;
 }
 
+// The autograd node of the lookup.  Compiled: a node written in Python costs more host time per step
+// than the kernels of a small batch take.
+struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& weight,
+                            double scale, int64_t padding_idx) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = weight.dim() == 2 ? weight.size(0) : int64_t(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_idx"] = padding_idx;
+    return embedding_forward(tokens, weight, scale);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "embedding is differentiable once (create_graph is not supported)");
+    const auto saved = ctx->get_saved_variables();
+    return {at::Tensor(),
+            embedding_backward(saved[0], g[0], ctx->saved_data["vocab"].toInt(), ctx->saved_data["scale"].toDouble(),
+                               ctx->saved_data["padding_idx"].toInt()),
+            at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor embedding(const at::Tensor& tokens, const at::Tensor& weight, double scale, int64_t padding_idx) {
+  if (at::GradMode::is_enabled() && weight.requires_grad()) return EmbeddingNode::apply(tokens, weight, scale, padding_idx);
+  return embedding_forward(tokens, weight, scale);
+}
+
 }  // namespace
 
 void register_token_ops(py::module& m) {
-  m.def("embedding_forward", &embedding_forward, py::arg("tokens"), py::arg("weight"), py::arg("scale"));
+  m.def("embedding", &embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"), py::arg("padding_idx"));
   m.def("embedding_backward", &embedding_backward, py::arg("tokens"), py::arg("g"), py::arg("vocab"), py::arg("scale"),
         py::arg("padding_idx"));
 }

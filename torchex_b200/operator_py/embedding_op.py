@@ -8,25 +8,8 @@ The reference has no counterpart; its users call ``torch.nn.functional.embedding
 from __future__ import annotations
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from .. import scatter_ext as _ext
-
-
-class EmbeddingFunction(Function):
-
-    @staticmethod
-    def forward(ctx, tokens: torch.Tensor, weight: torch.Tensor, scale: float, padding_idx: int):
-        ctx.save_for_backward(tokens)
-        ctx.vocab, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
-        return _ext.embedding_forward(tokens, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        (tokens,) = ctx.saved_tensors
-        return None, _ext.embedding_backward(tokens, g, ctx.vocab, ctx.scale, ctx.padding_idx), None, None
 
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx=None) -> torch.Tensor:
@@ -47,6 +30,4 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
         if not -vocab <= padding_idx < vocab:
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {vocab} rows")
         pad = int(padding_idx) % vocab
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return EmbeddingFunction.apply(tokens, weight, float(scale), pad)
-    return _ext.embedding_forward(tokens, weight, float(scale))
+    return _ext.embedding(tokens, weight, float(scale), pad)

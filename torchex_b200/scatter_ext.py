@@ -50,7 +50,7 @@ reduce_sequence = getattr(native, "reduce_sequence", None)
 broadcast_back = native.broadcast_back
 mean_max_backward = native.mean_max_backward
 segment_rank = native.segment_rank
-embedding_forward = native.embedding_forward
+embedding = native.embedding
 embedding_backward = native.embedding_backward
 abi_version = native.abi_version
 
