@@ -433,6 +433,28 @@ int texb_embedding_backward(const void* tokens, int id_bytes, int64_t n, const v
                             int64_t vocab, int dim, float scale, int64_t padding_idx, void* g_weight,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the norm over many gradients ---------------------------------------------
+ * norm = sqrt(sum of the squares of all values of `count` tensors), and the tensors
+ * scaled by min(1, max_norm / (norm + 1e-6)): gradient clipping before an optimizer
+ * step.  No counterpart in the reference.
+ *   grads, sizes, dtypes: host arrays: device pointer, number of values (consecutive in
+ *     memory) and TEXB_FLOAT32 / _BFLOAT16 / _FLOAT16 of each tensor.  They are read
+ *     during the call only.
+ *   outs, out_dtypes: where each scaled tensor goes: its input itself (in place), or
+ *     memory that overlaps no input and no other output; in the input's dtype or fp32.
+ *     Tensors scaled in place are not touched when the coefficient is 1.
+ *   norm_out: device float.  Nothing synchronises.
+ * Squares are added in fp64 above groups of eight, so neither many values nor values
+ * whose squares leave fp32's range lose the result; a NaN makes the norm NaN and every
+ * output NaN, an infinity makes it infinite and the other outputs 0.  No atomics:
+ * bit-reproducible run to run.  The workspace is 8-byte aligned. */
+size_t texb_grad_norm_workspace_bytes(int count);
+int texb_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes,
+                   float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, const int* dtypes,
+                    void* const* outs, const int* out_dtypes, float max_norm, float* norm_out,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- peer buffers for the multi-GPU driver ---------------------------------------
  * One process per GPU; a caller that wants every GPU to hold the whole result of a
  * sharded reduction lets each GPU write its shard into a buffer the other processes

@@ -88,6 +88,11 @@ _SIGNATURES = {
     "texb_embedding_backward": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_int64,
                                            _c.c_int, _c.c_float, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_size_t,
                                            _c.c_void_p]),
+    "texb_grad_norm_workspace_bytes": (_c.c_size_t, [_c.c_int]),
+    "texb_grad_norm": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t,
+                                  _c.c_void_p]),
+    "texb_clip_grads": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_float,
+                                   _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
 }
 
 OP_SUM, OP_MEAN, OP_MAX = 0, 1, 2

@@ -31,7 +31,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libtexb_scatter.so")
 HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "texb_scatter.h")
 SOURCES = ["abi.cu", "segment_reduce.cu", "reduce_unit_sum.cu", "reduce_unit_sum_plain.cu", "reduce_unit_max.cu",
            "reduce_unit_sum_max.cu", "segment_small.cu", "segment_plan.cu", "segment_backward.cu", "peer_copy.cu",
-           "embedding.cu", "embedding_backward.cu"]
+           "embedding.cu", "embedding_backward.cu", "grad_clip.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

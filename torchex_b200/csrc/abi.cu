@@ -60,6 +60,10 @@ int embedding_forward_impl(const void*, int, int64_t, const void*, int, int64_t,
 size_t embedding_backward_workspace_bytes_impl(int64_t, int64_t, int);
 int embedding_backward_impl(const void*, int, int64_t, const void*, int, int64_t, int, float, int64_t, void*, void*,
                             size_t, cudaStream_t);
+size_t grad_norm_workspace_bytes_impl(int);
+int grad_norm_impl(int, const void* const*, const int64_t*, const int*, float*, void*, size_t, cudaStream_t);
+int clip_grads_impl(int, const void* const*, const int64_t*, const int*, void* const*, const int*, float, float*, void*,
+                    size_t, cudaStream_t);
 
 namespace {
 thread_local char t_error[512] = "";
@@ -413,6 +417,18 @@ int texb_embedding_backward(const void* tokens, int id_bytes, int64_t n, const v
                             size_t workspace_bytes, void* stream) {
   return embedding_backward_impl(tokens, id_bytes, n, g, dtype, vocab, dim, scale, padding_idx, g_weight, workspace,
                                  workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+size_t texb_grad_norm_workspace_bytes(int count) { return grad_norm_workspace_bytes_impl(count); }
+int texb_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, float* norm_out,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  return grad_norm_impl(count, grads, sizes, dtypes, norm_out, workspace, workspace_bytes,
+                        static_cast<cudaStream_t>(stream));
+}
+int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, void* const* outs,
+                    const int* out_dtypes, float max_norm, float* norm_out, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  return clip_grads_impl(count, grads, sizes, dtypes, outs, out_dtypes, max_norm, norm_out, workspace, workspace_bytes,
+                         static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

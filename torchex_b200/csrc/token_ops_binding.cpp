@@ -1,9 +1,12 @@
-// Binding of the token operators (table lookup and its gradient) of the module `scatter_ext`:
+// Binding of the table lookup with its gradient, and of gradient clipping, of the module `scatter_ext`:
 // tensors in, the C ABI of include/texb_scatter.h underneath.  Each call checks its arguments,
 // runs on its tensors' device and on torch's current stream, and takes outputs and scratch from
 // torch's caching allocator.
 
 #include "binding.h"
+
+#include <algorithm>
+#include <tuple>
 
 namespace texb_binding {
 namespace {
@@ -90,12 +93,109 @@ at::Tensor embedding(const at::Tensor& tokens, const at::Tensor& weight, double 
   return embedding_forward(tokens, weight, scale);
 }
 
+// ---- gradient clipping -----------------------------------------------------------------
+
+struct Tensors {  // the host arrays of the C ABI
+  std::vector<const void*> in;
+  std::vector<int64_t> sizes;
+  std::vector<int> dtypes;
+};
+
+Tensors gather(const std::vector<at::Tensor>& grads) {
+  Tensors r;
+  for (const at::Tensor& g : grads) {
+    TORCH_CHECK(g.layout() == at::kStrided, "gradients must be dense tensors, got a sparse one");
+    TORCH_CHECK(g.device().is_cuda(), "gradients must be CUDAtensors ");
+    TORCH_CHECK(g.device() == grads[0].device(), "gradients live on different devices");
+    TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradients must fill their memory without gaps or overlaps");
+    r.in.push_back(g.data_ptr());
+    r.sizes.push_back(g.numel());
+    r.dtypes.push_back(dtype_code(g, "gradients"));
+  }
+  return r;
+}
+
+at::Tensor grad_norm(const std::vector<at::Tensor>& grads) {
+  TORCH_CHECK(!grads.empty(), "grad_norm needs at least one tensor");
+  const Tensors t = gather(grads);
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  const at::Tensor ws = scratch(texb_grad_norm_workspace_bytes(int(grads.size())), norm);
+  check_status(texb_grad_norm(int(grads.size()), t.in.data(), t.sizes.data(), t.dtypes.data(), norm.data_ptr<float>(),
+                              ws.data_ptr(), size_t(ws.numel()), stream_of(norm)),
+               "texb_grad_norm");
+  return norm;
+}
+
+// Outputs may not overlap each other, nor an input other than their own.
+void check_apart(const Tensors& t, const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs) {
+  struct Range { uintptr_t begin, end; size_t index; };
+  std::vector<Range> ranges;
+  for (size_t i = 0; i < outs.size(); ++i) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(outs[i].data_ptr());
+    if (outs[i].numel() > 0) ranges.push_back({p, p + outs[i].nbytes(), i});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < ranges.size(); ++i)
+    TORCH_CHECK(ranges[i - 1].end <= ranges[i].begin, "tensors ", ranges[i - 1].index, " and ", ranges[i].index,
+                " would be written to overlapping memory (the same gradient twice?)");
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.in[i]), e = p + grads[i].nbytes();
+    if (p == e) continue;
+    auto at = std::partition_point(ranges.begin(), ranges.end(), [&](const Range& r) { return r.end <= p; });
+    for (; at != ranges.end() && at->begin < e; ++at)
+      TORCH_CHECK(at->index == i && at->begin == p, "output ", at->index, " overlaps gradient ", i);
+  }
+}
+
+std::tuple<std::vector<at::Tensor>, at::Tensor> clip_grads(const std::vector<at::Tensor>& grads, double max_norm,
+                                                           c10::optional<std::vector<at::Tensor>> given) {
+  TORCH_CHECK(!grads.empty(), "clip_grads needs at least one tensor");
+  TORCH_CHECK(max_norm >= 0, "max_norm must not be negative, got ", max_norm);
+  const Tensors t = gather(grads);
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  std::vector<at::Tensor> outs;
+  if (given.has_value()) {
+    outs = std::move(*given);
+    TORCH_CHECK(outs.size() == grads.size(), "out has ", outs.size(), " tensors for ", grads.size(), " gradients");
+    for (size_t i = 0; i < outs.size(); ++i) {
+      const at::Tensor &o = outs[i], &g = grads[i];
+      TORCH_CHECK(o.device() == g.device(), "out[", i, "] lives on another device than its gradient");
+      TORCH_CHECK(o.sizes() == g.sizes(), "out[", i, "] has another shape than its gradient");
+      TORCH_CHECK(o.layout() == at::kStrided && ((o.is_contiguous() && g.is_contiguous()) || o.strides() == g.strides()),
+                  "out[", i, "] has other strides than its gradient");
+      TORCH_CHECK(o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat,
+                  "out[", i, "] must have the dtype of its gradient or float32");
+    }
+    check_apart(t, grads, outs);
+  } else {
+    for (const at::Tensor& g : grads) outs.push_back(at::empty_like(g));
+  }
+  std::vector<void*> out;
+  std::vector<int> out_dtypes;
+  for (const at::Tensor& o : outs) {
+    out.push_back(o.data_ptr());
+    out_dtypes.push_back(dtype_code(o, "out"));
+  }
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  const at::Tensor ws = scratch(texb_grad_norm_workspace_bytes(int(grads.size())), norm);
+  check_status(texb_clip_grads(int(grads.size()), t.in.data(), t.sizes.data(), t.dtypes.data(), out.data(),
+                               out_dtypes.data(), float(max_norm), norm.data_ptr<float>(), ws.data_ptr(),
+                               size_t(ws.numel()), stream_of(norm)),
+               "texb_clip_grads");
+  if (given.has_value())
+    for (const at::Tensor& o : outs) torch::autograd::impl::bump_version(o);
+  return {outs, norm};
+}
+
 }  // namespace
 
 void register_token_ops(py::module& m) {
   m.def("embedding", &embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"), py::arg("padding_idx"));
   m.def("embedding_backward", &embedding_backward, py::arg("tokens"), py::arg("g"), py::arg("vocab"), py::arg("scale"),
         py::arg("padding_idx"));
+  m.def("grad_norm", &grad_norm, py::arg("grads"));
+  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("max_norm"), py::arg("out") = c10::nullopt);
 }
 
 }  // namespace texb_binding

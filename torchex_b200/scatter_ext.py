@@ -52,6 +52,8 @@ mean_max_backward = native.mean_max_backward
 segment_rank = native.segment_rank
 embedding = native.embedding
 embedding_backward = native.embedding_backward
+grad_norm = native.grad_norm
+clip_grads = native.clip_grads
 abi_version = native.abi_version
 
 
