@@ -4,8 +4,8 @@
 // Bound by HBM: the norm reads every value once, the scaling reads them again and writes them.
 // A list is one launch per pass, whatever the number and sizes of its tensors: pointers and sizes
 // travel in the kernel's parameters (no copy to the device, so the call can be captured in a
-// graph), the tensors are cut into chunks of 16 384 values, and one resident wave of CTAs walks
-// the chunks.  The second pass walks them from the last to the first, so that what the first pass
+// graph), the tensors are cut into chunks of 16 KB, and one resident wave of CTAs walks the
+// chunks with 64 bytes of loads in flight per thread.  The second pass walks them from the last to the first, so that what the first pass
 // read last still comes from L2, and stores past it; it reads the coefficient's partial sums itself,
 // which saves a launch, and leaves tensors that are scaled in place alone when the coefficient is 1.
 //
@@ -23,11 +23,14 @@
 namespace texb {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kGroup = 8;                            // values of one access
-constexpr int kSteps = 4;                            // accesses of a thread in flight
-constexpr int kChunk = kThreads * kGroup * kSteps;   // 16 384 values
-constexpr int kWave = 148 * 2;
+constexpr int kThreads = 256;
+constexpr int kGroup = 8;              // squares that are added in fp32
+constexpr int kInFlight = 64;          // bytes of loads of a thread before the first is used (128: larger chunks,
+                                       // an eighth slower for 100 M values, as the last chunks leave SMs idle)
+constexpr int kChunkBytes = kThreads * kInFlight;
+inline int64_t chunk_values(int dtype) { return kChunkBytes / dtype_bytes(dtype); }
+constexpr int kCtasPerSm = 4;
+constexpr int kWave = 148 * kCtasPerSm;
 
 // How a tensor is read and written: its types, and whether rows of eight values are aligned.
 constexpr int kTypeBits = 2;
@@ -59,30 +62,6 @@ __device__ __forceinline__ int tensor_of(const List<CAPACITY>& l, uint32_t chunk
   return lo;
 }
 
-// Eight values from p on, widened; `wide`: p is aligned to 16 bytes.
-template <typename T>
-__device__ __forceinline__ void load_group(const T* p, float (&v)[kGroup]) {
-  constexpr int kPer = 16 / int(sizeof(T));
-#pragma unroll
-  for (int h = 0; h < kGroup / kPer; ++h) {
-    const Chunk<T, 16> c = load_chunk<T, 16>(p + h * kPer);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[h * kPer + e] = widen<T>(c.v[e]);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store_group(T* p, const float (&v)[kGroup]) {
-  constexpr int kPer = 16 / int(sizeof(T));
-#pragma unroll
-  for (int h = 0; h < kGroup / kPer; ++h) {
-    Chunk<T, 16> c;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) c.v[e] = narrow<T>(v[h * kPer + e]);
-    store_chunk_once<T, 16>(p + h * kPer, c);
-  }
-}
-
 __device__ __forceinline__ void add_squares(const float (&v)[kGroup], double& sum) {
   float s = v[0] * v[0];
 #pragma unroll
@@ -99,29 +78,28 @@ __device__ __forceinline__ void add_squares(const float (&v)[kGroup], double& su
   for (int e = 0; e < kGroup; ++e) sum = fma(double(v[e]), double(v[e]), sum);
 }
 
+// `wide`: p is aligned to 16 bytes.  A full chunk is read 16 bytes per lane, neighbouring lanes side by side.
 template <typename T>
-__device__ __forceinline__ void square_chunk(const T* p, int64_t count, bool wide, double& sum) {
-  float v[kSteps][kGroup];
-  if (wide && count == kChunk) {
+__device__ __forceinline__ void square_chunk(const T* p, int count, bool wide, double& sum) {
+  constexpr int kPer = 16 / int(sizeof(T)), kLoads = kInFlight / 16, kLoadsPerGroup = kGroup / kPer;
+  float v[kGroup];
+  if (wide && count == kThreads * kLoads * kPer) {
+    Chunk<T, 16> c[kLoads];
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) load_group<T>(p + (k * kThreads + int(threadIdx.x)) * kGroup, v[k]);
+    for (int k = 0; k < kLoads; ++k) c[k] = load_chunk<T, 16>(p + (k * kThreads + int(threadIdx.x)) * kPer);
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) add_squares(v[k], sum);
+    for (int k = 0; k < kLoads; k += kLoadsPerGroup) {
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e) v[e] = widen<T>(c[k + e / kPer].v[e % kPer]);
+      add_squares(v, sum);
+    }
     return;
   }
-  int64_t done = 0;
-  if (wide) {
-    done = count / kGroup * kGroup;
-    for (int64_t i = int64_t(threadIdx.x) * kGroup; i < done; i += kThreads * kGroup) {
-      load_group<T>(p + i, v[0]);
-      add_squares(v[0], sum);
-    }
-  }
-  // values that no aligned access of eight covers: one per lane and access, eight in flight
-  for (int64_t i = done + threadIdx.x; i < count; i += kThreads * kGroup) {
+  // the end of a tensor, or one that begins anywhere: single values, eight in flight
+  for (int i = threadIdx.x; i < count; i += kThreads * kGroup) {
 #pragma unroll
-    for (int e = 0; e < kGroup; ++e) v[0][e] = i + e * kThreads < count ? widen<T>(p[i + e * kThreads]) : 0.f;
-    add_squares(v[0], sum);
+    for (int e = 0; e < kGroup; ++e) v[e] = i + e * kThreads < count ? widen<T>(__ldg(p + i + e * kThreads)) : 0.f;
+    add_squares(v, sum);
   }
 }
 
@@ -138,16 +116,18 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 template <int CAPACITY>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
 square_sums_kernel(const __grid_constant__ List<CAPACITY> list, double* __restrict__ partial) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   double sum = 0.0;
   for (uint32_t c = blockIdx.x; c < list.chunks; c += gridDim.x) {
     const int t = tensor_of(list, c);
-    const int64_t at = int64_t(c - (t > 0 ? list.chunk_end[t - 1] : 0u)) * kChunk;
-    const int64_t count = min(int64_t(kChunk), list.size[t] - at);
+    const int in = list.kind[t] & ((1 << kTypeBits) - 1);
+    const int chunk = kChunkBytes / (in == TEXB_FLOAT32 ? 4 : 2);
+    const int64_t at = int64_t(c - (t > 0 ? list.chunk_end[t - 1] : 0u)) * chunk;
+    const int count = int(min(int64_t(chunk), list.size[t] - at));
     const bool wide = list.kind[t] & kWide;
-    switch (list.kind[t] & ((1 << kTypeBits) - 1)) {
+    switch (in) {
       case TEXB_FLOAT32: square_chunk<float>(static_cast<const float*>(list.in[t]) + at, count, wide, sum); break;
       case TEXB_BFLOAT16: square_chunk<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(list.in[t]) + at, count, wide, sum); break;
       default: square_chunk<__half>(static_cast<const __half*>(list.in[t]) + at, count, wide, sum); break;
@@ -170,35 +150,39 @@ norm_kernel(const double* __restrict__ partial, int partials, float* __restrict_
   if (threadIdx.x == 0) norm_out[0] = norm;
 }
 
+// Loads and stores run over the same values per lane, at most 16 bytes of either: 16-bit values into fp32
+// ones are read 8 bytes per lane, so that neighbouring lanes store side by side (stores of 32 bytes per
+// lane as two halves took 517 us instead of 418 for 400 M values).
 template <typename In, typename Out>
-__device__ __forceinline__ void scale_chunk(const In* p, Out* q, int64_t count, bool wide, float coef) {
-  float v[kSteps][kGroup];
-  if (wide && count == kChunk) {
+__device__ __forceinline__ void scale_chunk(const In* p, Out* q, int count, bool wide, float coef) {
+  constexpr int kPer = 16 / int(sizeof(Out) > sizeof(In) ? sizeof(Out) : sizeof(In));
+  constexpr int kBytes = kPer * int(sizeof(In)), kLoads = kInFlight / kBytes;
+  if (wide && count == kThreads * kLoads * kPer) {
+    Chunk<In, kBytes> c[kLoads];
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) load_group<In>(p + (k * kThreads + int(threadIdx.x)) * kGroup, v[k]);
+    for (int k = 0; k < kLoads; ++k) c[k] = load_chunk_once<In, kBytes>(p + (k * kThreads + int(threadIdx.x)) * kPer);
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
+    for (int k = 0; k < kLoads; ++k) {
+      Chunk<Out, kPer * int(sizeof(Out))> o;
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e) v[k][e] *= coef;
-      store_group<Out>(q + (k * kThreads + int(threadIdx.x)) * kGroup, v[k]);
+      for (int e = 0; e < kPer; ++e) o.v[e] = narrow<Out>(widen<In>(c[k].v[e]) * coef);
+      store_chunk_once<Out, kPer * int(sizeof(Out))>(q + (k * kThreads + int(threadIdx.x)) * kPer, o);
     }
     return;
   }
-  int64_t done = 0;
-  if (wide) {
-    done = count / kGroup * kGroup;
-    for (int64_t i = int64_t(threadIdx.x) * kGroup; i < done; i += kThreads * kGroup) {
-      load_group<In>(p + i, v[0]);
+  for (int i = threadIdx.x; i < count; i += kThreads * kGroup) {
+    In v[kGroup];
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e) v[0][e] *= coef;
-      store_group<Out>(q + i, v[0]);
-    }
+    for (int e = 0; e < kGroup; ++e)
+      if (i + e * kThreads < count) v[e] = __ldcs(p + i + e * kThreads);
+#pragma unroll
+    for (int e = 0; e < kGroup; ++e)
+      if (i + e * kThreads < count) q[i + e * kThreads] = narrow<Out>(widen<In>(v[e]) * coef);
   }
-  for (int64_t i = done + threadIdx.x; i < count; i += kThreads) q[i] = narrow<Out>(widen<In>(p[i]) * coef);
 }
 
 template <int CAPACITY>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
 scale_kernel(const __grid_constant__ List<CAPACITY> list, const double* __restrict__ partial, int partials, float max_norm,
              float* __restrict__ norm_out) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -210,8 +194,10 @@ scale_kernel(const __grid_constant__ List<CAPACITY> list, const double* __restri
     const uint32_t c = list.chunks - 1 - k;
     const int t = tensor_of(list, c);
     if (coef == 1.f && list.in[t] == list.out[t]) continue;
-    const int64_t at = int64_t(c - (t > 0 ? list.chunk_end[t - 1] : 0u)) * kChunk;
-    const int64_t count = min(int64_t(kChunk), list.size[t] - at);
+    const int in = list.kind[t] & ((1 << kTypeBits) - 1);
+    const int chunk = kChunkBytes / (in == TEXB_FLOAT32 ? 4 : 2);
+    const int64_t at = int64_t(c - (t > 0 ? list.chunk_end[t - 1] : 0u)) * chunk;
+    const int count = int(min(int64_t(chunk), list.size[t] - at));
     const bool wide = list.kind[t] & kWide;
 #define TEXB_SCALE(In, Out) \
   scale_chunk<In, Out>(static_cast<const In*>(list.in[t]) + at, static_cast<Out*>(list.out[t]) + at, count, wide, coef)
@@ -264,7 +250,7 @@ int fill(const Request& r, int first, List<CAPACITY>& l) {
   int i = first;
   for (; i < r.count && l.count < CAPACITY; ++i) {
     if (r.sizes[i] == 0) continue;
-    const int64_t chunks = ceil_div(r.sizes[i], kChunk);
+    const int64_t chunks = ceil_div(r.sizes[i], chunk_values(r.dtypes[i]));
     if (int64_t(l.chunks) + chunks > INT_MAX) break;
     const int out_dtype = r.out ? r.out_dtypes[i] : r.dtypes[i];
     void* out = r.out ? r.out[i] : nullptr;
@@ -311,8 +297,8 @@ int check(const Request& r, const float* norm_out, const void* workspace, size_t
     return fail(TEXB_ERR_INVALID_ARGUMENT, "grad_norm: NULL pointer");
   for (int i = 0; i < r.count; ++i) {
     if (r.sizes[i] < 0) return fail(TEXB_ERR_INVALID_ARGUMENT, "grad_norm: tensor %d has a negative size", i);
-    if (r.sizes[i] / kChunk >= INT_MAX) return fail(TEXB_ERR_UNSUPPORTED, "grad_norm: tensor %d is too large", i);
     if (!dtype_known(r.dtypes[i])) return fail(TEXB_ERR_INVALID_ARGUMENT, "grad_norm: tensor %d has an unknown dtype", i);
+    if (r.sizes[i] / chunk_values(r.dtypes[i]) >= INT_MAX) return fail(TEXB_ERR_UNSUPPORTED, "grad_norm: tensor %d is too large", i);
     if (r.sizes[i] > 0 && !r.in[i]) return fail(TEXB_ERR_INVALID_ARGUMENT, "grad_norm: tensor %d is NULL", i);
     if (!r.out) continue;
     if (r.sizes[i] > 0 && !r.out[i]) return fail(TEXB_ERR_INVALID_ARGUMENT, "clip_grads: output %d is NULL", i);
