@@ -455,6 +455,43 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
                     void* const* outs, const int* out_dtypes, float max_norm, float* norm_out,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention within segments -------------------------------------------------
+ * Softmax attention of every row over the rows of its own segment: the regions of a
+ * sparse point transformer, or documents packed into one batch, with the plan that
+ * the reductions use.  No counterpart in the reference.
+ *   x_ij = scale * q_i.k_j, then softcap * tanh(x_ij / softcap) where softcap > 0, then
+ *          minus slopes[head] * |i - j| where slopes is given (i, j: places within the
+ *          segment, in increasing row order);
+ *   out_i = sum_j softmax_j(x_ij) v_j over the rows j of i's segment, up to i if causal.
+ * Query heads share key / value heads in consecutive groups of heads / kv_heads.
+ * Scores, softmax statistics and sums are fp32; probabilities and the gradients of
+ * scores are rounded to the tensors' type before they are multiplied.  A row that a query
+ * does not see has no influence on it, whatever it holds (NaN and infinities included).
+ * No atomics: bit-reproducible run to run.  Nothing synchronises.
+ *   Limits: TEXB_BFLOAT16 or TEXB_FLOAT16; dim a multiple of 8 up to 128; pointers and
+ *   strides (in values) such that rows start on 16-byte boundaries; heads a multiple of
+ *   kv_heads; n < 2^31 - 65536. */
+typedef struct texb_attention_problem {
+  const void *q, *k, *v;           /* [n, heads, dim], [n, kv_heads, dim] twice */
+  int64_t q_strides[2], k_strides[2], v_strides[2]; /* values from row to row, from head to head */
+  int dtype;
+  const int32_t *sid, *perm, *offsets; /* the plan: texb_plan_build (perm NULL: rows in segment order) */
+  int64_t n, num_segments;
+  int64_t max_count;               /* rows of the largest segment, -1 if not known */
+  int heads, kv_heads, dim;
+  float scale, softcap;
+  const float* slopes;             /* device [heads], or NULL */
+  int causal;
+  void* out;                       /* [n, heads, dim], contiguous: written by forward, read by backward */
+  float* lse;                      /* [heads, n]: written by forward (NULL: not wanted), read by backward */
+  const void* g;                   /* backward: gradient of out */
+  int64_t g_strides[2];
+  void *g_q, *g_k, *g_v;           /* backward: contiguous gradients, every row written */
+} texb_attention_problem;
+size_t texb_attention_workspace_bytes(int64_t n, int heads, int kv_heads, int backward);
+int texb_attention_forward(const texb_attention_problem* problem, void* workspace, size_t workspace_bytes, void* stream);
+int texb_attention_backward(const texb_attention_problem* problem, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- peer buffers for the multi-GPU driver ---------------------------------------
  * One process per GPU; a caller that wants every GPU to hold the whole result of a
  * sharded reduction lets each GPU write its shard into a buffer the other processes

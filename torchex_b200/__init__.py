@@ -6,8 +6,8 @@ sm_100a kernels behind a C ABI (``include/texb_scatter.h``).
 """
 from .operator_py import (ScatterData, TorchTimer, clip_grad_norm_, clip_grads, embedding, gather_back, getPreSum,
                           grad_norm, ingroup_inds, ingroup_rank, scatter_max, scatter_mean, scatter_mean_max,
-                          scatter_multi, scatter_sum)
+                          scatter_multi, scatter_sum, segment_attention)
 
 __all__ = ["ScatterData", "TorchTimer", "getPreSum", "scatter_max", "scatter_mean", "scatter_sum",
            "ingroup_inds", "ingroup_rank", "gather_back", "scatter_mean_max", "scatter_multi",
-           "embedding", "grad_norm", "clip_grads", "clip_grad_norm_"]
+           "embedding", "grad_norm", "clip_grads", "clip_grad_norm_", "segment_attention"]

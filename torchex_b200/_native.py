@@ -16,6 +16,18 @@ _c = ctypes
 _lock = threading.Lock()
 _lib = None
 
+class AttentionProblem(_c.Structure):
+    """``texb_attention_problem`` of the C ABI."""
+
+    _fields_ = [("q", _c.c_void_p), ("k", _c.c_void_p), ("v", _c.c_void_p), ("q_strides", _c.c_int64 * 2),
+                ("k_strides", _c.c_int64 * 2), ("v_strides", _c.c_int64 * 2), ("dtype", _c.c_int),
+                ("sid", _c.c_void_p), ("perm", _c.c_void_p), ("offsets", _c.c_void_p), ("n", _c.c_int64),
+                ("num_segments", _c.c_int64), ("max_count", _c.c_int64), ("heads", _c.c_int), ("kv_heads", _c.c_int),
+                ("dim", _c.c_int), ("scale", _c.c_float), ("softcap", _c.c_float), ("slopes", _c.c_void_p),
+                ("causal", _c.c_int), ("out", _c.c_void_p), ("lse", _c.c_void_p), ("g", _c.c_void_p),
+                ("g_strides", _c.c_int64 * 2), ("g_q", _c.c_void_p), ("g_k", _c.c_void_p), ("g_v", _c.c_void_p)]
+
+
 _SIGNATURES = {
     # name: (restype, argtypes)
     "texb_version": (_c.c_int, []),
@@ -93,6 +105,9 @@ _SIGNATURES = {
                                   _c.c_void_p]),
     "texb_clip_grads": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_float,
                                    _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "texb_attention_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int, _c.c_int, _c.c_int]),
+    "texb_attention_forward": (_c.c_int, [_c.POINTER(AttentionProblem), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "texb_attention_backward": (_c.c_int, [_c.POINTER(AttentionProblem), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
 }
 
 OP_SUM, OP_MEAN, OP_MAX = 0, 1, 2

@@ -31,13 +31,14 @@ LIB_PATH = os.path.join(LIB_DIR, "libtexb_scatter.so")
 HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "texb_scatter.h")
 SOURCES = ["abi.cu", "segment_reduce.cu", "reduce_unit_sum.cu", "reduce_unit_sum_plain.cu", "reduce_unit_max.cu",
            "reduce_unit_sum_max.cu", "segment_small.cu", "segment_plan.cu", "segment_backward.cu", "peer_copy.cu",
-           "embedding.cu", "embedding_backward.cu", "grad_clip.cu"]
+           "embedding.cu", "embedding_backward.cu", "grad_clip.cu", "attention.cu",
+           *(f"attention_{way}_{dim}.cu" for way in ("forward", "backward") for dim in (16, 32, 64, 128))]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
 ]
 EXT_NAME = "scatter_ext"
-EXT_SOURCES = [os.path.join(CSRC, f) for f in ("scatter_ext_binding.cpp", "token_ops_binding.cpp")]
+EXT_SOURCES = [os.path.join(CSRC, f) for f in ("scatter_ext_binding.cpp", "token_ops_binding.cpp", "attention_binding.cpp")]
 EXT_HEADER = os.path.join(CSRC, "binding.h")
 EXT_PATH = os.path.join(LIB_DIR, EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 

@@ -64,6 +64,9 @@ size_t grad_norm_workspace_bytes_impl(int);
 int grad_norm_impl(int, const void* const*, const int64_t*, const int*, float*, void*, size_t, cudaStream_t);
 int clip_grads_impl(int, const void* const*, const int64_t*, const int*, void* const*, const int*, float, float*, void*,
                     size_t, cudaStream_t);
+size_t attention_workspace_bytes_impl(int64_t, int, int, int);
+int attention_forward_impl(const texb_attention_problem*, void*, size_t, cudaStream_t);
+int attention_backward_impl(const texb_attention_problem*, void*, size_t, cudaStream_t);
 
 namespace {
 thread_local char t_error[512] = "";
@@ -429,6 +432,15 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
                     void* stream) {
   return clip_grads_impl(count, grads, sizes, dtypes, outs, out_dtypes, max_norm, norm_out, workspace, workspace_bytes,
                          static_cast<cudaStream_t>(stream));
+}
+size_t texb_attention_workspace_bytes(int64_t n, int heads, int kv_heads, int backward) {
+  return attention_workspace_bytes_impl(n, heads, kv_heads, backward);
+}
+int texb_attention_forward(const texb_attention_problem* problem, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_forward_impl(problem, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+int texb_attention_backward(const texb_attention_problem* problem, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_backward_impl(problem, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,205 @@
+// Attention within segments: argument checks, workspaces, the pass that looks rows over, and the choice
+// of kernel.  The kernels are in attention_forward.cuh and attention_backward.cuh.
+
+#include "attention.cuh"
+
+namespace texb {
+namespace attention {
+
+template <int DP> int forward_by_type(const Problem&, int, bool, cudaStream_t);
+template <int DP> int backward_by_type(const Problem&, int, bool, cudaStream_t);
+
+namespace {
+
+// Flags the blocks of kBlock positions that hold a value that is not finite.  One CTA per (block, head).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) flag_values_kernel(const __grid_constant__ Problem a, uint8_t* __restrict__ flags) {
+  const int pos0 = blockIdx.x * kBlock;
+  const bool bad = look_over<T>(a, a.v, blockIdx.y, pos0, min(a.n, pos0 + kBlock));
+  if (threadIdx.x == 0) flags[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = bad;
+}
+
+// delta_i = g_i . o_i for the backward pass, and the flags of its blocks: of the queries or gradients of
+// a head (blockIdx.y < heads), or of the keys of a kv head.  Bound by HBM: q, g, o and k are read once.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+prepare_backward_kernel(const __grid_constant__ Problem a, float* __restrict__ delta,
+                        uint8_t* __restrict__ bad_q, uint8_t* __restrict__ bad_k) {
+  const int pos0 = blockIdx.x * kBlock, end = min(a.n, pos0 + kBlock), y = blockIdx.y;
+  if (y >= a.heads) {
+    const int kv = y - a.heads;
+    const bool bad = look_over<T>(a, a.k, kv, pos0, end);
+    if (threadIdx.x == 0) bad_k[int64_t(kv) * gridDim.x + blockIdx.x] = bad;
+    return;
+  }
+  // lanes of a group walk a row: 1, 2, 4, 8 or 16 of them, by the pieces of a row
+  const int pieces = a.dim / 8;
+  int lanes = 1;
+  while (lanes < pieces && lanes < 16) lanes *= 2;
+  const int sub = threadIdx.x & (lanes - 1);
+  bool bad = false;
+  for (int r = threadIdx.x / lanes; r < kBlock; r += kThreads / lanes) {
+    const int pos = pos0 + r;
+    float sum = 0.f;
+    if (pos < end && sub < pieces) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(row_at<T>(a, a.q, y, pos) + sub * 8));
+      const Chunk<T, 16> g = load_chunk<T, 16>(row_at<T>(a, a.g, y, pos) + sub * 8);
+      const Chunk<T, 16> o = load_chunk<T, 16>(row_at<T>(a, a.out, y, pos) + sub * 8);
+      bad |= not_finite<T>(q) || not_finite<T>(reinterpret_cast<const uint4&>(g));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(widen<T>(g.v[e]), widen<T>(o.v[e]), sum);
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (pos < end && sub == 0) delta[int64_t(y) * a.n + pos] = sum;
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) bad_q[int64_t(y) * gridDim.x + blockIdx.x] = bad;
+}
+
+int check(const Problem& a, int dtype, bool backward) {
+  if (dtype != TEXB_BFLOAT16 && dtype != TEXB_FLOAT16)
+    return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: bf16 or fp16 only (dtype %d)", dtype);
+  if (a.n < 0 || a.segments < 0 || a.heads < 1 || a.kv_heads < 1 || a.dim < 1)
+    return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: bad sizes");
+  if (a.heads % a.kv_heads != 0)
+    return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: %d heads do not share %d key/value heads evenly", a.heads, a.kv_heads);
+  if (a.dim % 8 != 0 || a.dim > 128)
+    return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: head dimension %d is not a multiple of 8 up to 128", a.dim);
+  if (a.heads + a.kv_heads > 65535) return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: too many heads");
+  if (!(a.cap >= 0.f) || !(a.scale == a.scale)) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: bad scale or softcap");
+  if (a.n == 0) return TEXB_OK;
+  if (!a.sid || !a.offsets || a.segments == 0) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: NULL plan");
+  const View* views[] = {&a.q, &a.k, &a.v, &a.out, &a.g, &a.gq, &a.gk, &a.gv};
+  for (int i = 0; i < (backward ? 8 : 4); ++i) {
+    if (!views[i]->p) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: NULL pointer");
+    if (reinterpret_cast<uintptr_t>(views[i]->p) % 16 != 0 || views[i]->row % 8 != 0 || views[i]->head % 8 != 0)
+      return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: rows must be 16-byte aligned");
+  }
+  if (backward && !a.lse) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: the backward pass needs lse");
+  return TEXB_OK;
+}
+
+inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kBlock)); }
+
+// Segments short enough that a tile looks at the values of its keys itself instead of a pass of its own
+// doing it: at most three tiles of keys.
+constexpr int kShortSegment = 64;
+
+}  // namespace
+}  // namespace attention
+
+size_t attention_workspace_bytes_impl(int64_t n, int heads, int kv_heads, int backward) {
+  if (n < 0 || heads < 1 || kv_heads < 1) return 0;
+  const size_t blocks = attention::blocks_of(n);
+  size_t bytes = align_up(blocks * size_t(kv_heads), 256) + 256;
+  if (backward) bytes += align_up(blocks * size_t(heads), 256) + align_up(size_t(n) * size_t(heads) * sizeof(float), 256);
+  return bytes;
+}
+
+namespace attention {
+namespace {
+
+View view_of(const void* p, const int64_t* strides) {
+  return {const_cast<void*>(p), strides ? strides[0] : 0, strides ? strides[1] : 0};
+}
+
+Problem problem_of(const texb_attention_problem& t) {
+  Problem a = {};
+  a.q = view_of(t.q, t.q_strides);
+  a.k = view_of(t.k, t.k_strides);
+  a.v = view_of(t.v, t.v_strides);
+  const int64_t rows[2] = {int64_t(t.heads) * t.dim, t.dim}, kv_rows[2] = {int64_t(t.kv_heads) * t.dim, t.dim};
+  a.out = view_of(t.out, rows);
+  a.g = view_of(t.g, t.g_strides);
+  a.gq = view_of(t.g_q, rows);
+  a.gk = view_of(t.g_k, kv_rows);
+  a.gv = view_of(t.g_v, kv_rows);
+  a.sid = t.sid;
+  a.perm = t.perm;
+  a.offsets = t.offsets;
+  a.slopes = t.slopes;
+  a.n = int(t.n);
+  a.segments = int(t.num_segments);
+  a.heads = t.heads;
+  a.kv_heads = t.kv_heads;
+  a.dim = t.dim;
+  a.causal = t.causal;
+  a.scale = t.scale;
+  a.cap = t.softcap;
+  a.lse = t.lse;
+  return a;
+}
+
+int check_problem(const texb_attention_problem* t) {
+  if (!t) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: NULL problem");
+  if (t->n > INT_MAX - 65536 || t->num_segments > INT_MAX - 65536)
+    return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: n and num_segments must be below 2^31 - 65536");
+  if (t->n < 0 || t->num_segments < 0) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: negative size");
+  return TEXB_OK;
+}
+
+}  // namespace
+}  // namespace attention
+
+int attention_forward_impl(const texb_attention_problem* t, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using namespace attention;
+  int st = check_problem(t);
+  if (st != TEXB_OK) return st;
+  Problem a = problem_of(*t);
+  const int dtype = t->dtype;
+  st = check(a, dtype, false);
+  if (st != TEXB_OK || a.n == 0) return st;
+  a.bad_v = nullptr;
+  if (t->max_count < 0 || t->max_count > kShortSegment) {
+    const size_t need = attention_workspace_bytes_impl(a.n, a.heads, a.kv_heads, 0);
+    if (!workspace || workspace_bytes < need)
+      return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", need, workspace_bytes);
+    uint8_t* flags = static_cast<uint8_t*>(workspace);
+    const dim3 grid(unsigned(blocks_of(a.n)), unsigned(a.kv_heads));
+    if (dtype == TEXB_BFLOAT16) flag_values_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a, flags);
+    else flag_values_kernel<__half><<<grid, kThreads, 0, stream>>>(a, flags);
+    st = check_launch("attention flag_values_kernel");
+    if (st != TEXB_OK) return st;
+    a.bad_v = flags;
+  }
+  const bool general = a.cap > 0.f || a.slopes != nullptr;
+  if (a.dim <= 16) return forward_by_type<16>(a, dtype, general, stream);
+  if (a.dim <= 32) return forward_by_type<32>(a, dtype, general, stream);
+  if (a.dim <= 64) return forward_by_type<64>(a, dtype, general, stream);
+  return forward_by_type<128>(a, dtype, general, stream);
+}
+
+int attention_backward_impl(const texb_attention_problem* t, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using namespace attention;
+  int st = check_problem(t);
+  if (st != TEXB_OK) return st;
+  Problem a = problem_of(*t);
+  const int dtype = t->dtype;
+  st = check(a, dtype, true);
+  if (st != TEXB_OK || a.n == 0) return st;
+  const size_t need = attention_workspace_bytes_impl(a.n, a.heads, a.kv_heads, 1);
+  const uintptr_t base = align_up(reinterpret_cast<uintptr_t>(workspace), 256);
+  if (!workspace || workspace_bytes < need)
+    return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", need, workspace_bytes);
+  const size_t blocks = blocks_of(a.n);
+  float* delta = reinterpret_cast<float*>(base);
+  uint8_t* bad_q = reinterpret_cast<uint8_t*>(base + align_up(size_t(a.n) * size_t(a.heads) * sizeof(float), 256));
+  uint8_t* bad_k = bad_q + align_up(blocks * size_t(a.heads), 256);
+  a.delta = delta;
+  a.bad_q = bad_q;
+  a.bad_k = bad_k;
+  const dim3 grid(unsigned(blocks), unsigned(a.heads + a.kv_heads));
+  if (dtype == TEXB_BFLOAT16)
+    prepare_backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a, delta, bad_q, bad_k);
+  else
+    prepare_backward_kernel<__half><<<grid, kThreads, 0, stream>>>(a, delta, bad_q, bad_k);
+  st = check_launch("attention prepare_backward_kernel");
+  if (st != TEXB_OK) return st;
+  const bool general = a.cap > 0.f || a.slopes != nullptr;
+  if (a.dim <= 16) return backward_by_type<16>(a, dtype, general, stream);
+  if (a.dim <= 32) return backward_by_type<32>(a, dtype, general, stream);
+  if (a.dim <= 64) return backward_by_type<64>(a, dtype, general, stream);
+  return backward_by_type<128>(a, dtype, general, stream);
+}
+
+}  // namespace texb

@@ -1,0 +1,435 @@
+// Softmax attention within segments: what the forward and the backward kernels share.
+//
+// Rows are walked in segment-sorted order (positions): position p is row perm[p] (or p) of the tensors
+// and belongs to segment sid[p], whose positions are offsets[s] .. offsets[s + 1].  A query position i
+// sees the keys begin(i) <= j < end(i): those of its segment, up to itself if causal.  A CTA owns a
+// tile of consecutive positions, whichever segments they belong to, so that a tile of many short
+// segments costs one tile; the mask is two comparisons per score against the row's bounds.
+//
+//   x_ij = scale q_i.k_j, capped: cap tanh(x / cap), minus slope_h |i - j|
+//   p_ij = exp(x_ij - lse_i),  lse_i = log sum_j exp(x_ij),  o_i = sum_j p_ij v_j
+//
+// A product with a masked probability is 0 only if the other factor is finite.  The matrix
+// instructions add up whole tiles, so a NaN or an infinity in a row that a query must not see would
+// reach its result.  Rows are therefore looked over first (blocks of kBlock positions are flagged), and
+// a tile whose rows meet a flagged block is computed by the plain loops at the end of this file,
+// which touch visible rows only.
+#pragma once
+
+#include <climits>
+
+#include "vector_io.cuh"
+
+namespace texb {
+namespace attention {
+
+constexpr int kBlock = 64;  // positions of a tile, and of a flag
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Rows of 16-bit values of several heads; strides in values, the head dimension is contiguous.
+struct View {
+  void* p;
+  int64_t row, head;
+};
+
+struct Problem {
+  View q, k, v;              // [n, heads, dim], [n, kv_heads, dim] twice
+  const int32_t *sid, *perm, *offsets;
+  const float* slopes;       // [heads] or NULL
+  int n, segments, heads, kv_heads, dim;
+  int causal;
+  float scale, cap;          // cap 0: none
+  // forward
+  View out;
+  float* lse;                // [heads, n] by position, in units of log2; forward may leave it out
+  // backward
+  View g;                    // gradient of out
+  const float* delta;        // [heads, n] by position: g_i . o_i
+  View gq, gk, gv;
+  // flags of blocks with a value that is not finite, [.., ceil(n / kBlock)]; NULL: look for oneself
+  const uint8_t *bad_v, *bad_k;  // per kv head
+  const uint8_t* bad_q;          // per head: in q or g
+};
+
+__device__ __forceinline__ int row_of(const Problem& a, int pos) {
+  const int r = a.perm ? __ldg(a.perm + pos) : pos;
+  return min(max(r, 0), a.n - 1);  // a corrupt plan reads a wrong row, not memory that is not there
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_at(const Problem& a, const View& x, int head, int pos) {
+  return static_cast<T*>(x.p) + row_of(a, pos) * x.row + head * x.head;
+}
+
+struct Bounds { int begin, end; };
+__device__ __forceinline__ Bounds segment_of(const Problem& a, int pos) {
+  const int s = min(max(__ldg(a.sid + pos), 0), a.segments - 1);
+  return {max(0, __ldg(a.offsets + s)), min(a.n, __ldg(a.offsets + s + 1))};
+}
+// keys that a query sees, and queries that see a key; empty for positions behind the last row
+__device__ __forceinline__ Bounds keys_of(const Problem& a, int pos) {
+  if (pos >= a.n) return {0, 0};
+  Bounds b = segment_of(a, pos);
+  if (a.causal) b.end = min(b.end, pos + 1);
+  return b;
+}
+__device__ __forceinline__ Bounds queries_of(const Problem& a, int pos) {
+  if (pos >= a.n) return {0, 0};
+  Bounds b = segment_of(a, pos);
+  if (a.causal) b.begin = max(b.begin, pos);
+  return b;
+}
+
+// The score in units of log2, from the plain product of a query and a key, and the derivative of the
+// score by scale * product.  exp(2y) of the tanh is infinite or 0 for large |y|: then tanh is +-1.
+struct Score { float x, slope; };
+template <bool GENERAL>
+__device__ __forceinline__ Score score_of(const Problem& a, float product, float bias_slope, int distance) {
+  if constexpr (!GENERAL) return {product * (a.scale * kLog2e), 1.f};
+  float x = product * a.scale, d = 1.f;
+  if (a.cap > 0.f) {
+    const float y = x * (1.f / a.cap);
+    const float t = 1.f - 2.f / (exp2f(y * (2.f * kLog2e)) + 1.f);
+    x = a.cap * t;
+    d = 1.f - t * t;
+  }
+  return {(x - bias_slope * float(abs(distance))) * kLog2e, d};
+}
+
+// ---- matrix instructions on 16-bit fragments -----------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes to shared memory; `bytes` 0 writes zeros and reads nothing
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A tile of rows of DP 16-bit values in shared memory (DP: the head dimension padded to 16, 32, 64 or
+// 128, columns behind it zero).  16-byte pieces are swizzled so that eight consecutive rows of one
+// column of pieces lie in different banks.
+template <int DP>
+struct Tile {
+  static constexpr int kPieces = DP / 8;
+  static constexpr int kRowBytes = DP * 2;
+  __device__ static __forceinline__ uint32_t at(int row, int piece) {
+    constexpr int kShift = DP == 16 ? 2 : DP == 32 ? 1 : 0;
+    constexpr int kMask = kPieces < 8 ? kPieces - 1 : 7;
+    return uint32_t(row * kRowBytes + ((piece ^ ((row >> kShift) & kMask)) << 4));
+  }
+};
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+
+// Copies rows [pos0, pos0 + ROWS) of head `head` into a tile; rows at or behind `end` become zeros.
+// The row numbers of the next tile are fetched ahead of it (`rows`), since they come through `perm`.
+template <int DP, int ROWS>
+struct Loader {
+  static constexpr int kPer = (ROWS * (DP / 8) + kThreads - 1) / kThreads;  // pieces of a thread
+  int rows[kPer];
+  __device__ __forceinline__ void look_up(const Problem& a, int pos0, int end) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int pos = pos0 + (threadIdx.x + i * kThreads) / (DP / 8);
+      rows[i] = pos < end ? row_of(a, pos) : -1;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void copy(const Problem& a, const View& x, int head, uint32_t to) const {
+    const T* base = static_cast<const T*>(x.p) + head * x.head;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = threadIdx.x + i * kThreads;
+      if (ROWS * (DP / 8) % kThreads != 0 && c >= ROWS * (DP / 8)) break;
+      const int row = c / (DP / 8), piece = c % (DP / 8);
+      const bool real = rows[i] >= 0 && piece * 8 < a.dim;
+      const T* from = base + (real ? rows[i] * x.row + piece * 8 : 0);
+      copy16(to + Tile<DP>::at(row, piece), from, real ? 16 : 0);
+    }
+  }
+};
+
+// A operand: rows row0 .. row0 + 15, columns 16 k .. 16 k + 15 of a tile.
+template <int DP>
+__device__ __forceinline__ void load_a(uint32_t (&r)[4], uint32_t tile, int row0, int k) {
+  const int lane = threadIdx.x & 31;
+  ldmatrix4(r, tile + Tile<DP>::at(row0 + (lane & 15), 2 * k + (lane >> 4)));
+}
+// B operand of a product over columns: rows row0 .. row0 + 15 (two n-tiles: r[0..1], r[2..3]), columns 16 k ...
+template <int DP>
+__device__ __forceinline__ void load_b(uint32_t (&r)[4], uint32_t tile, int row0, int k) {
+  const int lane = threadIdx.x & 31;
+  ldmatrix4(r, tile + Tile<DP>::at(row0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+}
+// B operand of a product over rows: rows row0 .. row0 + 15, columns 16 c .. 16 c + 15 (two n-tiles)
+template <int DP>
+__device__ __forceinline__ void load_bt(uint32_t (&r)[4], uint32_t tile, int row0, int c) {
+  const int lane = threadIdx.x & 31;
+  ldmatrix4t(r, tile + Tile<DP>::at(row0 + (lane & 15), 2 * c + (lane >> 4)));
+}
+
+// acc [16 x 8 NT] += A (rows a_row0 .. of tile a) times the transpose of NT * 8 rows of tile b
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void product_rows(float (&acc)[NT][4], uint32_t a, int a_row0, uint32_t b) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    uint32_t fa[4];
+    load_a<DP>(fa, a, a_row0, k);
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      uint32_t fb[4];
+      load_b<DP>(fb, b, t * 8, k);
+      mma16816<T>(acc[t], fa, fb[0], fb[1]);
+      mma16816<T>(acc[t + 1], fa, fb[2], fb[3]);
+    }
+  }
+}
+
+// acc [16 x DP] += P (16 x 8 NT, rounded to T) times NT * 8 rows of tile b
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void product_probabilities(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b) {
+#pragma unroll
+  for (int k = 0; k < NT / 2; ++k) {
+    const uint32_t fa[4] = {pack2<T>(p[2 * k][0], p[2 * k][1]), pack2<T>(p[2 * k][2], p[2 * k][3]),
+                            pack2<T>(p[2 * k + 1][0], p[2 * k + 1][1]), pack2<T>(p[2 * k + 1][2], p[2 * k + 1][3])};
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      uint32_t fb[4];
+      load_bt<DP>(fb, b, 16 * k, c);
+      mma16816<T>(acc[2 * c], fa, fb[0], fb[1]);
+      mma16816<T>(acc[2 * c + 1], fa, fb[2], fb[3]);
+    }
+  }
+}
+
+// Writes the warp's 16 x DP accumulators, times `factor` per row, to rows of a tensor, through the
+// warp's own 16 rows of a tile (16-byte stores; the tile's former contents are no longer needed).
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(const Problem& a, const View& x, int head, int pos0, const float (&acc)[DP / 8][4],
+                                           float factor0, float factor1, unsigned char* tile, int row0) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int t = 0; t < DP / 8; ++t) {
+    const int r = row0 + (lane >> 2);
+    *reinterpret_cast<uint32_t*>(tile + Tile<DP>::at(r, t) + (lane & 3) * 4) = pack2<T>(acc[t][0] * factor0, acc[t][1] * factor0);
+    *reinterpret_cast<uint32_t*>(tile + Tile<DP>::at(r + 8, t) + (lane & 3) * 4) = pack2<T>(acc[t][2] * factor1, acc[t][3] * factor1);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < (16 * (DP / 8) + 31) / 32; ++i) {
+    const int c = lane + i * 32;
+    const int r = c / (DP / 8), piece = c % (DP / 8), pos = pos0 + r;
+    if (r < 16 && pos < a.n && piece * 8 < a.dim) {
+      T* to = row_at<T>(a, x, head, pos) + piece * 8;
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(tile + Tile<DP>::at(row0 + r, piece));
+    }
+  }
+}
+
+// ---- values that are not finite ------------------------------------------------------------------
+
+// Whether one of eight 16-bit values is infinite or NaN: all bits of an exponent set.
+template <typename T> struct ExponentBits;
+template <> struct ExponentBits<__nv_bfloat16> { static constexpr uint32_t kMask = 0x7f80u; };
+template <> struct ExponentBits<__half> { static constexpr uint32_t kMask = 0x7c00u; };
+template <typename T>
+__device__ __forceinline__ bool not_finite(const uint4& v) {
+  constexpr uint32_t lo = ExponentBits<T>::kMask, hi = lo << 16;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & lo) == lo || (w[i] & hi) == hi;
+  return bad;
+}
+
+// Whether positions [begin, end) of head `head` hold one; called by the whole CTA.
+template <typename T>
+__device__ __forceinline__ bool look_over(const Problem& a, const View& x, int head, int begin, int end) {
+  const int pieces = a.dim / 8;
+  bool bad = false;
+  for (int c = threadIdx.x; c < (end - begin) * pieces; c += kThreads) {
+    const int pos = begin + c / pieces;
+    bad |= not_finite<T>(*reinterpret_cast<const uint4*>(row_at<T>(a, x, head, pos) + (c % pieces) * 8));
+  }
+  return __syncthreads_or(bad);
+}
+
+// Whether a flagged block meets positions [begin, end); called by the whole CTA.
+__device__ __forceinline__ bool any_flag(const Problem& a, const uint8_t* flags, int head, int begin, int end) {
+  const int blocks = (a.n + kBlock - 1) / kBlock;
+  bool bad = false;
+  for (int b = begin / kBlock + threadIdx.x; b * kBlock < end; b += kThreads) bad |= flags[int64_t(head) * blocks + b] != 0;
+  return __syncthreads_or(bad);
+}
+
+// ---- plain loops: only visible rows are touched ---------------------------------------------------
+// One warp per row.  32 rows of the other side at a time: a lane computes the product of one of them,
+// then the warp adds them up, each lane holding every 32nd column.
+
+constexpr int kColumns = 4;  // columns of a lane: dim <= 128
+
+template <typename T>
+__device__ __forceinline__ float dot(const T* x, const T* y, int dim) {
+  float s = 0.f;
+  for (int d = 0; d < dim; d += 8) {
+    const Chunk<T, 16> a = load_chunk<T, 16>(x + d), b = load_chunk<T, 16>(y + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(widen<T>(a.v[e]), widen<T>(b.v[e]), s);
+  }
+  return s;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+  for (int o = 16; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = (u > v || u != u) ? u : v;  // a NaN stays
+  }
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// acc += sum over the lanes k < count of w_k * row(j0 + k)
+template <typename T>
+__device__ __forceinline__ void add_weighted(const Problem& a, const View& x, int head, int j0, int count, float w,
+                                             float (&acc)[kColumns]) {
+  const int lane = threadIdx.x & 31;
+  for (int k = 0; k < count; ++k) {
+    const float wk = __shfl_sync(0xffffffffu, w, k);
+    const T* row = row_at<T>(a, x, head, j0 + k);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+      if (lane + 32 * c < a.dim) acc[c] = fmaf(wk, widen<T>(row[lane + 32 * c]), acc[c]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_columns(const Problem& a, const View& x, int head, int pos, const float (&acc)[kColumns],
+                                              float factor) {
+  const int lane = threadIdx.x & 31;
+  T* row = row_at<T>(a, x, head, pos);
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c)
+    if (lane + 32 * c < a.dim) row[lane + 32 * c] = narrow<T>(acc[c] * factor);
+}
+
+template <typename T>
+__device__ __noinline__ void plain_forward(const Problem& a, int pos0, int head) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = head / (a.heads / a.kv_heads);
+  const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
+  for (int i = pos0 + warp; i < min(a.n, pos0 + kBlock); i += kWarps) {
+    const Bounds see = keys_of(a, i);
+    const T* qi = row_at<T>(a, a.q, head, i);
+    float acc[kColumns] = {}, top = -INFINITY, sum = 0.f;
+    for (int j0 = see.begin; j0 < see.end; j0 += 32) {
+      const int j = j0 + lane;
+      const float x = j < see.end ? score_of<true>(a, dot<T>(qi, row_at<T>(a, a.k, kv, j), a.dim), slope, i - j).x : -INFINITY;
+      const float top_new = warp_max((x > top || x != x) ? x : top);
+      const float base = top_new == -INFINITY ? 0.f : top_new;  // infinitely low scores so far: weight 0, not NaN
+      const float w = j < see.end ? exp2f(x - base) : 0.f, shrink = top == -INFINITY ? 0.f : exp2f(top - base);
+      sum = sum * shrink + warp_sum(w);
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) acc[c] = top == -INFINITY ? 0.f : acc[c] * shrink;
+      add_weighted<T>(a, a.v, kv, j0, min(32, see.end - j0), w, acc);
+      top = top_new;
+    }
+    const bool none = see.end <= see.begin;
+    store_columns<T>(a, a.out, head, i, acc, none ? 0.f : 1.f / sum);
+    if (a.lse && lane == 0) a.lse[int64_t(head) * a.n + i] = none ? 0.f : top + log2f(sum);
+  }
+}
+
+struct Pair { float p, ds; };  // probability and gradient of scale * product
+template <typename T>
+__device__ __forceinline__ Pair pair_of(const Problem& a, const T* qi, const T* kj, const T* vj, const T* gi, int head, int i, int j,
+                                        float slope) {
+  const Score s = score_of<true>(a, dot<T>(qi, kj, a.dim), slope, i - j);
+  const float p = exp2f(s.x - a.lse[int64_t(head) * a.n + i]);
+  return {p, p * (dot<T>(gi, vj, a.dim) - a.delta[int64_t(head) * a.n + i]) * (s.slope * a.scale)};
+}
+
+template <typename T>
+__device__ __noinline__ void plain_query_gradient(const Problem& a, int pos0, int head) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = head / (a.heads / a.kv_heads);
+  const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
+  for (int i = pos0 + warp; i < min(a.n, pos0 + kBlock); i += kWarps) {
+    const Bounds see = keys_of(a, i);
+    const T *qi = row_at<T>(a, a.q, head, i), *gi = row_at<T>(a, a.g, head, i);
+    float acc[kColumns] = {};
+    for (int j0 = see.begin; j0 < see.end; j0 += 32) {
+      const int j = j0 + lane;
+      float w = 0.f;
+      if (j < see.end)
+        w = pair_of<T>(a, qi, row_at<T>(a, a.k, kv, j), row_at<T>(a, a.v, kv, j), gi, head, i, j, slope).ds;
+      add_weighted<T>(a, a.k, kv, j0, min(32, see.end - j0), w, acc);
+    }
+    store_columns<T>(a, a.gq, head, i, acc, 1.f);
+  }
+}
+
+template <typename T>
+__device__ __noinline__ void plain_key_gradients(const Problem& a, int pos0, int kv) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.kv_heads;
+  for (int j = pos0 + warp; j < min(a.n, pos0 + kBlock); j += kWarps) {
+    const Bounds seen = queries_of(a, j);
+    const T *kj = row_at<T>(a, a.k, kv, j), *vj = row_at<T>(a, a.v, kv, j);
+    float acc_k[kColumns] = {}, acc_v[kColumns] = {};
+    for (int head = kv * group; head < (kv + 1) * group; ++head) {
+      const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
+      for (int i0 = seen.begin; i0 < seen.end; i0 += 32) {
+        const int i = i0 + lane, count = min(32, seen.end - i0);
+        Pair w = {0.f, 0.f};
+        if (i < seen.end)
+          w = pair_of<T>(a, row_at<T>(a, a.q, head, i), kj, vj, row_at<T>(a, a.g, head, i), head, i, j, slope);
+        add_weighted<T>(a, a.g, head, i0, count, w.p, acc_v);
+        add_weighted<T>(a, a.q, head, i0, count, w.ds, acc_k);
+      }
+    }
+    store_columns<T>(a, a.gk, kv, j, acc_k, 1.f);
+    store_columns<T>(a, a.gv, kv, j, acc_v, 1.f);
+  }
+}
+
+}  // namespace attention
+}  // namespace texb

@@ -1,0 +1,232 @@
+// Backward kernels of the attention within segments; instantiated by the attention_backward_*.cu files.
+//
+// The probabilities are computed again from the scores and the log-sums of the forward pass.  Two
+// kernels, so that every gradient is summed by one CTA in a fixed order (no atomics, the same bits
+// every time), at the price of computing the scores twice:
+//   queries: as the forward kernel, 64 query positions of one head against the keys they see;
+//   keys   : 64 key positions of one kv head against the queries that see them, of all query heads
+//            that share it -- the gradient of a shared key or value is one sum.
+// With P and dS rounded to the inputs' type before their products (half a step each):
+//   dS = P (g v - delta) x (derivative of the capped score) x scale,  gq = dS k, gk = dS^T q, gv = P^T g.
+// A masked pair's dS is set to 0, not multiplied by 0: its g v may be infinite.
+#pragma once
+
+#include "attention.cuh"
+
+namespace texb {
+namespace attention {
+
+template <int DP>
+struct QueryMemory {
+  static constexpr int kTile = kBlock * DP * 2;
+  static constexpr int kQ = 0, kG = kTile, kK = 2 * kTile, kV = 4 * kTile;  // two stages of keys and values
+  static constexpr int kBytes = 6 * kTile;
+};
+
+template <typename T, int DP, bool GENERAL>
+__global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_constant__ Problem a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  using M = QueryMemory<DP>;
+  const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
+  const int pos0 = blockIdx.x * kBlock, last = min(a.n, pos0 + kBlock) - 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
+  if (any_flag(a, a.bad_k, kv, first_key, end_key)) {
+    plain_query_gradient<T>(a, pos0, head);
+    return;
+  }
+  const uint32_t base = smem_u32(smem);
+  Loader<DP, kBlock> loader;
+  loader.look_up(a, pos0, last + 1);
+  loader.template copy<T>(a, a.q, head, base + M::kQ);
+  loader.template copy<T>(a, a.g, head, base + M::kG);
+  loader.look_up(a, first_key, end_key);
+  loader.template copy<T>(a, a.k, kv, base + M::kK);
+  loader.template copy<T>(a, a.v, kv, base + M::kV);
+  commit_copies();
+  loader.look_up(a, first_key + kBlock, end_key);
+
+  const int row0 = warp * 16, i0 = pos0 + row0 + (lane >> 2), i1 = i0 + 8;
+  const Bounds see0 = keys_of(a, i0), see1 = keys_of(a, i1);
+  const int warp_begin = keys_of(a, pos0 + row0).begin, warp_last = min(last, pos0 + row0 + 15);
+  const int warp_end = pos0 + row0 <= last ? keys_of(a, warp_last).end : 0;
+  const float slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+  const int64_t place = int64_t(head) * a.n;
+  const float lse0 = i0 < a.n ? a.lse[place + i0] : 0.f, lse1 = i1 < a.n ? a.lse[place + i1] : 0.f;
+  const float delta0 = i0 < a.n ? a.delta[place + i0] : 0.f, delta1 = i1 < a.n ? a.delta[place + i1] : 0.f;
+
+  float gq[DP / 8][4] = {};
+  int stage = 0;
+  for (int j0 = first_key; j0 < end_key; j0 += kBlock) {
+    if (j0 + kBlock < end_key) {
+      loader.template copy<T>(a, a.k, kv, base + M::kK + (stage ^ 1) * M::kTile);
+      loader.template copy<T>(a, a.v, kv, base + M::kV + (stage ^ 1) * M::kTile);
+    }
+    commit_copies();
+    loader.look_up(a, j0 + 2 * kBlock, end_key);
+    wait_copies<1>();
+    __syncthreads();
+    if (j0 + kBlock > warp_begin && j0 < warp_end) {
+      constexpr int NT = kBlock / 8;
+      float s[NT][4] = {}, dp[NT][4] = {};
+      product_rows<T, DP, NT>(s, base + M::kQ, row0, base + M::kK + stage * M::kTile);
+      product_rows<T, DP, NT>(dp, base + M::kG, row0, base + M::kV + stage * M::kTile);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = j0 + t * 8 + (lane & 3) * 2 + e;
+          const Score x0 = score_of<GENERAL>(a, s[t][e], slope, i0 - j), x1 = score_of<GENERAL>(a, s[t][2 + e], slope, i1 - j);
+          const float d0 = exp2f(x0.x - lse0) * (dp[t][e] - delta0) * (x0.slope * a.scale);
+          const float d1 = exp2f(x1.x - lse1) * (dp[t][2 + e] - delta1) * (x1.slope * a.scale);
+          dp[t][e] = j >= see0.begin && j < see0.end ? d0 : 0.f;
+          dp[t][2 + e] = j >= see1.begin && j < see1.end ? d1 : 0.f;
+        }
+      }
+      product_probabilities<T, DP, NT>(gq, dp, base + M::kK + stage * M::kTile);
+    }
+    __syncthreads();
+    stage ^= 1;
+  }
+  wait_copies<0>();
+  __syncwarp();
+  store_rows<T, DP>(a, a.gq, head, pos0 + row0, gq, 1.f, 1.f, smem + M::kQ, row0);
+}
+
+// Queries per step of the key kernel: 32 for the widest rows, whose two accumulators of 64 registers
+// leave no room for more.
+template <int DP>
+struct KeyMemory {
+  static constexpr int kRows = DP == 128 ? 32 : 64;
+  static constexpr int kTile = kBlock * DP * 2, kStep = kRows * DP * 2;
+  static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile, kG = kQ + 2 * kStep;  // two stages of queries and gradients
+  static constexpr int kLse = kG + 2 * kStep, kDelta = kLse + 2 * kRows * 4;
+  static constexpr int kBytes = kDelta + 2 * kRows * 4;
+};
+
+template <typename T, int DP, bool GENERAL>
+__global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_constant__ Problem a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  using M = KeyMemory<DP>;
+  constexpr int R = M::kRows, NT = R / 8;
+  const int kv = blockIdx.y, group = a.heads / a.kv_heads;
+  const int pos0 = blockIdx.x * kBlock, last = min(a.n, pos0 + kBlock) - 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first_query = queries_of(a, pos0).begin, end_query = queries_of(a, last).end;
+  bool bad = false;
+  for (int head = kv * group; head < (kv + 1) * group; ++head) bad |= any_flag(a, a.bad_q, head, first_query, end_query);
+  if (bad) {
+    plain_key_gradients<T>(a, pos0, kv);
+    return;
+  }
+  const uint32_t base = smem_u32(smem);
+  {
+    Loader<DP, kBlock> keys;
+    keys.look_up(a, pos0, last + 1);
+    keys.template copy<T>(a, a.k, kv, base + M::kK);
+    keys.template copy<T>(a, a.v, kv, base + M::kV);
+  }
+  float* s_lse = reinterpret_cast<float*>(smem + M::kLse);
+  float* s_delta = reinterpret_cast<float*>(smem + M::kDelta);
+  Loader<DP, R> loader;
+  auto fetch = [&](int head, int q0, int stage) {
+    loader.template copy<T>(a, a.q, head, base + M::kQ + stage * M::kStep);
+    loader.template copy<T>(a, a.g, head, base + M::kG + stage * M::kStep);
+    for (int r = threadIdx.x; r < R; r += kThreads) {
+      const bool real = q0 + r < end_query;
+      const int64_t at = int64_t(head) * a.n + (real ? q0 + r : 0);
+      copy4(smem_u32(s_lse + stage * R + r), a.lse + at, real ? 4 : 0);
+      copy4(smem_u32(s_delta + stage * R + r), a.delta + at, real ? 4 : 0);
+    }
+  };
+  const int steps = (end_query - first_query + R - 1) / R, total = steps * group;
+  loader.look_up(a, first_query, end_query);
+  if (total > 0) fetch(kv * group, first_query, 0);
+  commit_copies();
+
+  const int row0 = warp * 16, j0 = pos0 + row0 + (lane >> 2), j1 = j0 + 8;
+  const Bounds seen0 = queries_of(a, j0), seen1 = queries_of(a, j1);
+  const int warp_begin = pos0 + row0 <= last ? queries_of(a, pos0 + row0).begin : INT_MAX;
+  const int warp_end = pos0 + row0 <= last ? queries_of(a, min(last, pos0 + row0 + 15)).end : 0;
+
+  float gk[DP / 8][4] = {}, gv[DP / 8][4] = {};
+  int stage = 0, head = kv * group, step = 0;
+  for (int it = 0; it < total; ++it) {
+    const int q0 = first_query + step * R;
+    int next_step = step + 1, next_head = head;
+    if (next_step == steps) {
+      next_step = 0;
+      ++next_head;
+    }
+    if (it + 1 < total) {
+      loader.look_up(a, first_query + next_step * R, end_query);
+      fetch(next_head, first_query + next_step * R, stage ^ 1);
+    }
+    commit_copies();
+    wait_copies<1>();
+    __syncthreads();
+    if (q0 + R > warp_begin && q0 < warp_end) {
+      const float slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+      const uint32_t tq = base + M::kQ + stage * M::kStep, tg = base + M::kG + stage * M::kStep;
+      float p[NT][4] = {}, ds[NT][4] = {};
+      product_rows<T, DP, NT>(p, base + M::kK, row0, tq);
+      product_rows<T, DP, NT>(ds, base + M::kV, row0, tg);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = t * 8 + (lane & 3) * 2 + e, i = q0 + r;
+          const float lse = s_lse[stage * R + r], delta = s_delta[stage * R + r];
+          const Score x0 = score_of<GENERAL>(a, p[t][e], slope, i - j0), x1 = score_of<GENERAL>(a, p[t][2 + e], slope, i - j1);
+          const bool on0 = i >= seen0.begin && i < seen0.end, on1 = i >= seen1.begin && i < seen1.end;
+          p[t][e] = on0 ? exp2f(x0.x - lse) : 0.f;
+          p[t][2 + e] = on1 ? exp2f(x1.x - lse) : 0.f;
+          ds[t][e] = on0 ? p[t][e] * (ds[t][e] - delta) * (x0.slope * a.scale) : 0.f;
+          ds[t][2 + e] = on1 ? p[t][2 + e] * (ds[t][2 + e] - delta) * (x1.slope * a.scale) : 0.f;
+        }
+      }
+      product_probabilities<T, DP, NT>(gv, p, tg);
+      product_probabilities<T, DP, NT>(gk, ds, tq);
+    }
+    __syncthreads();
+    stage ^= 1;
+    step = next_step;
+    head = next_head;
+  }
+  wait_copies<0>();
+  __syncthreads();  // the key tiles are written over below, by warps that read only their own rows of them
+  store_rows<T, DP>(a, a.gk, kv, pos0 + row0, gk, 1.f, 1.f, smem + M::kK, row0);
+  store_rows<T, DP>(a, a.gv, kv, pos0 + row0, gv, 1.f, 1.f, smem + M::kV, row0);
+}
+
+template <typename K>
+int prepare_kernel(K kernel, int bytes, const char* what) {
+  if (bytes <= 48 * 1024) return TEXB_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? TEXB_OK : fail(TEXB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+template <typename T, int DP, bool GENERAL>
+int launch_backward(const Problem& a, cudaStream_t stream) {
+  const unsigned tiles = unsigned((a.n + kBlock - 1) / kBlock);
+  auto queries = query_gradient_kernel<T, DP, GENERAL>;
+  auto keys = key_gradients_kernel<T, DP, GENERAL>;
+  int st = prepare_kernel(queries, QueryMemory<DP>::kBytes, "attention query_gradient_kernel");
+  if (st == TEXB_OK) st = prepare_kernel(keys, KeyMemory<DP>::kBytes, "attention key_gradients_kernel");
+  if (st != TEXB_OK) return st;
+  queries<<<dim3(tiles, unsigned(a.heads)), kThreads, QueryMemory<DP>::kBytes, stream>>>(a);
+  st = check_launch("attention query_gradient_kernel");
+  if (st != TEXB_OK) return st;
+  keys<<<dim3(tiles, unsigned(a.kv_heads)), kThreads, KeyMemory<DP>::kBytes, stream>>>(a);
+  return check_launch("attention key_gradients_kernel");
+}
+
+template <int DP>
+int backward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
+  if (dtype == TEXB_BFLOAT16)
+    return general ? launch_backward<__nv_bfloat16, DP, true>(a, stream) : launch_backward<__nv_bfloat16, DP, false>(a, stream);
+  return general ? launch_backward<__half, DP, true>(a, stream) : launch_backward<__half, DP, false>(a, stream);
+}
+
+}  // namespace attention
+}  // namespace texb

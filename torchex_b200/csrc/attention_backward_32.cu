@@ -1,0 +1,7 @@
+#include "attention_backward.cuh"
+
+namespace texb {
+namespace attention {
+template int backward_by_type<32>(const Problem&, int, bool, cudaStream_t);
+}  // namespace attention
+}  // namespace texb

@@ -1,0 +1,164 @@
+// Forward kernel of the attention within segments; instantiated by the attention_forward_*.cu files.
+//
+// A CTA of four warps owns 64 query positions of one head, 16 per warp, and walks the keys its rows
+// see in tiles of 64: scores, running maximum and sum (in units of log2), and the product with the
+// values stay in registers; keys and values are copied one tile ahead (cp.async, two stages).  A warp
+// passes over tiles that none of its 16 rows see, which is what keeps a tile of many short segments
+// cheap, and over the mask where all of its rows see the whole tile.  Probabilities are rounded to the
+// type of the values before the second product, which the matrix instructions require: half a step
+// of that type each (2^-8 for bf16), averaged over the keys.
+#pragma once
+
+#include "attention.cuh"
+
+namespace texb {
+namespace attention {
+
+template <typename T, int DP>
+struct ForwardMemory {
+  static constexpr int kQ = 0;
+  static constexpr int kTile = kBlock * DP * 2;
+  static constexpr int kK = kTile, kV = 3 * kTile;  // two stages each
+  static constexpr int kBytes = 5 * kTile;
+};
+
+template <typename T, int DP, bool GENERAL>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Problem a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  using M = ForwardMemory<T, DP>;
+  const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
+  const int pos0 = blockIdx.x * kBlock, last = min(a.n, pos0 + kBlock) - 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
+
+  const bool bad = a.bad_v ? any_flag(a, a.bad_v, kv, first_key, end_key)
+                           : look_over<T>(a, a.v, kv, first_key, end_key);
+  if (bad) {
+    plain_forward<T>(a, pos0, head);
+    return;
+  }
+
+  const uint32_t base = smem_u32(smem), sq = base + M::kQ;
+  Loader<DP, kBlock> loader;
+  loader.look_up(a, pos0, last + 1);
+  loader.template copy<T>(a, a.q, head, sq);
+  loader.look_up(a, first_key, end_key);
+  loader.template copy<T>(a, a.k, kv, base + M::kK);
+  loader.template copy<T>(a, a.v, kv, base + M::kV);
+  commit_copies();
+  loader.look_up(a, first_key + kBlock, end_key);
+
+  const int row0 = warp * 16, i0 = pos0 + row0 + (lane >> 2), i1 = i0 + 8;
+  const Bounds see0 = keys_of(a, i0), see1 = keys_of(a, i1);
+  // of the warp's rows: the first key and the end of what any of them sees, and of what all of them see
+  const int warp_begin = keys_of(a, pos0 + row0).begin, warp_last = min(last, pos0 + row0 + 15);
+  const Bounds tail = pos0 + row0 <= last ? keys_of(a, warp_last) : Bounds{0, 0};
+  const int warp_end = tail.end;
+  const int all_begin = tail.begin, all_end = pos0 + row0 + 15 <= last ? keys_of(a, pos0 + row0).end : 0;
+  const float slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+
+  float out[DP / 8][4] = {};
+  float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+  int stage = 0;
+  for (int j0 = first_key; j0 < end_key; j0 += kBlock) {
+    if (j0 + kBlock < end_key) {
+      loader.template copy<T>(a, a.k, kv, base + M::kK + (stage ^ 1) * M::kTile);
+      loader.template copy<T>(a, a.v, kv, base + M::kV + (stage ^ 1) * M::kTile);
+    }
+    commit_copies();
+    loader.look_up(a, j0 + 2 * kBlock, end_key);
+    wait_copies<1>();
+    __syncthreads();
+    if (j0 + kBlock > warp_begin && j0 < warp_end) {
+      constexpr int NT = kBlock / 8;
+      float s[NT][4] = {};
+      product_rows<T, DP, NT>(s, sq, row0, base + M::kK + stage * M::kTile);
+      const bool whole = j0 >= all_begin && j0 + kBlock <= all_end;
+      float top0_new = top0, top1_new = top1;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = j0 + t * 8 + (lane & 3) * 2 + e;
+          s[t][e] = score_of<GENERAL>(a, s[t][e], slope, i0 - j).x;
+          s[t][2 + e] = score_of<GENERAL>(a, s[t][2 + e], slope, i1 - j).x;
+          if (!whole) {
+            if (j < see0.begin || j >= see0.end) s[t][e] = -INFINITY;
+            if (j < see1.begin || j >= see1.end) s[t][2 + e] = -INFINITY;
+          }
+          top0_new = fmaxf(top0_new, s[t][e]);
+          top1_new = fmaxf(top1_new, s[t][2 + e]);
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top0_new = fmaxf(top0_new, __shfl_xor_sync(0xffffffffu, top0_new, o));
+        top1_new = fmaxf(top1_new, __shfl_xor_sync(0xffffffffu, top1_new, o));
+      }
+      // no visible key so far: subtract 0, so that the weights become 0 and not NaN
+      const float base0 = top0_new == -INFINITY ? 0.f : top0_new, base1 = top1_new == -INFINITY ? 0.f : top1_new;
+      const float shrink0 = exp2f(top0 - base0), shrink1 = exp2f(top1 - base1);
+      top0 = top0_new;
+      top1 = top1_new;
+      sum0 *= shrink0;
+      sum1 *= shrink1;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[t][e] = exp2f(s[t][e] - base0);
+          s[t][2 + e] = exp2f(s[t][2 + e] - base1);
+          sum0 += s[t][e];
+          sum1 += s[t][2 + e];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < DP / 8; ++t) {
+        out[t][0] *= shrink0;
+        out[t][1] *= shrink0;
+        out[t][2] *= shrink1;
+        out[t][3] *= shrink1;
+      }
+      product_probabilities<T, DP, NT>(out, s, base + M::kV + stage * M::kTile);
+    }
+    __syncthreads();
+    stage ^= 1;
+  }
+  wait_copies<0>();
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    sum0 += __shfl_xor_sync(0xffffffffu, sum0, o);
+    sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
+  }
+  // a row sees itself, so only rows behind the last position have an empty sum
+  const bool none0 = see0.end <= see0.begin, none1 = see1.end <= see1.begin;
+  if (a.lse && (lane & 3) == 0) {
+    if (i0 < a.n) a.lse[int64_t(head) * a.n + i0] = none0 ? 0.f : top0 + log2f(sum0);
+    if (i1 < a.n) a.lse[int64_t(head) * a.n + i1] = none1 ? 0.f : top1 + log2f(sum1);
+  }
+  store_rows<T, DP>(a, a.out, head, pos0 + row0, out, none0 ? 0.f : 1.f / sum0,
+                    none1 ? 0.f : 1.f / sum1, smem + M::kQ, row0);
+}
+
+template <typename T, int DP, bool GENERAL>
+int launch_forward(const Problem& a, cudaStream_t stream) {
+  auto kernel = forward_kernel<T, DP, GENERAL>;
+  constexpr int bytes = ForwardMemory<T, DP>::kBytes;
+  if (bytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "attention forward_kernel: %s", cudaGetErrorString(e));
+  }
+  const dim3 grid(unsigned((a.n + kBlock - 1) / kBlock), unsigned(a.heads));
+  kernel<<<grid, kThreads, bytes, stream>>>(a);
+  return check_launch("attention forward_kernel");
+}
+
+template <int DP>
+int forward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
+  if (dtype == TEXB_BFLOAT16)
+    return general ? launch_forward<__nv_bfloat16, DP, true>(a, stream) : launch_forward<__nv_bfloat16, DP, false>(a, stream);
+  return general ? launch_forward<__half, DP, true>(a, stream) : launch_forward<__half, DP, false>(a, stream);
+}
+
+}  // namespace attention
+}  // namespace texb

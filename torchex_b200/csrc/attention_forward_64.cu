@@ -1,0 +1,7 @@
+#include "attention_forward.cuh"
+
+namespace texb {
+namespace attention {
+template int forward_by_type<64>(const Problem&, int, bool, cudaStream_t);
+}  // namespace attention
+}  // namespace texb

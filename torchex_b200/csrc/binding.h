@@ -69,7 +69,7 @@ struct Plan {
   }
 };
 
-// token_ops_binding.cpp
-void register_token_ops(py::module& m);
+void register_token_ops(py::module& m);   // token_ops_binding.cpp
+void register_attention(py::module& m);   // attention_binding.cpp
 
 }  // namespace texb_binding

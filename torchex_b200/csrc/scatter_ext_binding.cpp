@@ -411,4 +411,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("segment_rank", &segment_rank);
   m.def("abi_version", &texb_version);
   register_token_ops(m);
+  register_attention(m);
 }

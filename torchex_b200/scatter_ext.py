@@ -54,6 +54,7 @@ embedding = native.embedding
 embedding_backward = native.embedding_backward
 grad_norm = native.grad_norm
 clip_grads = native.clip_grads
+segment_attention = native.segment_attention
 abi_version = native.abi_version
 
 
