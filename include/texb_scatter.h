@@ -483,6 +483,8 @@ typedef struct texb_attention_problem {
   const float* slopes;             /* device [heads], or NULL */
   int causal;
   void* out;                       /* [n, heads, dim], contiguous: written by forward, read by backward */
+  void* out_low;                   /* [n, heads, dim] or NULL: what rounding took from out, written by forward, read by
+                                      backward (whose gradients are less exact without it) */
   float* lse;                      /* [heads, n]: written by forward (NULL: not wanted), read by backward */
   const void* g;                   /* backward: gradient of out */
   int64_t g_strides[2];

@@ -24,7 +24,7 @@ class AttentionProblem(_c.Structure):
                 ("sid", _c.c_void_p), ("perm", _c.c_void_p), ("offsets", _c.c_void_p), ("n", _c.c_int64),
                 ("num_segments", _c.c_int64), ("max_count", _c.c_int64), ("heads", _c.c_int), ("kv_heads", _c.c_int),
                 ("dim", _c.c_int), ("scale", _c.c_float), ("softcap", _c.c_float), ("slopes", _c.c_void_p),
-                ("causal", _c.c_int), ("out", _c.c_void_p), ("lse", _c.c_void_p), ("g", _c.c_void_p),
+                ("causal", _c.c_int), ("out", _c.c_void_p), ("out_low", _c.c_void_p), ("lse", _c.c_void_p), ("g", _c.c_void_p),
                 ("g_strides", _c.c_int64 * 2), ("g_q", _c.c_void_p), ("g_k", _c.c_void_p), ("g_v", _c.c_void_p)]
 
 

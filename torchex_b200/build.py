@@ -32,7 +32,8 @@ HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "texb_scatter.h")
 SOURCES = ["abi.cu", "segment_reduce.cu", "reduce_unit_sum.cu", "reduce_unit_sum_plain.cu", "reduce_unit_max.cu",
            "reduce_unit_sum_max.cu", "segment_small.cu", "segment_plan.cu", "segment_backward.cu", "peer_copy.cu",
            "embedding.cu", "embedding_backward.cu", "grad_clip.cu", "attention.cu",
-           *(f"attention_{way}_{dim}.cu" for way in ("forward", "backward") for dim in (16, 32, 64, 128))]
+           *(f"attention_{way}_{dim}.cu" for way in ("forward", "backward") for dim in (16, 32, 64, 128)),
+           "attention_long_forward_64.cu", "attention_long_forward_128.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

@@ -8,6 +8,8 @@ namespace attention {
 
 template <int DP> int forward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int backward_by_type(const Problem&, int, bool, cudaStream_t);
+template <int DP> int long_forward_by_type(const Problem&, int, bool, cudaStream_t);
+template <int DP> int long_forward_timeouts(int*);
 
 namespace {
 
@@ -48,6 +50,11 @@ prepare_backward_kernel(const __grid_constant__ Problem a, float* __restrict__ d
       bad |= not_finite<T>(q) || not_finite<T>(reinterpret_cast<const uint4&>(g));
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf(widen<T>(g.v[e]), widen<T>(o.v[e]), sum);
+      if (a.out_low.p) {  // out itself is rounded: without the rest, delta's error would reach every dS of the row
+        const Chunk<T, 16> low = load_chunk<T, 16>(row_at<T>(a, a.out_low, y, pos) + sub * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(widen<T>(g.v[e]), widen<T>(low.v[e]), sum);
+      }
     }
     for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (pos < end && sub == 0) delta[int64_t(y) * a.n + pos] = sum;
@@ -75,6 +82,7 @@ int check(const Problem& a, int dtype, bool backward) {
     if (reinterpret_cast<uintptr_t>(views[i]->p) % 16 != 0 || views[i]->row % 8 != 0 || views[i]->head % 8 != 0)
       return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: rows must be 16-byte aligned");
   }
+  if (reinterpret_cast<uintptr_t>(a.out_low.p) % 16 != 0) return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: rows must be 16-byte aligned");
   if (backward && !a.lse) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: the backward pass needs lse");
   return TEXB_OK;
 }
@@ -85,8 +93,21 @@ inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kBlock)); }
 // doing it: at most three tiles of keys.
 constexpr int kShortSegment = 64;
 
+// Segments so long, on average, that tiles of 128 positions mostly hold one: then the products are matrix
+// products of some size, and run on the 5th-generation tensor cores.
+inline bool long_segments(const Problem& a) { return a.n >= int64_t(a.segments) * 128; }
+
 }  // namespace
 }  // namespace attention
+
+int attention_timeouts_impl(int* count) {
+  int total = 0, one = 0;
+  int st = attention::long_forward_timeouts<64>(&one);
+  total += one;
+  if (st == TEXB_OK) st = attention::long_forward_timeouts<128>(&one);
+  *count = total + one;
+  return st;
+}
 
 size_t attention_workspace_bytes_impl(int64_t n, int heads, int kv_heads, int backward) {
   if (n < 0 || heads < 1 || kv_heads < 1) return 0;
@@ -110,6 +131,7 @@ Problem problem_of(const texb_attention_problem& t) {
   a.v = view_of(t.v, t.v_strides);
   const int64_t rows[2] = {int64_t(t.heads) * t.dim, t.dim}, kv_rows[2] = {int64_t(t.kv_heads) * t.dim, t.dim};
   a.out = view_of(t.out, rows);
+  a.out_low = view_of(t.out_low, rows);
   a.g = view_of(t.g, t.g_strides);
   a.gq = view_of(t.g_q, rows);
   a.gk = view_of(t.g_k, kv_rows);
@@ -162,7 +184,11 @@ int attention_forward_impl(const texb_attention_problem* t, void* workspace, siz
     if (st != TEXB_OK) return st;
     a.bad_v = flags;
   }
-  const bool general = a.cap > 0.f || a.slopes != nullptr;
+  const bool general = a.cap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
+  if (a.bad_v && long_segments(a)) {
+    if (a.dim <= 64) return long_forward_by_type<64>(a, dtype, general, stream);
+    return long_forward_by_type<128>(a, dtype, general, stream);
+  }
   if (a.dim <= 16) return forward_by_type<16>(a, dtype, general, stream);
   if (a.dim <= 32) return forward_by_type<32>(a, dtype, general, stream);
   if (a.dim <= 64) return forward_by_type<64>(a, dtype, general, stream);

@@ -40,7 +40,8 @@ struct Problem {
   int causal;
   float scale, cap;          // cap 0: none
   // forward
-  View out;
+  View out;                  // [n, heads, dim]
+  View out_low;              // what rounding took from out, for the backward pass; p may be NULL
   float* lse;                // [heads, n] by position, in units of log2; forward may leave it out
   // backward
   View g;                    // gradient of out
@@ -66,6 +67,9 @@ __device__ __forceinline__ Bounds segment_of(const Problem& a, int pos) {
   const int s = min(max(__ldg(a.sid + pos), 0), a.segments - 1);
   return {max(0, __ldg(a.offsets + s)), min(a.n, __ldg(a.offsets + s + 1))};
 }
+// Bounded waits of the kernels for long segments that gave up (part of texb_device_status).
+static __device__ int g_wait_timeouts = 0;
+
 // keys that a query sees, and queries that see a key; empty for positions behind the last row
 __device__ __forceinline__ Bounds keys_of(const Problem& a, int pos) {
   if (pos >= a.n) return {0, 0};
@@ -157,7 +161,6 @@ struct Tile {
 };
 
 constexpr int kThreads = 128;
-constexpr int kWarps = kThreads / 32;
 
 // Copies rows [pos0, pos0 + ROWS) of head `head` into a tile; rows at or behind `end` become zeros.
 // The row numbers of the next tile are fetched ahead of it (`rows`), since they come through `perm`.
@@ -242,16 +245,21 @@ __device__ __forceinline__ void product_probabilities(float (&acc)[DP / 8][4], c
 
 // Writes the warp's 16 x DP accumulators, times `factor` per row, to rows of a tensor, through the
 // warp's own 16 rows of a tile (16-byte stores; the tile's former contents are no longer needed).
-template <typename T, int DP>
+// `low`: what rounding those values to T takes from them, instead of the values.
+template <typename T, int DP, bool LOW = false>
 __device__ __forceinline__ void store_rows(const Problem& a, const View& x, int head, int pos0, const float (&acc)[DP / 8][4],
                                            float factor0, float factor1, unsigned char* tile, int row0) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
+  auto value = [](float x, float factor) {
+    const float y = x * factor;
+    return LOW ? y - widen<T>(narrow<T>(y)) : y;
+  };
 #pragma unroll
   for (int t = 0; t < DP / 8; ++t) {
     const int r = row0 + (lane >> 2);
-    *reinterpret_cast<uint32_t*>(tile + Tile<DP>::at(r, t) + (lane & 3) * 4) = pack2<T>(acc[t][0] * factor0, acc[t][1] * factor0);
-    *reinterpret_cast<uint32_t*>(tile + Tile<DP>::at(r + 8, t) + (lane & 3) * 4) = pack2<T>(acc[t][2] * factor1, acc[t][3] * factor1);
+    *reinterpret_cast<uint32_t*>(tile + Tile<DP>::at(r, t) + (lane & 3) * 4) = pack2<T>(value(acc[t][0], factor0), value(acc[t][1], factor0));
+    *reinterpret_cast<uint32_t*>(tile + Tile<DP>::at(r + 8, t) + (lane & 3) * 4) = pack2<T>(value(acc[t][2], factor1), value(acc[t][3], factor1));
   }
   __syncwarp();
 #pragma unroll
@@ -297,7 +305,7 @@ __device__ __forceinline__ bool look_over(const Problem& a, const View& x, int h
 __device__ __forceinline__ bool any_flag(const Problem& a, const uint8_t* flags, int head, int begin, int end) {
   const int blocks = (a.n + kBlock - 1) / kBlock;
   bool bad = false;
-  for (int b = begin / kBlock + threadIdx.x; b * kBlock < end; b += kThreads) bad |= flags[int64_t(head) * blocks + b] != 0;
+  for (int b = begin / kBlock + threadIdx.x; b < blocks && b * kBlock < end; b += blockDim.x) bad |= flags[int64_t(head) * blocks + b] != 0;
   return __syncthreads_or(bad);
 }
 
@@ -355,10 +363,10 @@ __device__ __forceinline__ void store_columns(const Problem& a, const View& x, i
 }
 
 template <typename T>
-__device__ __noinline__ void plain_forward(const Problem& a, int pos0, int head) {
+__device__ __noinline__ void plain_forward(const Problem& a, int pos0, int rows, int head) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = head / (a.heads / a.kv_heads);
   const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
-  for (int i = pos0 + warp; i < min(a.n, pos0 + kBlock); i += kWarps) {
+  for (int i = pos0 + warp; i < min(a.n, pos0 + rows); i += blockDim.x / 32) {
     const Bounds see = keys_of(a, i);
     const T* qi = row_at<T>(a, a.q, head, i);
     float acc[kColumns] = {}, top = -INFINITY, sum = 0.f;
@@ -376,6 +384,14 @@ __device__ __noinline__ void plain_forward(const Problem& a, int pos0, int head)
     }
     const bool none = see.end <= see.begin;
     store_columns<T>(a, a.out, head, i, acc, none ? 0.f : 1.f / sum);
+    if (a.out_low.p) {
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) {
+        const float y = acc[c] * (none ? 0.f : 1.f / sum);
+        acc[c] = y - widen<T>(narrow<T>(y));
+      }
+      store_columns<T>(a, a.out_low, head, i, acc, 1.f);
+    }
     if (a.lse && lane == 0) a.lse[int64_t(head) * a.n + i] = none ? 0.f : top + log2f(sum);
   }
 }
@@ -390,10 +406,10 @@ __device__ __forceinline__ Pair pair_of(const Problem& a, const T* qi, const T* 
 }
 
 template <typename T>
-__device__ __noinline__ void plain_query_gradient(const Problem& a, int pos0, int head) {
+__device__ __noinline__ void plain_query_gradient(const Problem& a, int pos0, int rows, int head) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = head / (a.heads / a.kv_heads);
   const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
-  for (int i = pos0 + warp; i < min(a.n, pos0 + kBlock); i += kWarps) {
+  for (int i = pos0 + warp; i < min(a.n, pos0 + rows); i += blockDim.x / 32) {
     const Bounds see = keys_of(a, i);
     const T *qi = row_at<T>(a, a.q, head, i), *gi = row_at<T>(a, a.g, head, i);
     float acc[kColumns] = {};
@@ -409,9 +425,9 @@ __device__ __noinline__ void plain_query_gradient(const Problem& a, int pos0, in
 }
 
 template <typename T>
-__device__ __noinline__ void plain_key_gradients(const Problem& a, int pos0, int kv) {
+__device__ __noinline__ void plain_key_gradients(const Problem& a, int pos0, int rows, int kv) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.kv_heads;
-  for (int j = pos0 + warp; j < min(a.n, pos0 + kBlock); j += kWarps) {
+  for (int j = pos0 + warp; j < min(a.n, pos0 + rows); j += blockDim.x / 32) {
     const Bounds seen = queries_of(a, j);
     const T *kj = row_at<T>(a, a.k, kv, j), *vj = row_at<T>(a, a.v, kv, j);
     float acc_k[kColumns] = {}, acc_v[kColumns] = {};

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
   if (any_flag(a, a.bad_k, kv, first_key, end_key)) {
-    plain_query_gradient<T>(a, pos0, head);
+    plain_query_gradient<T>(a, pos0, kBlock, head);
     return;
   }
   const uint32_t base = smem_u32(smem);
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
   bool bad = false;
   for (int head = kv * group; head < (kv + 1) * group; ++head) bad |= any_flag(a, a.bad_q, head, first_query, end_query);
   if (bad) {
-    plain_key_gradients<T>(a, pos0, kv);
+    plain_key_gradients<T>(a, pos0, kBlock, kv);
     return;
   }
   const uint32_t base = smem_u32(smem);

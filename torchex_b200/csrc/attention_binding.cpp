@@ -3,6 +3,8 @@
 
 #include "binding.h"
 
+#include <tuple>
+
 namespace texb_binding {
 namespace {
 
@@ -61,20 +63,24 @@ void check_rows(const at::Tensor& t, const char* name, const at::Tensor& sid, co
   TORCH_CHECK(t.size(2) == q.size(2), name, " has another head dimension than q");
 }
 
-// out and, where a gradient will be wanted, the log-sums of the rows
-std::pair<at::Tensor, at::Tensor> forward(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+// out and, where a gradient will be wanted, what rounding took from it and the log-sums of the rows
+std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                           const at::Tensor& sid, const at::Tensor& perm, const at::Tensor& offsets,
                                           const at::Tensor& slopes, const Options& o, bool want_lse) {
   const c10::cuda::CUDAGuard guard(q_in.device());
   const at::Tensor q = readable_rows(q_in), k = readable_rows(k_in), v = readable_rows(v_in);
-  at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous)), lse;
+  at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous)), low, lse;
   texb_attention_problem p = problem_of(q, k, v, sid, perm, offsets, slopes, o);
-  if (want_lse) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  if (want_lse) {
+    low = at::empty_like(out);
+    lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  }
   p.out = out.data_ptr();
+  p.out_low = want_lse ? low.data_ptr() : nullptr;
   p.lse = want_lse ? lse.data_ptr<float>() : nullptr;
   const at::Tensor ws = scratch(texb_attention_workspace_bytes(p.n, p.heads, p.kv_heads, 0), q);
   check_status(texb_attention_forward(&p, ws.data_ptr(), size_t(ws.numel()), stream_of(q)), "texb_attention_forward");
-  return {out, lse};
+  return {out, low, lse};
 }
 
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
@@ -84,8 +90,8 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
                             int64_t num_segments, int64_t max_count) {
     const at::Tensor perm = perm_given.value_or(at::Tensor()), slopes = slopes_given.value_or(at::Tensor());
     const Options o = {scale, softcap, causal, num_segments, max_count};
-    const auto [out, lse] = texb_binding::forward(q, k, v, sid, perm, offsets, slopes, o, true);
-    ctx->save_for_backward({q, k, v, sid, perm, offsets, slopes, out, lse});
+    const auto [out, low, lse] = texb_binding::forward(q, k, v, sid, perm, offsets, slopes, o, true);
+    ctx->save_for_backward({q, k, v, sid, perm, offsets, slopes, out, low, lse});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["softcap"] = softcap;
     ctx->saved_data["causal"] = causal;
@@ -100,10 +106,11 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
                        ctx->saved_data["num_segments"].toInt(), ctx->saved_data["max_count"].toInt()};
     const c10::cuda::CUDAGuard guard(s[0].device());
     const at::Tensor q = readable_rows(s[0]), k = readable_rows(s[1]), v = readable_rows(s[2]), g = readable_rows(grads[0]);
-    const at::Tensor out = s[7].contiguous(), lse = s[8];
+    const at::Tensor out = s[7].contiguous(), low = s[8], lse = s[9];
     at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
     texb_attention_problem p = problem_of(q, k, v, s[3], s[4], s[5], s[6], o);
     p.out = out.data_ptr();
+    p.out_low = low.data_ptr();
     p.lse = lse.data_ptr<float>();
     p.g = g.data_ptr();
     p.g_strides[0] = g.stride(0);
@@ -146,7 +153,7 @@ at::Tensor segment_attention(const Plan& plan, const at::Tensor& q, const at::Te
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return AttentionNode::apply(q, k, v, plan.sid, given(plan.perm), plan.offsets, given(slopes), scale, softcap, causal,
                                 plan.num_segments, plan.max_cnt);
-  return forward(q, k, v, plan.sid, plan.perm, plan.offsets, slopes, o, false).first;
+  return std::get<0>(forward(q, k, v, plan.sid, plan.perm, plan.offsets, slopes, o, false));
 }
 
 }  // namespace

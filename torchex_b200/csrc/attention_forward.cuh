@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   const bool bad = a.bad_v ? any_flag(a, a.bad_v, kv, first_key, end_key)
                            : look_over<T>(a, a.v, kv, first_key, end_key);
   if (bad) {
-    plain_forward<T>(a, pos0, head);
+    plain_forward<T>(a, pos0, kBlock, head);
     return;
   }
 
@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     if (i0 < a.n) a.lse[int64_t(head) * a.n + i0] = none0 ? 0.f : top0 + log2f(sum0);
     if (i1 < a.n) a.lse[int64_t(head) * a.n + i1] = none1 ? 0.f : top1 + log2f(sum1);
   }
-  store_rows<T, DP>(a, a.out, head, pos0 + row0, out, none0 ? 0.f : 1.f / sum0,
-                    none1 ? 0.f : 1.f / sum1, smem + M::kQ, row0);
+  const float factor0 = none0 ? 0.f : 1.f / sum0, factor1 = none1 ? 0.f : 1.f / sum1;
+  store_rows<T, DP>(a, a.out, head, pos0 + row0, out, factor0, factor1, smem + M::kQ, row0);
+  if (a.out_low.p) store_rows<T, DP, true>(a, a.out_low, head, pos0 + row0, out, factor0, factor1, smem + M::kQ, row0);
 }
 
 template <typename T, int DP, bool GENERAL>

@@ -177,8 +177,10 @@ int plan_bad_indices_impl(int* count);   // segment_plan.cu
 int lookup_bad_tokens_impl(int* count);      // embedding.cu
 int table_grad_bad_tokens_impl(int* count);  // embedding_backward.cu
 
+int attention_timeouts_impl(int* count);     // attention.cu
+
 int device_status_impl(int* wait_timeouts, int* bad_indices) {
-  int v = 0, w = 0, w_small = 0, w_plan = 0, w_lookup = 0, w_table = 0;
+  int v = 0, w = 0, w_small = 0, w_plan = 0, w_lookup = 0, w_table = 0, v_attention = 0;
   int st = reduce_counters_sum(&v, &w);
   if (st == TEXB_OK) st = reduce_counters_sum_plain(&v, &w);
   if (st == TEXB_OK) st = reduce_counters_max(&v, &w);
@@ -187,8 +189,9 @@ int device_status_impl(int* wait_timeouts, int* bad_indices) {
   if (st == TEXB_OK) st = plan_bad_indices_impl(&w_plan);
   if (st == TEXB_OK) st = lookup_bad_tokens_impl(&w_lookup);
   if (st == TEXB_OK) st = table_grad_bad_tokens_impl(&w_table);
+  if (st == TEXB_OK) st = attention_timeouts_impl(&v_attention);
   if (st != TEXB_OK) return st;
-  if (wait_timeouts) *wait_timeouts = v;
+  if (wait_timeouts) *wait_timeouts = v + v_attention;
   if (bad_indices) *bad_indices = w + w_small + w_plan + w_lookup + w_table;
   return TEXB_OK;
 }

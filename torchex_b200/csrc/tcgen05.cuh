@@ -1,0 +1,148 @@
+// Thin wrappers of the sm_100a instructions that the attention kernels for long segments use: matrix
+// products into tensor memory (tcgen05), tensor memory loads and stores, and mbarriers with bounded waits.
+//
+// Operand tiles in shared memory are blocks of 64 columns (128 bytes) by any number of rows, 128 bytes from
+// row to row, their 16-byte pieces swizzled by the row (piece ^ row % 8), at 1024-byte boundaries.  Read
+// with the contraction along the columns ("by columns") or along the rows ("by rows") the same image
+// serves as either kind of operand:
+//   by columns: 8-row groups 1024 bytes apart; 16 columns further on are 32 bytes further on;
+//   by rows   : 64-column blocks `block` bytes apart, 8-row groups 1024 bytes apart; 16 rows are 2048 bytes.
+#pragma once
+
+#include "vector_io.cuh"
+
+namespace texb {
+namespace t5 {
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// ---- mbarriers ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+
+// Waits, for a bounded number of polls, until the phase of that parity is complete.  When the polls run out
+// or another thread's have (`*dead`), it gives up: the caller leaves its loop, and the kernel tears down and
+// returns instead of hanging.
+constexpr int kPolls = 1 << 20;
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (barrier_try(bar, parity)) return true;
+  for (int i = 0; i < kPolls; ++i) {
+    if (barrier_try(bar, parity)) return true;
+    if (*dead) return false;
+  }
+  *dead = 1;
+  return false;
+}
+
+// ---- tensor memory -----------------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, int columns) {  // one whole warp
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, int columns) {  // the same warp
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_copies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 columns of the warp's 32 lanes: lane l of the warp reads lane 32 (warp % 4) + l of tensor memory, which
+// the upper half of the address names.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- matrix products ---------------------------------------------------------------------------------
+// Descriptor of an operand tile: swizzle of 128 bytes (2 in the top bits), descriptor version 1.
+__device__ __forceinline__ uint64_t operand_by_columns(uint32_t addr) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+__device__ __forceinline__ uint64_t operand_by_rows(uint32_t addr, uint32_t block) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | uint64_t(block >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 |
+         uint64_t(2) << 61;
+}
+// Instruction descriptor: fp32 sums of products of 16-bit values (both operands of one type), M x N,
+// `b_by_rows`: the second operand's contraction runs along the rows of its tile.
+template <typename T>
+__host__ __device__ constexpr uint32_t instruction(int m, int n, bool b_by_rows) {
+  const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return 1u << 4 | type << 7 | type << 10 | (b_by_rows ? 1u << 16 : 0u) | uint32_t(n / 8) << 17 | uint32_t(m / 16) << 24;
+}
+// One thread; `add` false overwrites the sums.
+__device__ __forceinline__ void multiply(uint32_t sums, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(sums),
+               "l"(a), "l"(b), "r"(instr), "r"(uint32_t(add)) : "memory");
+}
+// First operand from tensor memory: one row per lane, two 16-bit values per column.
+__device__ __forceinline__ void multiply_tmem(uint32_t sums, uint32_t a, uint64_t b, uint32_t instr, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(sums),
+               "r"(a), "l"(b), "r"(instr), "r"(uint32_t(add)) : "memory");
+}
+// The barrier completes a phase when all products that this thread issued are done.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// sums[128 x n] (+)= rows of tile a times rows of tile b, contraction over DP columns.  Tiles of `rows_a`,
+// `rows_b` rows: blocks of 64 columns one after the other.
+template <int DP>
+__device__ __forceinline__ void multiply_columns(uint32_t sums, uint32_t a, int rows_a, uint32_t b, int rows_b, uint32_t instr) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k)
+    multiply(sums, operand_by_columns(a + (k / 4) * rows_a * 128 + (k % 4) * 32),
+             operand_by_columns(b + (k / 4) * rows_b * 128 + (k % 4) * 32), instr, k > 0);
+}
+// sums[128 x DP] (+)= P (16-bit, tensor memory, 128 x ROWS) times the rows of tile b
+template <int ROWS>
+__device__ __forceinline__ void multiply_rows(uint32_t sums, uint32_t p, uint32_t b, uint32_t instr, bool add) {
+#pragma unroll
+  for (int k = 0; k < ROWS / 16; ++k)
+    multiply_tmem(sums, p + k * 8, operand_by_rows(b + k * 2048, ROWS * 128), instr, add || k > 0);
+}
+
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place; tiny results become 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace t5
+}  // namespace texb
