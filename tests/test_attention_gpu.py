@@ -33,7 +33,9 @@ def _inputs(n, heads, kv_heads, dim, dtype, seed=0):
 def _definition(q, k, v, g, ids, segments, scale, causal, cap, slopes):
     """Outputs and gradients in 64 bits, and the bound of each: [(value, bound)] for o, gq, gk, gv."""
     h = torch.finfo(q.dtype).eps / 2
-    under = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2  # half of the smallest step
+    # half of the type's smallest step; and exponentials below 2^-126 become 0, so that a probability may be off by that
+    # much before it is rounded, and a gradient of a score by that much times |g v - delta| scale (added below)
+    under = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2 + 2 ** -126
     q, k, v, g = (x.double() for x in (q, k, v, g))
     group = q.shape[1] // k.shape[1]
     found = [[torch.zeros_like(x), torch.zeros_like(x)] for x in (q, q, k, v)]
@@ -73,6 +75,7 @@ def _definition(q, k, v, g, ids, segments, scale, causal, cap, slopes):
         d_delta = (gs.abs() * bound_o).sum(-1, keepdim=True) + (qs.shape[2] + 2) * 2 ** -24 * (gs * o).abs().sum(-1, keepdim=True)
         ds = p * (dp - delta) * slope * scale
         d_ds = p * (d_dp + d_delta) * abs(scale) + (e + h + 2 ** -22) * (ds.abs() + p * (d_dp + d_delta) * abs(scale)) + under * seen
+        d_ds = d_ds + 2 ** -126 * ((dp - delta).abs() + d_dp + d_delta) * slope * abs(scale) * seen
         if cap:
             d_ds = d_ds + p * ((dp - delta).abs() + d_dp + d_delta) * abs(scale) * 2 ** -19  # 1 - t^2 from t
         d_p = p * (h + e) + under * seen

@@ -1,7 +1,7 @@
 // Attention within segments: argument checks, workspaces, the pass that looks rows over, and the choice
 // of kernel.  The kernels are in attention_forward.cuh and attention_backward.cuh.
 
-#include "attention.cuh"
+#include "attention_long.cuh"
 
 namespace texb {
 namespace attention {
@@ -10,6 +10,28 @@ template <int DP> int forward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int backward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int long_forward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int long_forward_timeouts(int*);
+
+bool make_map(CUtensorMap* map, const Problem& a, const View& x, int heads, int box_rows, int dtype) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (!encode || x.row <= 0 || x.head <= 0) return false;
+  const cuuint64_t size[3] = {cuuint64_t(a.dim), cuuint64_t(heads), cuuint64_t(a.n)};
+  const cuuint64_t stride[2] = {cuuint64_t(x.head) * 2, cuuint64_t(x.row) * 2};
+  const cuuint32_t box[3] = {64, 1, cuuint32_t(box_rows)}, step[3] = {1, 1, 1};
+  return encode(map, dtype == TEXB_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.p, size, stride,
+                box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 namespace {
 
@@ -148,6 +170,9 @@ Problem problem_of(const texb_attention_problem& t) {
   a.causal = t.causal;
   a.scale = t.scale;
   a.cap = t.softcap;
+  a.unit = t.scale * kLog2e;
+  a.bend_in = t.softcap > 0.f ? float(2.0 * 1.4426950408889634 * double(t.scale) / double(t.softcap)) : 0.f;
+  a.bend_out = t.softcap * kLog2e;
   a.lse = t.lse;
   return a;
 }

@@ -39,6 +39,7 @@ struct Problem {
   int n, segments, heads, kv_heads, dim;
   int causal;
   float scale, cap;          // cap 0: none
+  float unit, bend_in, bend_out;  // scale log2(e), 2 scale log2(e) / cap, cap log2(e)
   // forward
   View out;                  // [n, heads, dim]
   View out_low;              // what rounding took from out, for the backward pass; p may be NULL
@@ -84,21 +85,33 @@ __device__ __forceinline__ Bounds queries_of(const Problem& a, int pos) {
   return b;
 }
 
-// The score in units of log2, from the plain product of a query and a key, and the derivative of the
-// score by scale * product.  exp(2y) of the tanh is infinite or 0 for large |y|: then tanh is +-1.
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place; tiny results become 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {  // 1 unit in the last place
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The score in units of log2, from the plain product of a query and a key, and its derivative by scale *
+// product.  tanh y = 1 - 2 / (exp(2 y) + 1), off by a few 2^-24 whatever y is: the exponential is infinite or 0
+// for large |y|, and tanh then +-1.  `slope` is the head's, in units of log2.
 struct Score { float x, slope; };
 template <bool GENERAL>
-__device__ __forceinline__ Score score_of(const Problem& a, float product, float bias_slope, int distance) {
-  if constexpr (!GENERAL) return {product * (a.scale * kLog2e), 1.f};
-  float x = product * a.scale, d = 1.f;
+__device__ __forceinline__ Score score_of(const Problem& a, float product, float slope, float distance) {
+  if constexpr (!GENERAL) return {product * a.unit, 1.f};
+  float x = product * a.unit, d = 1.f;
   if (a.cap > 0.f) {
-    const float y = x * (1.f / a.cap);
-    const float t = 1.f - 2.f / (exp2f(y * (2.f * kLog2e)) + 1.f);
-    x = a.cap * t;
-    d = 1.f - t * t;
+    const float t = fmaf(-2.f, reciprocal_fast(exp2_fast(product * a.bend_in) + 1.f), 1.f);
+    x = a.bend_out * t;
+    d = fmaf(-t, t, 1.f);
   }
-  return {(x - bias_slope * float(abs(distance))) * kLog2e, d};
+  return {fmaf(-slope, fabsf(distance), x), d};
 }
+__device__ __forceinline__ float slope_of(const Problem& a, int head) { return a.slopes ? __ldg(a.slopes + head) * kLog2e : 0.f; }
 
 // ---- matrix instructions on 16-bit fragments -----------------------------------------------------
 
@@ -365,14 +378,14 @@ __device__ __forceinline__ void store_columns(const Problem& a, const View& x, i
 template <typename T>
 __device__ __noinline__ void plain_forward(const Problem& a, int pos0, int rows, int head) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = head / (a.heads / a.kv_heads);
-  const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
+  const float slope = slope_of(a, head);
   for (int i = pos0 + warp; i < min(a.n, pos0 + rows); i += blockDim.x / 32) {
     const Bounds see = keys_of(a, i);
     const T* qi = row_at<T>(a, a.q, head, i);
     float acc[kColumns] = {}, top = -INFINITY, sum = 0.f;
     for (int j0 = see.begin; j0 < see.end; j0 += 32) {
       const int j = j0 + lane;
-      const float x = j < see.end ? score_of<true>(a, dot<T>(qi, row_at<T>(a, a.k, kv, j), a.dim), slope, i - j).x : -INFINITY;
+      const float x = j < see.end ? score_of<true>(a, dot<T>(qi, row_at<T>(a, a.k, kv, j), a.dim), slope, float(i - j)).x : -INFINITY;
       const float top_new = warp_max((x > top || x != x) ? x : top);
       const float base = top_new == -INFINITY ? 0.f : top_new;  // infinitely low scores so far: weight 0, not NaN
       const float w = j < see.end ? exp2f(x - base) : 0.f, shrink = top == -INFINITY ? 0.f : exp2f(top - base);
@@ -400,7 +413,7 @@ struct Pair { float p, ds; };  // probability and gradient of scale * product
 template <typename T>
 __device__ __forceinline__ Pair pair_of(const Problem& a, const T* qi, const T* kj, const T* vj, const T* gi, int head, int i, int j,
                                         float slope) {
-  const Score s = score_of<true>(a, dot<T>(qi, kj, a.dim), slope, i - j);
+  const Score s = score_of<true>(a, dot<T>(qi, kj, a.dim), slope, float(i - j));
   const float p = exp2f(s.x - a.lse[int64_t(head) * a.n + i]);
   return {p, p * (dot<T>(gi, vj, a.dim) - a.delta[int64_t(head) * a.n + i]) * (s.slope * a.scale)};
 }
@@ -408,7 +421,7 @@ __device__ __forceinline__ Pair pair_of(const Problem& a, const T* qi, const T* 
 template <typename T>
 __device__ __noinline__ void plain_query_gradient(const Problem& a, int pos0, int rows, int head) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = head / (a.heads / a.kv_heads);
-  const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
+  const float slope = slope_of(a, head);
   for (int i = pos0 + warp; i < min(a.n, pos0 + rows); i += blockDim.x / 32) {
     const Bounds see = keys_of(a, i);
     const T *qi = row_at<T>(a, a.q, head, i), *gi = row_at<T>(a, a.g, head, i);
@@ -432,7 +445,7 @@ __device__ __noinline__ void plain_key_gradients(const Problem& a, int pos0, int
     const T *kj = row_at<T>(a, a.k, kv, j), *vj = row_at<T>(a, a.v, kv, j);
     float acc_k[kColumns] = {}, acc_v[kColumns] = {};
     for (int head = kv * group; head < (kv + 1) * group; ++head) {
-      const float slope = a.slopes ? __ldg(a.slopes + head) : 0.f;
+      const float slope = slope_of(a, head);
       for (int i0 = seen.begin; i0 < seen.end; i0 += 32) {
         const int i = i0 + lane, count = min(32, seen.end - i0);
         Pair w = {0.f, 0.f};

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_c
   const Bounds see0 = keys_of(a, i0), see1 = keys_of(a, i1);
   const int warp_begin = keys_of(a, pos0 + row0).begin, warp_last = min(last, pos0 + row0 + 15);
   const int warp_end = pos0 + row0 <= last ? keys_of(a, warp_last).end : 0;
-  const float slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+  const float slope = GENERAL ? slope_of(a, head) : 0.f;
   const int64_t place = int64_t(head) * a.n;
   const float lse0 = i0 < a.n ? a.lse[place + i0] : 0.f, lse1 = i1 < a.n ? a.lse[place + i1] : 0.f;
   const float delta0 = i0 < a.n ? a.delta[place + i0] : 0.f, delta1 = i1 < a.n ? a.delta[place + i1] : 0.f;
@@ -76,9 +76,9 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = j0 + t * 8 + (lane & 3) * 2 + e;
-          const Score x0 = score_of<GENERAL>(a, s[t][e], slope, i0 - j), x1 = score_of<GENERAL>(a, s[t][2 + e], slope, i1 - j);
-          const float d0 = exp2f(x0.x - lse0) * (dp[t][e] - delta0) * (x0.slope * a.scale);
-          const float d1 = exp2f(x1.x - lse1) * (dp[t][2 + e] - delta1) * (x1.slope * a.scale);
+          const Score x0 = score_of<GENERAL>(a, s[t][e], slope, float(i0 - j)), x1 = score_of<GENERAL>(a, s[t][2 + e], slope, float(i1 - j));
+          const float d0 = exp2_fast(x0.x - lse0) * (dp[t][e] - delta0) * (x0.slope * a.scale);
+          const float d1 = exp2_fast(x1.x - lse1) * (dp[t][2 + e] - delta1) * (x1.slope * a.scale);
           dp[t][e] = j >= see0.begin && j < see0.end ? d0 : 0.f;
           dp[t][2 + e] = j >= see1.begin && j < see1.end ? d1 : 0.f;
         }
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
     wait_copies<1>();
     __syncthreads();
     if (q0 + R > warp_begin && q0 < warp_end) {
-      const float slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+      const float slope = GENERAL ? slope_of(a, head) : 0.f;
       const uint32_t tq = base + M::kQ + stage * M::kStep, tg = base + M::kG + stage * M::kStep;
       float p[NT][4] = {}, ds[NT][4] = {};
       product_rows<T, DP, NT>(p, base + M::kK, row0, tq);
@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
         for (int e = 0; e < 2; ++e) {
           const int r = t * 8 + (lane & 3) * 2 + e, i = q0 + r;
           const float lse = s_lse[stage * R + r], delta = s_delta[stage * R + r];
-          const Score x0 = score_of<GENERAL>(a, p[t][e], slope, i - j0), x1 = score_of<GENERAL>(a, p[t][2 + e], slope, i - j1);
+          const Score x0 = score_of<GENERAL>(a, p[t][e], slope, float(i - j0)), x1 = score_of<GENERAL>(a, p[t][2 + e], slope, float(i - j1));
           const bool on0 = i >= seen0.begin && i < seen0.end, on1 = i >= seen1.begin && i < seen1.end;
-          p[t][e] = on0 ? exp2f(x0.x - lse) : 0.f;
-          p[t][2 + e] = on1 ? exp2f(x1.x - lse) : 0.f;
+          p[t][e] = on0 ? exp2_fast(x0.x - lse) : 0.f;
+          p[t][2 + e] = on1 ? exp2_fast(x1.x - lse) : 0.f;
           ds[t][e] = on0 ? p[t][e] * (ds[t][e] - delta) * (x0.slope * a.scale) : 0.f;
           ds[t][2 + e] = on1 ? p[t][2 + e] * (ds[t][2 + e] - delta) * (x1.slope * a.scale) : 0.f;
         }

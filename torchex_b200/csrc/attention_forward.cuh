@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   const Bounds tail = pos0 + row0 <= last ? keys_of(a, warp_last) : Bounds{0, 0};
   const int warp_end = tail.end;
   const int all_begin = tail.begin, all_end = pos0 + row0 + 15 <= last ? keys_of(a, pos0 + row0).end : 0;
-  const float slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+  const float slope = GENERAL ? slope_of(a, head) : 0.f;
 
   float out[DP / 8][4] = {};
   float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = j0 + t * 8 + (lane & 3) * 2 + e;
-          s[t][e] = score_of<GENERAL>(a, s[t][e], slope, i0 - j).x;
-          s[t][2 + e] = score_of<GENERAL>(a, s[t][2 + e], slope, i1 - j).x;
+          s[t][e] = score_of<GENERAL>(a, s[t][e], slope, float(i0 - j)).x;
+          s[t][2 + e] = score_of<GENERAL>(a, s[t][2 + e], slope, float(i1 - j)).x;
           if (!whole) {
             if (j < see0.begin || j >= see0.end) s[t][e] = -INFINITY;
             if (j < see1.begin || j >= see1.end) s[t][2 + e] = -INFINITY;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
       }
       // no visible key so far: subtract 0, so that the weights become 0 and not NaN
       const float base0 = top0_new == -INFINITY ? 0.f : top0_new, base1 = top1_new == -INFINITY ? 0.f : top1_new;
-      const float shrink0 = exp2f(top0 - base0), shrink1 = exp2f(top1 - base1);
+      const float shrink0 = exp2_fast(top0 - base0), shrink1 = exp2_fast(top1 - base1);
       top0 = top0_new;
       top1 = top1_new;
       sum0 *= shrink0;
@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[t][e] = exp2f(s[t][e] - base0);
-          s[t][2 + e] = exp2f(s[t][2 + e] - base1);
+          s[t][e] = exp2_fast(s[t][e] - base0);
+          s[t][2 + e] = exp2_fast(s[t][2 + e] - base1);
           sum0 += s[t][e];
           sum1 += s[t][2 + e];
         }

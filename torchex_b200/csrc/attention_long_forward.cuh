@@ -5,24 +5,22 @@
 // keys and values in shared memory (keys and values in two stages each).  Sixteen warps:
 //   0-3, 4-7 : softmax of query tile 0 and 1, one row per thread.  A thread reads its row of scores, and
 //              writes its probabilities over them in 16 bits, where the second product takes them from;
-//   8-11     : copies of rows into shared memory (rows come through the plan's permutation, so that they
-//              are gathered, 16 bytes per copy);
-//   12       : one thread issues all products.  While one tile's softmax runs, the other tile's products do.
+//   8-11     : copies of rows into shared memory: rows that lie in segment order by the copy engine, a tile
+//              of 64 columns by 128 rows at a time (one thread); rows that come through the plan's permutation
+//              16 bytes at a time, by all four warps;
+//   12, 13   : one thread each issues the products of query tile 0 and 1.  While one tile's softmax runs, the
+//              other tile's products do.
 // The outputs are rescaled only when a row's maximum has grown by more than 2^8 (the sums carry the stale
 // maximum until then: probabilities up to 2^8 lose nothing in fp32 sums), which is rare after the first tiles.
 // Bound: exponentials.  128 x 128 of them take 1024 cycles of an SM, the two products of that tile 512 at
 // the tensor cores' nominal rate.
 #pragma once
 
-#include "attention.cuh"
-#include "tcgen05.cuh"
+#include "attention_long.cuh"
 
 namespace texb {
 namespace attention {
 
-constexpr int kLongTile = 128;
-constexpr int kLongRows = 2 * kLongTile;
-constexpr int kLongThreads = 512;
 constexpr float kStale = 8.f;  // growth of a row's maximum, in units of log2, that is left unscaled
 
 template <int DP>
@@ -33,27 +31,6 @@ struct LongForwardMemory {
   static constexpr int kBytes = kBarriers + 256 + 1024;  // and room to align the start to 1024 bytes
   static constexpr int kScores = 0, kOut = 2 * kLongTile, kColumns = 512;  // tensor memory
 };
-
-// Copies 128 rows from position pos0 on (zeros from `end` on) into a tile of blocks of 64 columns, by a
-// warpgroup.  Four rows of a 128-byte block per warp and step: the 16-byte pieces of a row go to the eight
-// places that its swizzle gives.
-template <typename T, int DP>
-__device__ __forceinline__ void copy_long_tile(const Problem& a, const View& x, int head, int pos0, int end, uint32_t to) {
-  const int thread = threadIdx.x & 127, piece = thread & 7;
-  const T* base = static_cast<const T*>(x.p) + head * x.head;
-#pragma unroll 4
-  for (int r = thread >> 3; r < kLongTile; r += 16) {
-    const int pos = pos0 + r;
-    const bool real = pos < end;
-    const T* from = base + (real ? row_of(a, pos) * x.row : 0);
-#pragma unroll
-    for (int b = 0; b < DP / 64; ++b) {
-      const int column = b * 64 + piece * 8;
-      const bool on = real && column < a.dim;
-      copy16(to + b * (kLongTile * 128) + r * 128 + ((piece ^ (r & 7)) << 4), from + (on ? column : 0), on ? 16 : 0);
-    }
-  }
-}
 
 struct LongRange {  // of a query tile: the tiles of keys that some row sees, and those that all rows see
   int begin, end, all_begin, all_end;
@@ -66,7 +43,8 @@ __device__ __forceinline__ LongRange range_of(const Problem& a, int pos0) {
 }
 
 template <typename T, int DP, bool GENERAL>
-__global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __grid_constant__ Problem a) {
+__global__ void __launch_bounds__(kLongThreads, 1)
+long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ Maps maps) {
   extern __shared__ unsigned char raw[];
   using M = LongForwardMemory<DP>;
   unsigned char* smem = raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023);
@@ -75,10 +53,12 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
   const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
   // the last tiles of a causal segment see the most keys: begin with them
   const int pos0 = (a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * kLongRows;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
   const LongRange range[2] = {range_of(a, pos0), range_of(a, pos0 + kLongTile)};
   const int first_key = range[0].begin, end_key = max(range[0].end, range[1].end);
-  if (any_flag(a, a.bad_v, kv, first_key, end_key)) {
+  const int tiles = (end_key - first_key + kLongTile - 1) / kLongTile;
+  // boxes are copied whole: the last one may hold rows behind the last key, which must be finite as well
+  if (any_flag(a, a.bad_v, kv, first_key, min(a.n, first_key + tiles * kLongTile))) {
     plain_forward<T>(a, pos0, kLongRows, head);
     return;
   }
@@ -88,12 +68,13 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
   // 9-10 scores full, 11-12 probabilities full, 13-14 outputs done (by query tile)
   if (threadIdx.x == 0) {
     s_dead = 0;
-    t5::barrier_init(bar(0), 128);
+    const int copiers = maps.used ? 1 : 128;
+    t5::barrier_init(bar(0), copiers);
     for (int s = 0; s < 2; ++s) {
-      t5::barrier_init(bar(1 + s), 128);
-      t5::barrier_init(bar(3 + s), 1);
-      t5::barrier_init(bar(5 + s), 128);
-      t5::barrier_init(bar(7 + s), 1);
+      t5::barrier_init(bar(1 + s), copiers);
+      t5::barrier_init(bar(3 + s), 2);
+      t5::barrier_init(bar(5 + s), copiers);
+      t5::barrier_init(bar(7 + s), 2);
       t5::barrier_init(bar(9 + s), 1);
       t5::barrier_init(bar(11 + s), 128);
       t5::barrier_init(bar(13 + s), 1);
@@ -104,9 +85,8 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
   t5::fence_before_sync();
   __syncthreads();
   t5::fence_after_sync();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   volatile int* dead = &s_dead;
-  const int tiles = (end_key - first_key + kLongTile - 1) / kLongTile;
   auto sees = [&](int w, int j) {  // whether query tile w sees some key of tile j
     const int j0 = first_key + j * kLongTile;
     return j < tiles && j0 < range[w].end && j0 + kLongTile > range[w].begin;
@@ -118,7 +98,7 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t scores = tmem + lanes + M::kScores + w * kLongTile, sums = tmem + lanes + M::kOut + w * DP;
     const Bounds see = keys_of(a, i);
-    const float unit = a.scale * kLog2e, slope = GENERAL && a.slopes ? __ldg(a.slopes + head) : 0.f;
+    const float unit = a.unit, slope = GENERAL ? slope_of(a, head) : 0.f;
     float top = -INFINITY, sum = 0.f;  // in units of log2
     int done = 0;                      // tiles of this query tile so far
     bool alive = true;
@@ -134,7 +114,7 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
       const int j0 = first_key + j * kLongTile;
       if constexpr (GENERAL) {
 #pragma unroll
-        for (int c = 0; c < kLongTile; ++c) s[c] = score_of<true>(a, s[c], slope, i - (j0 + c)).x;
+        for (int c = 0; c < kLongTile; ++c) s[c] = score_of<true>(a, s[c], slope, float(i - j0) - float(c)).x;
       }
       if (!(j0 >= range[w].all_begin && j0 + kLongTile <= range[w].all_end && pos0 + (w + 1) * kLongTile <= a.n)) {
         const int from = see.begin - j0, to = see.end - j0;
@@ -154,7 +134,7 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
         if (!alive) break;
         t5::fence_after_sync();
         const float next = fmaxf(top, now);
-        const float shrink = next == -INFINITY ? 1.f : t5::exp2_fast(top - next);
+        const float shrink = next == -INFINITY ? 1.f : exp2_fast(top - next);
         top = next;
         sum *= shrink;
 #pragma unroll
@@ -174,8 +154,8 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float x0 = t5::exp2_fast(GENERAL ? s[c + e] - less : fmaf(s[c + e], unit, -less));
-          const float x1 = t5::exp2_fast(GENERAL ? s[c + e + 1] - less : fmaf(s[c + e + 1], unit, -less));
+          const float x0 = exp2_fast(GENERAL ? s[c + e] - less : fmaf(s[c + e], unit, -less));
+          const float x1 = exp2_fast(GENERAL ? s[c + e + 1] - less : fmaf(s[c + e + 1], unit, -less));
           part[e & 2] += x0;
           part[(e & 2) + 1] += x1;
           p[e / 2] = pack2<T>(x0, x1);
@@ -229,8 +209,27 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
     };
     const int items = 2 * tiles;
     bool alive = true;
-    int item = 0;
-    for (; item < items; ++item) {
+    if (maps.used) {
+      if (warp == 8 && t5::elect_one()) {
+        auto box = [&](const CUtensorMap& map, uint32_t to, int full, int h, int pos) {
+#pragma unroll
+          for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (kLongTile * 128), &map, bar(full), b * 64, h, pos);
+        };
+        for (int item = 0; item < items; ++item) {
+          const int j = item >> 1, stage = j & 1, pos = first_key + j * kLongTile, full = (item & 1 ? 5 : 1) + stage;
+          if (j >= 2 && !t5::barrier_wait(bar((item & 1 ? 7 : 3) + stage), ((j >> 1) - 1) & 1, dead)) break;
+          if (item == 0) {
+            t5::barrier_arrive_expect(bar(0), 2 * M::kTile);
+            box(maps.q, base + M::kQ, 0, head, pos0);
+            box(maps.q, base + M::kQ + M::kTile, 0, head, pos0 + kLongTile);
+          }
+          t5::barrier_arrive_expect(bar(full), M::kTile);
+          if (item & 1) box(maps.v, base + M::kV + stage * M::kTile, full, kv, pos);
+          else box(maps.k, base + M::kK + stage * M::kTile, full, kv, pos);
+        }
+      }
+    }
+    for (int item = maps.used ? items : 0; item < items; ++item) {
       const int j = item >> 1, stage = j & 1, pos = first_key + j * kLongTile;
       if (j >= 2) {
         alive = __all_sync(0xffffffffu, t5::barrier_wait(bar((item & 1 ? 7 : 3) + stage), ((j >> 1) - 1) & 1, dead));
@@ -248,87 +247,78 @@ __global__ void __launch_bounds__(kLongThreads, 1) long_forward_kernel(const __g
         announce(item - 2);
       }
     }
-    if (alive) {
+    if (alive && !maps.used) {
       wait_copies<0>();
       for (int late = max(0, items - 2); late < items; ++late) announce(late);
     }
     wait_copies<0>();
   } else {
     t5::fewer_registers<72>();
-    if (warp == 12 && lane == 0) {  // ---- products
+    if (warp < 14 && t5::elect_one()) {  // ---- products
       constexpr uint32_t score_instr = t5::instruction<T>(128, kLongTile, false), out_instr = t5::instruction<T>(128, DP, true);
-      int done[2] = {0, 0};
-      auto keys = [&](int j) {
+      const int w = warp - 12;
+      const uint32_t scores = tmem + M::kScores + w * kLongTile, sums = tmem + M::kOut + w * DP;
+      int done = 0;
+      // Scores of tile j.  Either way the keys' stage is given back, if it is filled again: nothing may arrive at
+      // a barrier that nobody waits for any more.
+      auto score = [&](int j) {
         if (!t5::barrier_wait(bar(1 + (j & 1)), (j >> 1) & 1, dead)) return false;
         t5::fence_after_sync();
+        if (sees(w, j)) {
+          t5::multiply_columns<DP>(scores, base + M::kQ + w * M::kTile, kLongTile, base + M::kK + (j & 1) * M::kTile, kLongTile, score_instr);
+          t5::commit(bar(9 + w));
+        }
+        if (j + 2 < tiles) t5::commit(bar(3 + (j & 1)));
         return true;
       };
-      auto score = [&](int w, int j) {
-        t5::multiply_columns<DP>(tmem + M::kScores + w * kLongTile, base + M::kQ + w * M::kTile, kLongTile,
-                                 base + M::kK + (j & 1) * M::kTile, kLongTile, score_instr);
-        t5::commit(bar(9 + w));
-      };
-      bool alive = tiles == 0 || (t5::barrier_wait(bar(0), 0, dead) && keys(0));
-      if (alive && tiles > 0) {
-        for (int w = 0; w < 2; ++w)
-          if (sees(w, 0)) score(w, 0);
-        if (tiles > 2) t5::commit(bar(3));
-      }
+      bool alive = tiles == 0 || (t5::barrier_wait(bar(0), 0, dead) && score(0));
       for (int j = 0; alive && j < tiles; ++j) {
         alive = t5::barrier_wait(bar(5 + (j & 1)), (j >> 1) & 1, dead);
-        if (alive && j + 1 < tiles) alive = keys(j + 1);
-        for (int w = 0; alive && w < 2; ++w) {
-          if (sees(w, j)) {
-            alive = t5::barrier_wait(bar(11 + w), done[w] & 1, dead);
-            if (!alive) break;
-            t5::fence_after_sync();
-            t5::multiply_rows<kLongTile>(tmem + M::kOut + w * DP, tmem + M::kScores + w * kLongTile,
-                                         base + M::kV + (j & 1) * M::kTile, out_instr, done[w] > 0);
-            t5::commit(bar(13 + w));
-            ++done[w];
-          }
-          // products are done in the order of their issue: the scores may overwrite the probabilities
-          if (sees(w, j + 1)) score(w, j + 1);
+        if (alive && sees(w, j)) {
+          alive = t5::barrier_wait(bar(11 + w), done & 1, dead);
+          if (!alive) break;
+          t5::fence_after_sync();
+          t5::multiply_rows<kLongTile>(sums, scores, base + M::kV + (j & 1) * M::kTile, out_instr, done > 0);
+          t5::commit(bar(13 + w));
+          ++done;
         }
-        if (alive) {  // only stages that are filled again: nothing may arrive at a barrier nobody waits for any more
-          if (j + 2 < tiles) t5::commit(bar(7 + (j & 1)));
-          if (j + 3 < tiles) t5::commit(bar(3 + ((j + 1) & 1)));
-        }
+        if (!alive) break;
+        if (j + 2 < tiles) t5::commit(bar(7 + (j & 1)));
+        // products of one thread are done in the order of their issue: the scores may overwrite the probabilities
+        if (j + 1 < tiles) alive = score(j + 1);
       }
     }
   }
-  // All products have been waited for by the softmax warps, except after a wait that gave up: those that
-  // were issued finish by themselves, within the memory that this CTA still holds, before the barrier below
-  // lets it go -- the issuing thread waits for them.
+  // All products and copies have been waited for, except after a wait that gave up: then what is still under
+  // way ends within the memory that this CTA holds.
   t5::fence_before_sync();
   __syncthreads();
-  if (s_dead && threadIdx.x == 12 * 32) {
-    t5::barrier_init(bar(15), 1);
-    t5::commit(bar(15));
-    for (int p = 0; p < t5::kPolls && !t5::barrier_try(bar(15), 0); ++p) {}
-    atomicAdd(&g_wait_timeouts, 1);
-  }
+  if (s_dead) t5::settle(bar(15 + (warp & 1)), (warp == 12 || warp == 13) && t5::elect_one(), &g_wait_timeouts);
   __syncthreads();
   t5::fence_after_sync();
   if (warp == 12) t5::tmem_free(tmem, M::kColumns);
 }
 
 template <typename T, int DP, bool GENERAL>
-int launch_long_forward(const Problem& a, cudaStream_t stream) {
+int launch_long_forward(const Problem& a, int dtype, cudaStream_t stream) {
   auto kernel = long_forward_kernel<T, DP, GENERAL>;
   constexpr int bytes = LongForwardMemory<DP>::kBytes;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "attention long_forward_kernel: %s", cudaGetErrorString(e));
+  Maps maps = {};
+  maps.used = a.perm == nullptr && make_map(&maps.q, a, a.q, a.heads, kLongTile, dtype) && make_map(&maps.k, a, a.k, a.kv_heads, kLongTile, dtype) &&
+              make_map(&maps.v, a, a.v, a.kv_heads, kLongTile, dtype);
   const dim3 grid(unsigned((a.n + kLongRows - 1) / kLongRows), unsigned(a.heads));
-  kernel<<<grid, kLongThreads, bytes, stream>>>(a);
+  kernel<<<grid, kLongThreads, bytes, stream>>>(a, maps);
   return check_launch("attention long_forward_kernel");
 }
 
 template <int DP>
 int long_forward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
   if (dtype == TEXB_BFLOAT16)
-    return general ? launch_long_forward<__nv_bfloat16, DP, true>(a, stream) : launch_long_forward<__nv_bfloat16, DP, false>(a, stream);
-  return general ? launch_long_forward<__half, DP, true>(a, stream) : launch_long_forward<__half, DP, false>(a, stream);
+    return general ? launch_long_forward<__nv_bfloat16, DP, true>(a, dtype, stream)
+                   : launch_long_forward<__nv_bfloat16, DP, false>(a, dtype, stream);
+  return general ? launch_long_forward<__half, DP, true>(a, dtype, stream) : launch_long_forward<__half, DP, false>(a, dtype, stream);
 }
 
 // Waits that gave up in this unit's kernels since the library was loaded.

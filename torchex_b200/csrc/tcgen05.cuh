@@ -9,6 +9,10 @@
 //   by rows   : 64-column blocks `block` bytes apart, 8-row groups 1024 bytes apart; 16 rows are 2048 bytes.
 #pragma once
 
+#include <cuda.h>
+
+#include <type_traits>
+
 #include "vector_io.cuh"
 
 namespace texb {
@@ -42,6 +46,17 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
   }
   *dead = 1;
   return false;
+}
+
+// Also expects `bytes` of copies in this phase.
+__device__ __forceinline__ void barrier_arrive_expect(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A box of a three-dimensional tensor (columns, heads, rows) into shared memory; the barrier counts its bytes.
+// Places behind the tensor's end read as zeros.  The first column is a multiple of 8 (16 bytes).
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, uint32_t bar, int column, int head, int row) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
+               "l"(map), "r"(bar), "r"(column), "r"(head), "r"(row) : "memory");
 }
 
 // ---- tensor memory -----------------------------------------------------------------------------------
@@ -88,13 +103,13 @@ __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::
 __device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- matrix products ---------------------------------------------------------------------------------
-// Descriptor of an operand tile: swizzle of 128 bytes (2 in the top bits), descriptor version 1.
-__device__ __forceinline__ uint64_t operand_by_columns(uint32_t addr) {
-  return uint64_t((addr & 0x3ffffu) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
-}
-__device__ __forceinline__ uint64_t operand_by_rows(uint32_t addr, uint32_t block) {
-  return uint64_t((addr & 0x3ffffu) >> 4) | uint64_t(block >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 |
-         uint64_t(2) << 61;
+// Descriptor of an operand tile: swizzle of 128 bytes (2 in the top bits), descriptor version 1, 8-row groups
+// 1024 bytes apart.  Only the lower half differs between tiles: address and, read by rows, the distance of
+// the 64-column blocks, both in units of 16 bytes.
+constexpr uint32_t kOperandUpper = 1024u >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand_by_columns(uint32_t addr) { return (addr & 0x3ffffu) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t operand_by_rows(uint32_t addr, uint32_t block) {
+  return (addr & 0x3ffffu) >> 4 | (block >> 4) << 16;
 }
 // Instruction descriptor: fp32 sums of products of 16-bit values (both operands of one type), M x N,
 // `b_by_rows`: the second operand's contraction runs along the rows of its tile.
@@ -104,14 +119,18 @@ __host__ __device__ constexpr uint32_t instruction(int m, int n, bool b_by_rows)
   return 1u << 4 | type << 7 | type << 10 | (b_by_rows ? 1u << 16 : 0u) | uint32_t(n / 8) << 17 | uint32_t(m / 16) << 24;
 }
 // One thread; `add` false overwrites the sums.
-__device__ __forceinline__ void multiply(uint32_t sums, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(sums),
-               "l"(a), "l"(b), "r"(instr), "r"(uint32_t(add)) : "memory");
+__device__ __forceinline__ void multiply(uint32_t sums, uint32_t a, uint32_t b, uint32_t instr, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(sums), "r"(a), "r"(b), "r"(instr), "r"(uint32_t(add)),
+      "r"(kOperandUpper) : "memory");
 }
 // First operand from tensor memory: one row per lane, two 16-bit values per column.
-__device__ __forceinline__ void multiply_tmem(uint32_t sums, uint32_t a, uint64_t b, uint32_t instr, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(sums),
-               "r"(a), "l"(b), "r"(instr), "r"(uint32_t(add)) : "memory");
+__device__ __forceinline__ void multiply_tmem(uint32_t sums, uint32_t a, uint32_t b, uint32_t instr, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(sums), "r"(a), "r"(b), "r"(instr), "r"(uint32_t(add)),
+      "r"(kOperandUpper) : "memory");
 }
 // The barrier completes a phase when all products that this thread issued are done.
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -122,27 +141,40 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 // `rows_b` rows: blocks of 64 columns one after the other.
 template <int DP>
 __device__ __forceinline__ void multiply_columns(uint32_t sums, uint32_t a, int rows_a, uint32_t b, int rows_b, uint32_t instr) {
+  const uint32_t first_a = operand_by_columns(a), first_b = operand_by_columns(b);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k)
-    multiply(sums, operand_by_columns(a + (k / 4) * rows_a * 128 + (k % 4) * 32),
-             operand_by_columns(b + (k / 4) * rows_b * 128 + (k % 4) * 32), instr, k > 0);
+    multiply(sums, first_a + (k / 4) * (rows_a * 8) + (k % 4) * 2, first_b + (k / 4) * (rows_b * 8) + (k % 4) * 2, instr, k > 0);
 }
 // sums[128 x DP] (+)= P (16-bit, tensor memory, 128 x ROWS) times the rows of tile b
 template <int ROWS>
 __device__ __forceinline__ void multiply_rows(uint32_t sums, uint32_t p, uint32_t b, uint32_t instr, bool add) {
+  const uint32_t first_b = operand_by_rows(b, ROWS * 128);
 #pragma unroll
-  for (int k = 0; k < ROWS / 16; ++k)
-    multiply_tmem(sums, p + k * 8, operand_by_rows(b + k * 2048, ROWS * 128), instr, add || k > 0);
+  for (int k = 0; k < ROWS / 16; ++k) multiply_tmem(sums, p + k * 8, first_b + k * (2048 >> 4), instr, add || k > 0);
+}
+
+// One lane of the (converged) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on != 0;
+}
+
+// After a wait that gave up: waits, with a limit, for the products that `issuer` issued, and about a
+// millisecond for copies that are still under way, and counts the event.  Called by all threads between two
+// barriers.
+__device__ __forceinline__ void settle(uint32_t bar, bool issuer, int* counter) {
+  if (!issuer) return;
+  barrier_init(bar, 1);
+  commit(bar);
+  for (int p = 0; p < kPolls && !barrier_try(bar, 0); ++p) {}
+  for (int p = 0; p < 1000; ++p) __nanosleep(1000);
+  atomicAdd(counter, 1);
 }
 
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
-__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place; tiny results become 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 }  // namespace t5
 }  // namespace texb
