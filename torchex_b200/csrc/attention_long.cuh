@@ -21,15 +21,15 @@ struct Maps {
 // False where the copy engine cannot describe the tensor (then the rows are copied 16 bytes at a time).
 bool make_map(CUtensorMap* map, const Problem& a, const View& x, int heads, int box_rows, int dtype);  // attention.cu
 
-// Copies 128 rows from position pos0 on (zeros from `end` on) into a tile of blocks of 64 columns, by a
+// Copies ROWS rows from position pos0 on (zeros from `end` on) into a tile of blocks of 64 columns, by a
 // warpgroup.  Four rows of a 128-byte block per warp and step: the 16-byte pieces of a row go to the eight
 // places that its swizzle gives.
-template <typename T, int DP>
+template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void copy_long_tile(const Problem& a, const View& x, int head, int pos0, int end, uint32_t to) {
   const int thread = threadIdx.x & 127, piece = thread & 7;
   const T* base = static_cast<const T*>(x.p) + head * x.head;
 #pragma unroll 4
-  for (int r = thread >> 3; r < kLongTile; r += 16) {
+  for (int r = thread >> 3; r < ROWS; r += 16) {
     const int pos = pos0 + r;
     const bool real = pos < end;
     const T* from = base + (real ? row_of(a, pos) * x.row : 0);
@@ -37,7 +37,7 @@ __device__ __forceinline__ void copy_long_tile(const Problem& a, const View& x, 
     for (int b = 0; b < DP / 64; ++b) {
       const int column = b * 64 + piece * 8;
       const bool on = real && column < a.dim;
-      copy16(to + b * (kLongTile * 128) + r * 128 + ((piece ^ (r & 7)) << 4), from + (on ? column : 0), on ? 16 : 0);
+      copy16(to + b * (ROWS * 128) + r * 128 + ((piece ^ (r & 7)) << 4), from + (on ? column : 0), on ? 16 : 0);
     }
   }
 }

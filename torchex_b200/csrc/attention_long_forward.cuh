@@ -1,18 +1,19 @@
 // Forward kernel of the attention within segments for long segments, on the 5th-generation tensor cores.
 //
-// A CTA owns 256 query positions of one head, as two tiles of 128, and walks the keys they see in tiles of
-// 128.  Scores and outputs live in tensor memory (2 x 128 columns of scores, 2 x DP of outputs), queries,
-// keys and values in shared memory (keys and values in two stages each).  Sixteen warps:
+// A CTA owns 256 query positions of one head, as two tiles of 128, and walks the keys they see in tiles of 64.
+// Scores and outputs live in tensor memory (two buffers of 64 columns of scores and DP columns of outputs for each
+// query tile), queries, keys and values in shared memory (keys and values in four stages each).  Sixteen warps:
 //   0-3, 4-7 : softmax of query tile 0 and 1, one row per thread.  A thread reads its row of scores, and
 //              writes its probabilities over them in 16 bits, where the second product takes them from;
 //   8-11     : copies of rows into shared memory: rows that lie in segment order by the copy engine, a tile
-//              of 64 columns by 128 rows at a time (one thread); rows that come through the plan's permutation
-//              16 bytes at a time, by all four warps;
-//   12, 13   : one thread each issues the products of query tile 0 and 1.  While one tile's softmax runs, the
-//              other tile's products do.
+//              of 64 columns at a time (one thread); rows that come through the plan's permutation 16 bytes at a
+//              time, by all four warps;
+//   12, 13   : one thread each issues the products of query tile 0 and 1.
+// While the softmax works on one buffer of scores, the products of the other one run (with one buffer of 128 columns
+// per query tile the softmax waited 1600 of every 4300 cycles for the products between two of its tiles).
 // The outputs are rescaled only when a row's maximum has grown by more than 2^8 (the sums carry the stale
 // maximum until then: probabilities up to 2^8 lose nothing in fp32 sums), which is rare after the first tiles.
-// Bound: exponentials.  128 x 128 of them take 1024 cycles of an SM, the two products of that tile 512 at
+// Bound: exponentials.  128 x 128 of them take 1024 cycles of an SM, the two products of that many 512 at
 // the tensor cores' nominal rate.
 #pragma once
 
@@ -25,11 +26,12 @@ constexpr float kStale = 8.f;  // growth of a row's maximum, in units of log2, t
 
 template <int DP>
 struct LongForwardMemory {
-  static constexpr int kTile = kLongTile * DP * 2;
-  static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile;
-  static constexpr int kBarriers = 6 * kTile;
+  static constexpr int kKeys = 64, kStages = 4;
+  static constexpr int kTile = kLongTile * DP * 2, kStage = kKeys * DP * 2;
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kStage;
+  static constexpr int kBarriers = kV + kStages * kStage;
   static constexpr int kBytes = kBarriers + 256 + 1024;  // and room to align the start to 1024 bytes
-  static constexpr int kScores = 0, kOut = 2 * kLongTile, kColumns = 512;  // tensor memory
+  static constexpr int kScores = 0, kOut = 4 * kKeys, kColumns = 512;  // tensor memory
 };
 
 struct LongRange {  // of a query tile: the tiles of keys that some row sees, and those that all rows see
@@ -47,6 +49,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
 long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ Maps maps) {
   extern __shared__ unsigned char raw[];
   using M = LongForwardMemory<DP>;
+  constexpr int N = M::kKeys, S = M::kStages;
   unsigned char* smem = raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023);
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;
@@ -56,28 +59,33 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
   const LongRange range[2] = {range_of(a, pos0), range_of(a, pos0 + kLongTile)};
   const int first_key = range[0].begin, end_key = max(range[0].end, range[1].end);
-  const int tiles = (end_key - first_key + kLongTile - 1) / kLongTile;
+  const int tiles = (end_key - first_key + N - 1) / N;
   // boxes are copied whole: the last one may hold rows behind the last key, which must be finite as well
-  if (any_flag(a, a.bad_v, kv, first_key, min(a.n, first_key + tiles * kLongTile))) {
+  if (any_flag(a, a.bad_v, kv, first_key, min(a.n, first_key + tiles * N))) {
     plain_forward<T>(a, pos0, kLongRows, head);
     return;
   }
   const uint32_t base = t5::smem_u32(smem);
   auto bar = [&](int i) { return base + M::kBarriers + i * 8; };
-  // barriers: 0 queries full; 1-2 keys full, 3-4 keys empty, 5-6 values full, 7-8 values empty (by stage);
-  // 9-10 scores full, 11-12 probabilities full, 13-14 outputs done (by query tile)
+  // barriers by stage: keys full, keys empty, values full, values empty; by query tile and buffer: scores full,
+  // probabilities full, outputs done
+  enum { kQueries = 0, kKeysFull = 1, kKeysEmpty = kKeysFull + S, kValuesFull = kKeysEmpty + S, kValuesEmpty = kValuesFull + S,
+         kScoresFull = kValuesEmpty + S, kWeightsFull = kScoresFull + 4, kDone = kWeightsFull + 4, kSettle = kDone + 4 };
+  static_assert((kSettle + 2) * 8 <= 256, "room for the barriers");
   if (threadIdx.x == 0) {
     s_dead = 0;
-    const int copiers = maps.used ? 1 : 128;
-    t5::barrier_init(bar(0), copiers);
-    for (int s = 0; s < 2; ++s) {
-      t5::barrier_init(bar(1 + s), copiers);
-      t5::barrier_init(bar(3 + s), 2);
-      t5::barrier_init(bar(5 + s), copiers);
-      t5::barrier_init(bar(7 + s), 2);
-      t5::barrier_init(bar(9 + s), 1);
-      t5::barrier_init(bar(11 + s), 128);
-      t5::barrier_init(bar(13 + s), 1);
+    const int copiers = maps.used ? 1 : 4;
+    t5::barrier_init(bar(kQueries), copiers);
+    for (int s = 0; s < S; ++s) {
+      t5::barrier_init(bar(kKeysFull + s), copiers);
+      t5::barrier_init(bar(kKeysEmpty + s), 2);
+      t5::barrier_init(bar(kValuesFull + s), copiers);
+      t5::barrier_init(bar(kValuesEmpty + s), 2);
+    }
+    for (int s = 0; s < 4; ++s) {
+      t5::barrier_init(bar(kScoresFull + s), 1);
+      t5::barrier_init(bar(kWeightsFull + s), 4);
+      t5::barrier_init(bar(kDone + s), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -87,58 +95,58 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   t5::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   volatile int* dead = &s_dead;
-  auto sees = [&](int w, int j) {  // whether query tile w sees some key of tile j
-    const int j0 = first_key + j * kLongTile;
-    return j < tiles && j0 < range[w].end && j0 + kLongTile > range[w].begin;
-  };
+  // This warp's query tile, and the tiles of keys that some row of it sees: from `from` on, before `until`.  In
+  // registers: looked up by an index in the loops below they took 400 cycles of every 2000.
+  const int w = warp < 8 ? warp >> 2 : warp & 1;
+  const LongRange mine = w ? range[1] : range[0];
+  const int from_tile = mine.end > mine.begin ? (mine.begin - first_key) / N : 0;
+  const int until_tile = mine.end > mine.begin ? (mine.end - first_key + N - 1) / N : 0;
 
   if (warp < 8) {  // ---- softmax
-    t5::more_registers<184>();
-    const int w = warp >> 2, row = threadIdx.x & 127, i = pos0 + w * kLongTile + row;
+    const int row = threadIdx.x & 127, i = pos0 + w * kLongTile + row;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t scores = tmem + lanes + M::kScores + w * kLongTile, sums = tmem + lanes + M::kOut + w * DP;
+    const uint32_t sums = tmem + lanes + M::kOut + w * DP;
     const Bounds see = keys_of(a, i);
     const float unit = a.unit, slope = GENERAL ? slope_of(a, head) : 0.f;
-    float top = -INFINITY, sum = 0.f;  // in units of log2
-    int done = 0;                      // tiles of this query tile so far
-    bool alive = true;
-    for (int j = 0; j < tiles; ++j) {
-      if (!sees(w, j)) continue;
-      alive = __all_sync(0xffffffffu, t5::barrier_wait(bar(9 + w), done & 1, dead));
-      if (!alive) break;
-      t5::fence_after_sync();
-      float s[kLongTile];
+    float top = -INFINITY;  // in units of log2
+    float2 sum = {0.f, 0.f};
+    int done = 0;           // tiles of this query tile so far
+    for (int j = from_tile; j < until_tile; ++j) {
+      const int buffer = 2 * w + (done & 1);
+      const uint32_t scores = tmem + lanes + M::kScores + buffer * N;
+      t5::warp_wait(bar(kScoresFull + buffer), (done >> 1) & 1, dead);
+      float s[N];
 #pragma unroll
-      for (int c = 0; c < kLongTile; c += 32) t5::tmem_load32(scores + c, reinterpret_cast<float(&)[32]>(s[c]));
+      for (int c = 0; c < N; c += 32) t5::tmem_load32(scores + c, reinterpret_cast<float(&)[32]>(s[c]));
       t5::tmem_wait_loads();
-      const int j0 = first_key + j * kLongTile;
+      const int j0 = first_key + j * N;
       if constexpr (GENERAL) {
 #pragma unroll
-        for (int c = 0; c < kLongTile; ++c) s[c] = score_of<true>(a, s[c], slope, float(i - j0) - float(c)).x;
+        for (int c = 0; c < N; ++c) s[c] = score_of<true>(a, s[c], slope, float(i - j0) - float(c)).x;
       }
-      if (!(j0 >= range[w].all_begin && j0 + kLongTile <= range[w].all_end && pos0 + (w + 1) * kLongTile <= a.n)) {
+      if (!(j0 >= mine.all_begin && j0 + N <= mine.all_end)) {
         const int from = see.begin - j0, to = see.end - j0;
 #pragma unroll
-        for (int c = 0; c < kLongTile; ++c) s[c] = c >= from && c < to ? s[c] : -INFINITY;
+        for (int c = 0; c < N; ++c) s[c] = c >= from && c < to ? s[c] : -INFINITY;
       }
       float most[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < kLongTile; ++c) most[c & 3] = fmaxf(most[c & 3], s[c]);
+      for (int c = 4; c + 1 < N; c += 2) most[(c >> 1) & 3] = t5::max3(most[(c >> 1) & 3], s[c], s[c + 1]);
       float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
       if constexpr (!GENERAL) now *= unit;  // the scale is positive here
       if (done == 0) {
         top = now;
       } else if (__any_sync(0xffffffffu, now > top + kStale)) {
         // rescale this warp's rows: the product that last added to them must be done
-        alive = __all_sync(0xffffffffu, t5::barrier_wait(bar(13 + w), (done - 1) & 1, dead));
-        if (!alive) break;
-        t5::fence_after_sync();
+        const int last = done - 1;
+        t5::warp_wait(bar(kDone + 2 * w + (last & 1)), (last >> 1) & 1, dead);
         const float next = fmaxf(top, now);
         const float shrink = next == -INFINITY ? 1.f : exp2_fast(top - next);
         top = next;
-        sum *= shrink;
+        sum.x *= shrink;
+        sum.y *= shrink;
 #pragma unroll
-        for (int c = 0; c < DP; c += 16) {  // 16 at a time: the row of scores is in registers as well
+        for (int c = 0; c < DP; c += 16) {
           float o[16];
           t5::tmem_load16(sums + c, o);
           t5::tmem_wait_loads();
@@ -148,152 +156,141 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
         }
       }
       const float less = top == -INFINITY ? 0.f : top;  // a row without a visible key so far: weights 0, not NaN
-      float part[4] = {};
+      const float2 factor = {GENERAL ? 1.f : unit, GENERAL ? 1.f : unit}, shift = {-less, -less};
+      float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-      for (int c = 0; c < kLongTile; c += 32) {
+      for (int c = 0; c < N; c += 32) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float x0 = exp2_fast(GENERAL ? s[c + e] - less : fmaf(s[c + e], unit, -less));
-          const float x1 = exp2_fast(GENERAL ? s[c + e + 1] - less : fmaf(s[c + e + 1], unit, -less));
-          part[e & 2] += x0;
-          part[(e & 2) + 1] += x1;
-          p[e / 2] = pack2<T>(x0, x1);
+          const float2 x = t5::fma2({s[c + e], s[c + e + 1]}, factor, shift);
+          const float2 y = {exp2_fast(x.x), exp2_fast(x.y)};
+          part[(e >> 1) & 1] = t5::add2(part[(e >> 1) & 1], y);
+          p[e / 2] = pack2<T>(y.x, y.y);
         }
         t5::tmem_store16(scores + c / 2, p);
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      sum = t5::add2(sum, t5::add2(part[0], part[1]));
       t5::tmem_wait_stores();
       t5::fence_before_sync();
-      t5::barrier_arrive(bar(11 + w));
+      t5::warp_arrive(bar(kWeightsFull + buffer));
       ++done;
     }
-    if (done > 0 && alive) {
-      alive = __all_sync(0xffffffffu, t5::barrier_wait(bar(13 + w), (done - 1) & 1, dead));
-      t5::fence_after_sync();
-      if (alive) {
-        const bool there = i < a.n;
-        const float factor = see.end > see.begin ? 1.f / sum : 0.f;
-        if (there && a.lse) a.lse[int64_t(head) * a.n + i] = see.end > see.begin ? top + log2f(sum) : 0.f;
-        T* to = row_at<T>(a, a.out, head, min(i, a.n - 1));
-        T* low = a.out_low.p ? row_at<T>(a, a.out_low, head, min(i, a.n - 1)) : nullptr;
+    if (done > 0) {
+      const int last = done - 1;  // products are done in order: the last one means all
+      t5::warp_wait(bar(kDone + 2 * w + (last & 1)), (last >> 1) & 1, dead);
+      const bool there = i < a.n;
+      const float total = sum.x + sum.y, factor = see.end > see.begin ? 1.f / total : 0.f;
+      if (there && a.lse) a.lse[int64_t(head) * a.n + i] = see.end > see.begin ? top + log2f(total) : 0.f;
+      T* to = row_at<T>(a, a.out, head, min(i, a.n - 1));
+      T* low = a.out_low.p ? row_at<T>(a, a.out_low, head, min(i, a.n - 1)) : nullptr;
 #pragma unroll
-        for (int c = 0; c < DP; c += 32) {
-          float o[32];
-          t5::tmem_load32(sums + c, o);
-          t5::tmem_wait_loads();
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        t5::tmem_load32(sums + c, o);
+        t5::tmem_wait_loads();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (there && c + e < a.dim) {
-              Chunk<T, 16> high, rest;
+        for (int e = 0; e < 32; e += 8) {
+          if (there && c + e < a.dim) {
+            Chunk<T, 16> high, rest;
 #pragma unroll
-              for (int x = 0; x < 8; ++x) {
-                const float y = o[e + x] * factor;
-                high.v[x] = narrow<T>(y);
-                rest.v[x] = narrow<T>(y - widen<T>(high.v[x]));
-              }
-              store_chunk<T, 16>(to + c + e, high);
-              if (low) store_chunk<T, 16>(low + c + e, rest);
+            for (int x = 0; x < 8; ++x) {
+              const float y = o[e + x] * factor;
+              high.v[x] = narrow<T>(y);
+              rest.v[x] = narrow<T>(y - widen<T>(high.v[x]));
             }
+            store_chunk<T, 16>(to + c + e, high);
+            if (low) store_chunk<T, 16>(low + c + e, rest);
           }
         }
       }
     }
   } else if (warp < 12) {  // ---- copies: queries and the first keys, then values and keys in turn
-    t5::fewer_registers<72>();
     // item 0: queries and keys of tile 0; item 2 j + 1: values of tile j; item 2 j: keys of tile j
     auto announce = [&](int item) {
       t5::fence_copies();
-      if (item == 0) t5::barrier_arrive(bar(0));
-      t5::barrier_arrive(bar((item & 1 ? 5 : 1) + ((item >> 1) & 1)));
+      if (item == 0) t5::warp_arrive(bar(kQueries));
+      t5::warp_arrive(bar((item & 1 ? kValuesFull : kKeysFull) + (item >> 1) % S));
     };
     const int items = 2 * tiles;
-    bool alive = true;
     if (maps.used) {
       if (warp == 8 && t5::elect_one()) {
-        auto box = [&](const CUtensorMap& map, uint32_t to, int full, int h, int pos) {
+        auto box = [&](const CUtensorMap& map, uint32_t to, int rows, int full, int h, int pos) {
 #pragma unroll
-          for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (kLongTile * 128), &map, bar(full), b * 64, h, pos);
+          for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (rows * 128), &map, bar(full), b * 64, h, pos);
         };
         for (int item = 0; item < items; ++item) {
-          const int j = item >> 1, stage = j & 1, pos = first_key + j * kLongTile, full = (item & 1 ? 5 : 1) + stage;
-          if (j >= 2 && !t5::barrier_wait(bar((item & 1 ? 7 : 3) + stage), ((j >> 1) - 1) & 1, dead)) break;
+          const int j = item >> 1, stage = j % S, pos = first_key + j * N, full = (item & 1 ? kValuesFull : kKeysFull) + stage;
+          if (j >= S) t5::barrier_wait(bar((item & 1 ? kValuesEmpty : kKeysEmpty) + stage), (j / S - 1) & 1, dead);
           if (item == 0) {
-            t5::barrier_arrive_expect(bar(0), 2 * M::kTile);
-            box(maps.q, base + M::kQ, 0, head, pos0);
-            box(maps.q, base + M::kQ + M::kTile, 0, head, pos0 + kLongTile);
+            t5::barrier_arrive_expect(bar(kQueries), 2 * M::kTile);
+            for (int t = 0; t < 2; ++t) box(maps.q, base + M::kQ + t * M::kTile, kLongTile, kQueries, head, pos0 + t * kLongTile);
           }
-          t5::barrier_arrive_expect(bar(full), M::kTile);
-          if (item & 1) box(maps.v, base + M::kV + stage * M::kTile, full, kv, pos);
-          else box(maps.k, base + M::kK + stage * M::kTile, full, kv, pos);
+          t5::barrier_arrive_expect(bar(full), M::kStage);
+          if (item & 1) box(maps.v, base + M::kV + stage * M::kStage, N, full, kv, pos);
+          else box(maps.k, base + M::kK + stage * M::kStage, N, full, kv, pos);
         }
       }
     }
+    constexpr int kLag = 4;  // items under way
     for (int item = maps.used ? items : 0; item < items; ++item) {
-      const int j = item >> 1, stage = j & 1, pos = first_key + j * kLongTile;
-      if (j >= 2) {
-        alive = __all_sync(0xffffffffu, t5::barrier_wait(bar((item & 1 ? 7 : 3) + stage), ((j >> 1) - 1) & 1, dead));
-        if (!alive) break;
-      }
+      const int j = item >> 1, stage = j % S, pos = first_key + j * N;
+      if (j >= S) t5::warp_wait(bar((item & 1 ? kValuesEmpty : kKeysEmpty) + stage), (j / S - 1) & 1, dead);
       if (item == 0) {
-        copy_long_tile<T, DP>(a, a.q, head, pos0, a.n, base + M::kQ);
-        copy_long_tile<T, DP>(a, a.q, head, pos0 + kLongTile, a.n, base + M::kQ + M::kTile);
+        for (int t = 0; t < 2; ++t) copy_long_tile<T, DP, kLongTile>(a, a.q, head, pos0 + t * kLongTile, a.n, base + M::kQ + t * M::kTile);
       }
-      if (item & 1) copy_long_tile<T, DP>(a, a.v, kv, pos, end_key, base + M::kV + stage * M::kTile);
-      else copy_long_tile<T, DP>(a, a.k, kv, pos, end_key, base + M::kK + stage * M::kTile);
+      if (item & 1) copy_long_tile<T, DP, N>(a, a.v, kv, pos, end_key, base + M::kV + stage * M::kStage);
+      else copy_long_tile<T, DP, N>(a, a.k, kv, pos, end_key, base + M::kK + stage * M::kStage);
       commit_copies();
-      if (item >= 2) {
-        wait_copies<2>();
-        announce(item - 2);
+      if (item >= kLag) {
+        wait_copies<kLag>();
+        announce(item - kLag);
       }
     }
-    if (alive && !maps.used) {
+    if (!maps.used) {
       wait_copies<0>();
-      for (int late = max(0, items - 2); late < items; ++late) announce(late);
+      for (int late = max(0, items - kLag); late < items; ++late) announce(late);
     }
-    wait_copies<0>();
   } else {
-    t5::fewer_registers<72>();
     if (warp < 14 && t5::elect_one()) {  // ---- products
-      constexpr uint32_t score_instr = t5::instruction<T>(128, kLongTile, false), out_instr = t5::instruction<T>(128, DP, true);
-      const int w = warp - 12;
-      const uint32_t scores = tmem + M::kScores + w * kLongTile, sums = tmem + M::kOut + w * DP;
-      int done = 0;
-      // Scores of tile j.  Either way the keys' stage is given back, if it is filled again: nothing may arrive at
+      constexpr uint32_t score_instr = t5::instruction<T>(128, N, false), out_instr = t5::instruction<T>(128, DP, true);
+      const uint32_t sums = tmem + M::kOut + w * DP;
+      int scored = 0, done = 0;
+      auto buffer_of = [&](int count) { return tmem + M::kScores + (2 * w + (count & 1)) * N; };
+      // Scores of tile j.  The keys' stage is given back in any case, if it is filled again: nothing may arrive at
       // a barrier that nobody waits for any more.
       auto score = [&](int j) {
-        if (!t5::barrier_wait(bar(1 + (j & 1)), (j >> 1) & 1, dead)) return false;
+        t5::barrier_wait(bar(kKeysFull + j % S), (j / S) & 1, dead);
         t5::fence_after_sync();
-        if (sees(w, j)) {
-          t5::multiply_columns<DP>(scores, base + M::kQ + w * M::kTile, kLongTile, base + M::kK + (j & 1) * M::kTile, kLongTile, score_instr);
-          t5::commit(bar(9 + w));
+        if (j >= from_tile && j < until_tile) {
+          t5::multiply_columns<DP>(buffer_of(scored), base + M::kQ + w * M::kTile, kLongTile, base + M::kK + (j % S) * M::kStage, N, score_instr);
+          t5::commit(bar(kScoresFull + 2 * w + (scored & 1)));
+          ++scored;
         }
-        if (j + 2 < tiles) t5::commit(bar(3 + (j & 1)));
-        return true;
+        if (j + S < tiles) t5::commit(bar(kKeysEmpty + j % S));
       };
-      bool alive = tiles == 0 || (t5::barrier_wait(bar(0), 0, dead) && score(0));
-      for (int j = 0; alive && j < tiles; ++j) {
-        alive = t5::barrier_wait(bar(5 + (j & 1)), (j >> 1) & 1, dead);
-        if (alive && sees(w, j)) {
-          alive = t5::barrier_wait(bar(11 + w), done & 1, dead);
-          if (!alive) break;
+      t5::barrier_wait(bar(kQueries), 0, dead);
+      for (int j = 0; j < min(2, tiles); ++j) score(j);
+      for (int j = 0; j < tiles; ++j) {
+        t5::barrier_wait(bar(kValuesFull + j % S), (j / S) & 1, dead);
+        if (j >= from_tile && j < until_tile) {
+          t5::barrier_wait(bar(kWeightsFull + 2 * w + (done & 1)), (done >> 1) & 1, dead);
           t5::fence_after_sync();
-          t5::multiply_rows<kLongTile>(sums, scores, base + M::kV + (j & 1) * M::kTile, out_instr, done > 0);
-          t5::commit(bar(13 + w));
+          t5::multiply_rows<N>(sums, buffer_of(done), base + M::kV + (j % S) * M::kStage, out_instr, done > 0);
+          t5::commit(bar(kDone + 2 * w + (done & 1)));
           ++done;
         }
-        if (!alive) break;
-        if (j + 2 < tiles) t5::commit(bar(7 + (j & 1)));
+        if (j + S < tiles) t5::commit(bar(kValuesEmpty + j % S));
         // products of one thread are done in the order of their issue: the scores may overwrite the probabilities
-        if (j + 1 < tiles) alive = score(j + 1);
+        if (j + 2 < tiles) score(j + 2);
       }
     }
   }
   // All products and copies have been waited for, except after a wait that gave up: then what is still under
-  // way ends within the memory that this CTA holds.
+  // way must end within the memory that this CTA holds.
   t5::fence_before_sync();
   __syncthreads();
-  if (s_dead) t5::settle(bar(15 + (warp & 1)), (warp == 12 || warp == 13) && t5::elect_one(), &g_wait_timeouts);
+  if (s_dead) t5::settle(bar(kSettle + (warp & 1)), (warp == 12 || warp == 13) && t5::elect_one(), &g_wait_timeouts);
   __syncthreads();
   t5::fence_after_sync();
   if (warp == 12) t5::tmem_free(tmem, M::kColumns);
@@ -306,8 +303,9 @@ int launch_long_forward(const Problem& a, int dtype, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "attention long_forward_kernel: %s", cudaGetErrorString(e));
   Maps maps = {};
-  maps.used = a.perm == nullptr && make_map(&maps.q, a, a.q, a.heads, kLongTile, dtype) && make_map(&maps.k, a, a.k, a.kv_heads, kLongTile, dtype) &&
-              make_map(&maps.v, a, a.v, a.kv_heads, kLongTile, dtype);
+  constexpr int keys = LongForwardMemory<DP>::kKeys;
+  maps.used = a.perm == nullptr && make_map(&maps.q, a, a.q, a.heads, kLongTile, dtype) && make_map(&maps.k, a, a.k, a.kv_heads, keys, dtype) &&
+              make_map(&maps.v, a, a.v, a.kv_heads, keys, dtype);
   const dim3 grid(unsigned((a.n + kLongRows - 1) / kLongRows), unsigned(a.heads));
   kernel<<<grid, kLongThreads, bytes, stream>>>(a, maps);
   return check_launch("attention long_forward_kernel");

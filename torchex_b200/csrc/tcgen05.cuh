@@ -27,6 +27,12 @@ __device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
 __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// One arrival for the whole (converged) warp, behind what all its lanes did: 32 arrivals at one word are done one
+// after the other, and the warp's next wait queues behind them.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) barrier_arrive(bar);
+}
 __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -34,18 +40,25 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Waits, for a bounded number of polls, until the phase of that parity is complete.  When the polls run out
-// or another thread's have (`*dead`), it gives up: the caller leaves its loop, and the kernel tears down and
-// returns instead of hanging.
+// Waits, for a bounded number of polls, until the phase of that parity is complete.  When the polls run out,
+// or another thread's have (`*dead`), it returns all the same: the kernel then runs to its end on whatever its
+// memory holds, every later wait returning at once, counts the event (texb_device_status, wait_timeouts) and
+// returns, instead of hanging.
 constexpr int kPolls = 1 << 20;
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (barrier_try(bar, parity)) return true;
+__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (barrier_try(bar, parity)) return;
   for (int i = 0; i < kPolls; ++i) {
-    if (barrier_try(bar, parity)) return true;
-    if (*dead) return false;
+    if (barrier_try(bar, parity)) return;
+    if (*dead) return;
   }
   *dead = 1;
-  return false;
+}
+// The same by all lanes of a warp, which are together again behind it; what the tensor cores did before the phase
+// completed is visible.
+__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  barrier_wait(bar, parity, dead);
+  __syncwarp();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
 // Also expects `bytes` of copies in this phase.
@@ -101,6 +114,31 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- arithmetic on pairs, and of three -----------------------------------------------------------------
+__device__ __forceinline__ float max3(float a, float b, float c) {  // a NaN is passed over, as by fmaxf
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)),
+      "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)),
+      "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)),
+      "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
 
 // ---- matrix products ---------------------------------------------------------------------------------
 // Descriptor of an operand tile: swizzle of 128 bytes (2 in the top bits), descriptor version 1, 8-row groups
