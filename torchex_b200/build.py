@@ -33,7 +33,7 @@ SOURCES = ["abi.cu", "segment_reduce.cu", "reduce_unit_sum.cu", "reduce_unit_sum
            "reduce_unit_sum_max.cu", "segment_small.cu", "segment_plan.cu", "segment_backward.cu", "peer_copy.cu",
            "embedding.cu", "embedding_backward.cu", "grad_clip.cu", "attention.cu",
            *(f"attention_{way}_{dim}.cu" for way in ("forward", "backward") for dim in (16, 32, 64, 128)),
-           "attention_long_forward_64.cu", "attention_long_forward_128.cu"]
+           *(f"attention_long_{way}_{dim}.cu" for way in ("forward", "backward") for dim in (64, 128))]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

@@ -10,6 +10,8 @@ template <int DP> int forward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int backward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int long_forward_by_type(const Problem&, int, bool, cudaStream_t);
 template <int DP> int long_forward_timeouts(int*);
+template <int DP> int long_backward_by_type(const Problem&, int, bool, cudaStream_t);
+template <int DP> int long_backward_timeouts(int*);
 
 bool make_map(CUtensorMap* map, const Problem& a, const View& x, int heads, int box_rows, int dtype) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -43,7 +45,7 @@ __global__ void __launch_bounds__(kThreads) flag_values_kernel(const __grid_cons
   if (threadIdx.x == 0) flags[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = bad;
 }
 
-// delta_i = g_i . o_i for the backward pass, and the flags of its blocks: of the queries or gradients of
+// delta_i = scale g_i . o_i for the backward pass, and the flags of its blocks: of the queries or gradients of
 // a head (blockIdx.y < heads), or of the keys of a kv head.  Bound by HBM: q, g, o and k are read once.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -79,7 +81,7 @@ prepare_backward_kernel(const __grid_constant__ Problem a, float* __restrict__ d
       }
     }
     for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (pos < end && sub == 0) delta[int64_t(y) * a.n + pos] = sum;
+    if (pos < end && sub == 0) delta[int64_t(y) * a.n + pos] = sum * a.scale;
   }
   bad = __syncthreads_or(bad);
   if (threadIdx.x == 0) bad_q[int64_t(y) * gridDim.x + blockIdx.x] = bad;
@@ -123,12 +125,16 @@ inline bool long_segments(const Problem& a) { return a.n >= int64_t(a.segments) 
 }  // namespace attention
 
 int attention_timeouts_impl(int* count) {
-  int total = 0, one = 0;
-  int st = attention::long_forward_timeouts<64>(&one);
-  total += one;
-  if (st == TEXB_OK) st = attention::long_forward_timeouts<128>(&one);
-  *count = total + one;
-  return st;
+  int (*const units[])(int*) = {attention::long_forward_timeouts<64>, attention::long_forward_timeouts<128>,
+                                attention::long_backward_timeouts<64>, attention::long_backward_timeouts<128>};
+  *count = 0;
+  for (auto unit : units) {
+    int one = 0;
+    const int st = unit(&one);
+    if (st != TEXB_OK) return st;
+    *count += one;
+  }
+  return TEXB_OK;
 }
 
 size_t attention_workspace_bytes_impl(int64_t n, int heads, int kv_heads, int backward) {
@@ -247,6 +253,10 @@ int attention_backward_impl(const texb_attention_problem* t, void* workspace, si
   st = check_launch("attention prepare_backward_kernel");
   if (st != TEXB_OK) return st;
   const bool general = a.cap > 0.f || a.slopes != nullptr;
+  if (long_segments(a)) {
+    if (a.dim <= 64) return long_backward_by_type<64>(a, dtype, general, stream);
+    return long_backward_by_type<128>(a, dtype, general, stream);
+  }
   if (a.dim <= 16) return backward_by_type<16>(a, dtype, general, stream);
   if (a.dim <= 32) return backward_by_type<32>(a, dtype, general, stream);
   if (a.dim <= 64) return backward_by_type<64>(a, dtype, general, stream);

@@ -46,7 +46,7 @@ struct Problem {
   float* lse;                // [heads, n] by position, in units of log2; forward may leave it out
   // backward
   View g;                    // gradient of out
-  const float* delta;        // [heads, n] by position: g_i . o_i
+  const float* delta;        // [heads, n] by position: scale * g_i . o_i
   View gq, gk, gv;
   // flags of blocks with a value that is not finite, [.., ceil(n / kBlock)]; NULL: look for oneself
   const uint8_t *bad_v, *bad_k;  // per kv head
@@ -415,7 +415,7 @@ __device__ __forceinline__ Pair pair_of(const Problem& a, const T* qi, const T* 
                                         float slope) {
   const Score s = score_of<true>(a, dot<T>(qi, kj, a.dim), slope, float(i - j));
   const float p = exp2f(s.x - a.lse[int64_t(head) * a.n + i]);
-  return {p, p * (dot<T>(gi, vj, a.dim) - a.delta[int64_t(head) * a.n + i]) * (s.slope * a.scale)};
+  return {p, p * (dot<T>(gi, vj, a.dim) * a.scale - a.delta[int64_t(head) * a.n + i]) * s.slope};
 }
 
 template <typename T>

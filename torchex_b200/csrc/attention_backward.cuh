@@ -7,7 +7,7 @@
 //   keys   : 64 key positions of one kv head against the queries that see them, of all query heads
 //            that share it -- the gradient of a shared key or value is one sum.
 // With P and dS rounded to the inputs' type before their products (half a step each):
-//   dS = P (g v - delta) x (derivative of the capped score) x scale,  gq = dS k, gk = dS^T q, gv = P^T g.
+//   dS = P (scale g v - delta) x (derivative of the capped score), delta = scale g o,  gq = dS k, gk = dS^T q, gv = P^T g.
 // A masked pair's dS is set to 0, not multiplied by 0: its g v may be infinite.
 #pragma once
 
@@ -77,8 +77,8 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_c
         for (int e = 0; e < 2; ++e) {
           const int j = j0 + t * 8 + (lane & 3) * 2 + e;
           const Score x0 = score_of<GENERAL>(a, s[t][e], slope, float(i0 - j)), x1 = score_of<GENERAL>(a, s[t][2 + e], slope, float(i1 - j));
-          const float d0 = exp2_fast(x0.x - lse0) * (dp[t][e] - delta0) * (x0.slope * a.scale);
-          const float d1 = exp2_fast(x1.x - lse1) * (dp[t][2 + e] - delta1) * (x1.slope * a.scale);
+          const float d0 = exp2_fast(x0.x - lse0) * fmaf(dp[t][e], a.scale, -delta0) * x0.slope;
+          const float d1 = exp2_fast(x1.x - lse1) * fmaf(dp[t][2 + e], a.scale, -delta1) * x1.slope;
           dp[t][e] = j >= see0.begin && j < see0.end ? d0 : 0.f;
           dp[t][2 + e] = j >= see1.begin && j < see1.end ? d1 : 0.f;
         }
@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
           const bool on0 = i >= seen0.begin && i < seen0.end, on1 = i >= seen1.begin && i < seen1.end;
           p[t][e] = on0 ? exp2_fast(x0.x - lse) : 0.f;
           p[t][2 + e] = on1 ? exp2_fast(x1.x - lse) : 0.f;
-          ds[t][e] = on0 ? p[t][e] * (ds[t][e] - delta) * (x0.slope * a.scale) : 0.f;
-          ds[t][2 + e] = on1 ? p[t][2 + e] * (ds[t][2 + e] - delta) * (x1.slope * a.scale) : 0.f;
+          ds[t][e] = on0 ? p[t][e] * fmaf(ds[t][e], a.scale, -delta) * x0.slope : 0.f;
+          ds[t][2 + e] = on1 ? p[t][2 + e] * fmaf(ds[t][2 + e], a.scale, -delta) * x1.slope : 0.f;
         }
       }
       product_probabilities<T, DP, NT>(gv, p, tg);

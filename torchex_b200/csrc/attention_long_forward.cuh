@@ -60,6 +60,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   const LongRange range[2] = {range_of(a, pos0), range_of(a, pos0 + kLongTile)};
   const int first_key = range[0].begin, end_key = max(range[0].end, range[1].end);
   const int tiles = (end_key - first_key + N - 1) / N;
+  if (tiles <= 0) return;  // a plan without the row itself in its segment
   // boxes are copied whole: the last one may hold rows behind the last key, which must be finite as well
   if (any_flag(a, a.bad_v, kv, first_key, min(a.n, first_key + tiles * N))) {
     plain_forward<T>(a, pos0, kLongRows, head);
