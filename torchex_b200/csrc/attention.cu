@@ -6,11 +6,11 @@
 namespace texb {
 namespace attention {
 
-template <int DP> int forward_by_type(const Problem&, int, bool, cudaStream_t);
-template <int DP> int backward_by_type(const Problem&, int, bool, cudaStream_t);
-template <int DP> int long_forward_by_type(const Problem&, int, bool, cudaStream_t);
+template <int DP> int forward_by_type(const Problem&, int, int, cudaStream_t);
+template <int DP> int backward_by_type(const Problem&, int, int, cudaStream_t);
+template <int DP> int long_forward_by_type(const Problem&, int, int, cudaStream_t);
 template <int DP> int long_forward_timeouts(int*);
-template <int DP> int long_backward_by_type(const Problem&, int, bool, cudaStream_t);
+template <int DP> int long_backward_by_type(const Problem&, int, int, cudaStream_t);
 template <int DP> int long_backward_timeouts(int*);
 
 bool make_map(CUtensorMap* map, const Problem& a, const View& x, int heads, int box_rows, int dtype) {
@@ -37,54 +37,80 @@ bool make_map(CUtensorMap* map, const Problem& a, const View& x, int heads, int 
 
 namespace {
 
-// Flags the blocks of kBlock positions that hold a value that is not finite.  One CTA per (block, head).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) flag_values_kernel(const __grid_constant__ Problem a, uint8_t* __restrict__ flags) {
-  const int pos0 = blockIdx.x * kBlock;
-  const bool bad = look_over<T>(a, a.v, blockIdx.y, pos0, min(a.n, pos0 + kBlock));
-  if (threadIdx.x == 0) flags[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = bad;
+// How the threads of a CTA share a block of kFlag positions: `lanes` threads walk one row of one head, and the
+// rows of as many neighbouring heads as fit are taken together, since they lie side by side in memory (one head
+// per CTA reads 256 bytes of every 4 KB).
+struct Spread {
+  int lanes, heads, rows;  // of a row; heads of a CTA; rows of a pass
+};
+inline Spread spread_of(int dim, int heads) {
+  Spread s = {1, 0, 0};
+  while (s.lanes < dim / 8) s.lanes *= 2;
+  const int slots = kThreads / s.lanes;
+  s.heads = heads < slots ? heads : slots;
+  s.rows = slots / s.heads;
+  return s;
 }
 
-// delta_i = scale g_i . o_i for the backward pass, and the flags of its blocks: of the queries or gradients of
-// a head (blockIdx.y < heads), or of the keys of a kv head.  Bound by HBM: q, g, o and k are read once.
-template <typename T>
+// The flags of the blocks of the values (forward: Q_ROWS false, the CTAs along y are groups of kv heads), or, for
+// the backward pass, delta_i = scale g_i . o_i and the flags of the queries or gradients of each head (the first
+// CTAs along y) and of the keys of each kv head.  Bound by HBM: every row is read once.
+template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads)
-prepare_backward_kernel(const __grid_constant__ Problem a, float* __restrict__ delta,
-                        uint8_t* __restrict__ bad_q, uint8_t* __restrict__ bad_k) {
-  const int pos0 = blockIdx.x * kBlock, end = min(a.n, pos0 + kBlock), y = blockIdx.y;
-  if (y >= a.heads) {
-    const int kv = y - a.heads;
-    const bool bad = look_over<T>(a, a.k, kv, pos0, end);
-    if (threadIdx.x == 0) bad_k[int64_t(kv) * gridDim.x + blockIdx.x] = bad;
-    return;
-  }
-  // lanes of a group walk a row: 1, 2, 4, 8 or 16 of them, by the pieces of a row
-  const int pieces = a.dim / 8;
-  int lanes = 1;
-  while (lanes < pieces && lanes < 16) lanes *= 2;
-  const int sub = threadIdx.x & (lanes - 1);
+look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_spread, int q_groups, float* __restrict__ delta,
+                 uint8_t* __restrict__ bad_q, uint8_t* __restrict__ bad_k) {
+  __shared__ int s_bad[kThreads];  // by head of the CTA
+  const int pos0 = blockIdx.x * kFlag, end = min(a.n, pos0 + kFlag);
+  const bool keys = !BACKWARD || int(blockIdx.y) >= q_groups;
+  const Spread sp = keys ? k_spread : q_spread;
+  const int first_head = (keys ? blockIdx.y - q_groups : blockIdx.y) * sp.heads, heads = keys ? a.kv_heads : a.heads;
+  const int sub = threadIdx.x & (sp.lanes - 1), slot = threadIdx.x / sp.lanes, mine = slot % sp.heads, head = first_head + mine;
+  const bool active = slot < sp.heads * sp.rows && head < heads && sub < a.dim / 8;
+  s_bad[threadIdx.x] = 0;
+  __syncthreads();
+  constexpr int kInFlight = 4;  // rows of a thread whose loads are issued together
   bool bad = false;
-  for (int r = threadIdx.x / lanes; r < kBlock; r += kThreads / lanes) {
-    const int pos = pos0 + r;
-    float sum = 0.f;
-    if (pos < end && sub < pieces) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(row_at<T>(a, a.q, y, pos) + sub * 8));
-      const Chunk<T, 16> g = load_chunk<T, 16>(row_at<T>(a, a.g, y, pos) + sub * 8);
-      const Chunk<T, 16> o = load_chunk<T, 16>(row_at<T>(a, a.out, y, pos) + sub * 8);
-      bad |= not_finite<T>(q) || not_finite<T>(reinterpret_cast<const uint4&>(g));
+  for (int r0 = slot / sp.heads; r0 < kFlag; r0 += sp.rows * kInFlight) {
+    uint4 q[kInFlight], g[kInFlight], o[kInFlight], low[kInFlight];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(widen<T>(g.v[e]), widen<T>(o.v[e]), sum);
-      if (a.out_low.p) {  // out itself is rounded: without the rest, delta's error would reach every dS of the row
-        const Chunk<T, 16> low = load_chunk<T, 16>(row_at<T>(a, a.out_low, y, pos) + sub * 8);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(widen<T>(g.v[e]), widen<T>(low.v[e]), sum);
+    for (int k = 0; k < kInFlight; ++k) {
+      q[k] = g[k] = o[k] = low[k] = uint4{0u, 0u, 0u, 0u};
+      const int pos = pos0 + r0 + k * sp.rows;
+      if (active && pos < end) {
+        const int64_t row = row_of(a, pos);
+        auto piece = [&](const View& x) {
+          return __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(x.p) + row * x.row + head * x.head + sub * 8));
+        };
+        q[k] = piece(!BACKWARD ? a.v : keys ? a.k : a.q);
+        if (!keys) {
+          g[k] = piece(a.g);
+          o[k] = piece(a.out);
+          if (a.out_low.p) low[k] = piece(a.out_low);
+        }
       }
     }
-    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (pos < end && sub == 0) delta[int64_t(y) * a.n + pos] = sum * a.scale;
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      bad |= not_finite<T>(q[k]) || not_finite<T>(g[k]);
+      if (keys) continue;
+      // out itself is rounded: without the rest, delta's error would reach every dS of the row
+      float sum = 0.f;
+      const Chunk<T, 16>&gv = reinterpret_cast<const Chunk<T, 16>&>(g[k]), &ov = reinterpret_cast<const Chunk<T, 16>&>(o[k]),
+            &lv = reinterpret_cast<const Chunk<T, 16>&>(low[k]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum = fmaf(widen<T>(gv.v[e]), widen<T>(ov.v[e]), sum);
+        sum = fmaf(widen<T>(gv.v[e]), widen<T>(lv.v[e]), sum);
+      }
+      for (int x = sp.lanes / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      const int pos = pos0 + r0 + k * sp.rows;
+      if (active && sub == 0 && pos < end && r0 + k * sp.rows < kFlag) delta[int64_t(head) * a.n + pos] = sum * a.scale;
+    }
   }
-  bad = __syncthreads_or(bad);
-  if (threadIdx.x == 0) bad_q[int64_t(y) * gridDim.x + blockIdx.x] = bad;
+  if (bad) s_bad[mine] = 1;
+  __syncthreads();
+  if (int(threadIdx.x) < sp.heads && first_head + int(threadIdx.x) < heads)
+    (keys ? bad_k : bad_q)[int64_t(first_head + threadIdx.x) * gridDim.x + blockIdx.x] = uint8_t(s_bad[threadIdx.x]);
 }
 
 int check(const Problem& a, int dtype, bool backward) {
@@ -111,7 +137,7 @@ int check(const Problem& a, int dtype, bool backward) {
   return TEXB_OK;
 }
 
-inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kBlock)); }
+inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kFlag)); }  // of flags
 
 // Segments short enough that a tile looks at the values of its keys itself instead of a pass of its own
 // doing it: at most three tiles of keys.
@@ -208,22 +234,23 @@ int attention_forward_impl(const texb_attention_problem* t, void* workspace, siz
     if (!workspace || workspace_bytes < need)
       return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", need, workspace_bytes);
     uint8_t* flags = static_cast<uint8_t*>(workspace);
-    const dim3 grid(unsigned(blocks_of(a.n)), unsigned(a.kv_heads));
-    if (dtype == TEXB_BFLOAT16) flag_values_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a, flags);
-    else flag_values_kernel<__half><<<grid, kThreads, 0, stream>>>(a, flags);
-    st = check_launch("attention flag_values_kernel");
+    const Spread ks = spread_of(a.dim, a.kv_heads);
+    const dim3 grid(unsigned(blocks_of(a.n)), unsigned(ceil_div(a.kv_heads, ks.heads)));
+    auto look = dtype == TEXB_BFLOAT16 ? look_over_kernel<__nv_bfloat16, false> : look_over_kernel<__half, false>;
+    look<<<grid, kThreads, 0, stream>>>(a, ks, ks, 0, nullptr, nullptr, flags);
+    st = check_launch("attention look_over_kernel");
     if (st != TEXB_OK) return st;
     a.bad_v = flags;
   }
-  const bool general = a.cap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
+  const int mode = mode_of(a);
   if (a.bad_v && long_segments(a)) {
-    if (a.dim <= 64) return long_forward_by_type<64>(a, dtype, general, stream);
-    return long_forward_by_type<128>(a, dtype, general, stream);
+    if (a.dim <= 64) return long_forward_by_type<64>(a, dtype, mode, stream);
+    return long_forward_by_type<128>(a, dtype, mode, stream);
   }
-  if (a.dim <= 16) return forward_by_type<16>(a, dtype, general, stream);
-  if (a.dim <= 32) return forward_by_type<32>(a, dtype, general, stream);
-  if (a.dim <= 64) return forward_by_type<64>(a, dtype, general, stream);
-  return forward_by_type<128>(a, dtype, general, stream);
+  if (a.dim <= 16) return forward_by_type<16>(a, dtype, mode, stream);
+  if (a.dim <= 32) return forward_by_type<32>(a, dtype, mode, stream);
+  if (a.dim <= 64) return forward_by_type<64>(a, dtype, mode, stream);
+  return forward_by_type<128>(a, dtype, mode, stream);
 }
 
 int attention_backward_impl(const texb_attention_problem* t, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
@@ -245,22 +272,22 @@ int attention_backward_impl(const texb_attention_problem* t, void* workspace, si
   a.delta = delta;
   a.bad_q = bad_q;
   a.bad_k = bad_k;
-  const dim3 grid(unsigned(blocks), unsigned(a.heads + a.kv_heads));
-  if (dtype == TEXB_BFLOAT16)
-    prepare_backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a, delta, bad_q, bad_k);
-  else
-    prepare_backward_kernel<__half><<<grid, kThreads, 0, stream>>>(a, delta, bad_q, bad_k);
-  st = check_launch("attention prepare_backward_kernel");
+  const Spread qs = spread_of(a.dim, a.heads), ks = spread_of(a.dim, a.kv_heads);
+  const int q_groups = int(ceil_div(a.heads, qs.heads));
+  const dim3 grid(unsigned(blocks), unsigned(q_groups + ceil_div(a.kv_heads, ks.heads)));
+  auto look = dtype == TEXB_BFLOAT16 ? look_over_kernel<__nv_bfloat16, true> : look_over_kernel<__half, true>;
+  look<<<grid, kThreads, 0, stream>>>(a, qs, ks, q_groups, delta, bad_q, bad_k);
+  st = check_launch("attention look_over_kernel");
   if (st != TEXB_OK) return st;
-  const bool general = a.cap > 0.f || a.slopes != nullptr;
+  const int mode = mode_of(a);
   if (long_segments(a)) {
-    if (a.dim <= 64) return long_backward_by_type<64>(a, dtype, general, stream);
-    return long_backward_by_type<128>(a, dtype, general, stream);
+    if (a.dim <= 64) return long_backward_by_type<64>(a, dtype, mode, stream);
+    return long_backward_by_type<128>(a, dtype, mode, stream);
   }
-  if (a.dim <= 16) return backward_by_type<16>(a, dtype, general, stream);
-  if (a.dim <= 32) return backward_by_type<32>(a, dtype, general, stream);
-  if (a.dim <= 64) return backward_by_type<64>(a, dtype, general, stream);
-  return backward_by_type<128>(a, dtype, general, stream);
+  if (a.dim <= 16) return backward_by_type<16>(a, dtype, mode, stream);
+  if (a.dim <= 32) return backward_by_type<32>(a, dtype, mode, stream);
+  if (a.dim <= 64) return backward_by_type<64>(a, dtype, mode, stream);
+  return backward_by_type<128>(a, dtype, mode, stream);
 }
 
 }  // namespace texb

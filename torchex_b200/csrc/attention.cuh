@@ -11,7 +11,7 @@
 //
 // A product with a masked probability is 0 only if the other factor is finite.  The matrix
 // instructions add up whole tiles, so a NaN or an infinity in a row that a query must not see would
-// reach its result.  Rows are therefore looked over first (blocks of kBlock positions are flagged), and
+// reach its result.  Rows are therefore looked over first (blocks of kFlag positions are flagged), and
 // a tile whose rows meet a flagged block is computed by the plain loops at the end of this file,
 // which touch visible rows only.
 #pragma once
@@ -23,7 +23,8 @@
 namespace texb {
 namespace attention {
 
-constexpr int kBlock = 64;  // positions of a tile, and of a flag
+constexpr int kBlock = 64;  // positions of a tile
+constexpr int kFlag = 16;   // positions of a flag
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Rows of 16-bit values of several heads; strides in values, the head dimension is contiguous.
@@ -48,7 +49,7 @@ struct Problem {
   View g;                    // gradient of out
   const float* delta;        // [heads, n] by position: scale * g_i . o_i
   View gq, gk, gv;
-  // flags of blocks with a value that is not finite, [.., ceil(n / kBlock)]; NULL: look for oneself
+  // flags of blocks with a value that is not finite, [.., ceil(n / kFlag)]; NULL: look for oneself
   const uint8_t *bad_v, *bad_k;  // per kv head
   const uint8_t* bad_q;          // per head: in q or g
 };
@@ -100,16 +101,19 @@ __device__ __forceinline__ float reciprocal_fast(float x) {  // 1 unit in the la
 // product.  tanh y = 1 - 2 / (exp(2 y) + 1), off by a few 2^-24 whatever y is: the exponential is infinite or 0
 // for large |y|, and tanh then +-1.  `slope` is the head's, in units of log2.
 struct Score { float x, slope; };
-template <bool GENERAL>
+// How scores are formed: scaled (by a positive factor) and nothing else; with a bias by distance, or any factor;
+// capped, with or without that.  A template parameter: the choice made per score took a third of the capped kernels' time.
+constexpr int kPlain = 0, kBiased = 1, kCapped = 2;
+inline int mode_of(const Problem& a) { return a.cap > 0.f ? kCapped : a.slopes || !(a.scale > 0.f) ? kBiased : kPlain; }
+template <int MODE>
 __device__ __forceinline__ Score score_of(const Problem& a, float product, float slope, float distance) {
-  if constexpr (!GENERAL) return {product * a.unit, 1.f};
-  float x = product * a.unit, d = 1.f;
-  if (a.cap > 0.f) {
-    const float t = fmaf(-2.f, reciprocal_fast(exp2_fast(product * a.bend_in) + 1.f), 1.f);
-    x = a.bend_out * t;
-    d = fmaf(-t, t, 1.f);
-  }
-  return {fmaf(-slope, fabsf(distance), x), d};
+  if constexpr (MODE == kPlain) return {product * a.unit, 1.f};
+  if constexpr (MODE == kBiased) return {fmaf(-slope, fabsf(distance), product * a.unit), 1.f};
+  const float t = fmaf(-2.f, reciprocal_fast(exp2_fast(product * a.bend_in) + 1.f), 1.f);
+  return {fmaf(-slope, fabsf(distance), a.bend_out * t), fmaf(-t, t, 1.f)};
+}
+__device__ __forceinline__ Score any_score(const Problem& a, float product, float slope, float distance) {
+  return a.cap > 0.f ? score_of<kCapped>(a, product, slope, distance) : score_of<kBiased>(a, product, slope, distance);
 }
 __device__ __forceinline__ float slope_of(const Problem& a, int head) { return a.slopes ? __ldg(a.slopes + head) * kLog2e : 0.f; }
 
@@ -239,19 +243,35 @@ __device__ __forceinline__ void product_rows(float (&acc)[NT][4], uint32_t a, in
   }
 }
 
-// acc [16 x DP] += P (16 x 8 NT, rounded to T) times NT * 8 rows of tile b
-template <typename T, int DP, int NT>
+// acc [16 x DP] += P (16 x 8 NT, rounded to T) times NT * 8 rows of tile b.  SPLIT: what the rounding takes from P
+// is multiplied as well, so that the products are those of some twice as many bits.
+template <typename T, int DP, int NT, bool SPLIT = false>
 __device__ __forceinline__ void product_probabilities(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b) {
+  auto rest = [](float x) {
+    const float high = widen<T>(narrow<T>(x));
+    return fabsf(high) < INFINITY ? x - high : 0.f;
+  };
 #pragma unroll
   for (int k = 0; k < NT / 2; ++k) {
-    const uint32_t fa[4] = {pack2<T>(p[2 * k][0], p[2 * k][1]), pack2<T>(p[2 * k][2], p[2 * k][3]),
-                            pack2<T>(p[2 * k + 1][0], p[2 * k + 1][1]), pack2<T>(p[2 * k + 1][2], p[2 * k + 1][3])};
+    const float (&x)[4] = p[2 * k], (&y)[4] = p[2 * k + 1];
+    const uint32_t fa[4] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+    uint32_t fr[4];
+    if constexpr (SPLIT) {
+      fr[0] = pack2<T>(rest(x[0]), rest(x[1]));
+      fr[1] = pack2<T>(rest(x[2]), rest(x[3]));
+      fr[2] = pack2<T>(rest(y[0]), rest(y[1]));
+      fr[3] = pack2<T>(rest(y[2]), rest(y[3]));
+    }
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       uint32_t fb[4];
       load_bt<DP>(fb, b, 16 * k, c);
       mma16816<T>(acc[2 * c], fa, fb[0], fb[1]);
       mma16816<T>(acc[2 * c + 1], fa, fb[2], fb[3]);
+      if constexpr (SPLIT) {
+        mma16816<T>(acc[2 * c], fr, fb[0], fb[1]);
+        mma16816<T>(acc[2 * c + 1], fr, fb[2], fb[3]);
+      }
     }
   }
 }
@@ -316,9 +336,9 @@ __device__ __forceinline__ bool look_over(const Problem& a, const View& x, int h
 
 // Whether a flagged block meets positions [begin, end); called by the whole CTA.
 __device__ __forceinline__ bool any_flag(const Problem& a, const uint8_t* flags, int head, int begin, int end) {
-  const int blocks = (a.n + kBlock - 1) / kBlock;
+  const int blocks = (a.n + kFlag - 1) / kFlag;
   bool bad = false;
-  for (int b = begin / kBlock + threadIdx.x; b < blocks && b * kBlock < end; b += blockDim.x) bad |= flags[int64_t(head) * blocks + b] != 0;
+  for (int b = begin / kFlag + threadIdx.x; b < blocks && b * kFlag < end; b += blockDim.x) bad |= flags[int64_t(head) * blocks + b] != 0;
   return __syncthreads_or(bad);
 }
 
@@ -385,7 +405,7 @@ __device__ __noinline__ void plain_forward(const Problem& a, int pos0, int rows,
     float acc[kColumns] = {}, top = -INFINITY, sum = 0.f;
     for (int j0 = see.begin; j0 < see.end; j0 += 32) {
       const int j = j0 + lane;
-      const float x = j < see.end ? score_of<true>(a, dot<T>(qi, row_at<T>(a, a.k, kv, j), a.dim), slope, float(i - j)).x : -INFINITY;
+      const float x = j < see.end ? any_score(a, dot<T>(qi, row_at<T>(a, a.k, kv, j), a.dim), slope, float(i - j)).x : -INFINITY;
       const float top_new = warp_max((x > top || x != x) ? x : top);
       const float base = top_new == -INFINITY ? 0.f : top_new;  // infinitely low scores so far: weight 0, not NaN
       const float w = j < see.end ? exp2f(x - base) : 0.f, shrink = top == -INFINITY ? 0.f : exp2f(top - base);
@@ -413,7 +433,7 @@ struct Pair { float p, ds; };  // probability and gradient of scale * product
 template <typename T>
 __device__ __forceinline__ Pair pair_of(const Problem& a, const T* qi, const T* kj, const T* vj, const T* gi, int head, int i, int j,
                                         float slope) {
-  const Score s = score_of<true>(a, dot<T>(qi, kj, a.dim), slope, float(i - j));
+  const Score s = any_score(a, dot<T>(qi, kj, a.dim), slope, float(i - j));
   const float p = exp2f(s.x - a.lse[int64_t(head) * a.n + i]);
   return {p, p * (dot<T>(gi, vj, a.dim) * a.scale - a.delta[int64_t(head) * a.n + i]) * s.slope};
 }

@@ -6,7 +6,8 @@
 //   queries: as the forward kernel, 64 query positions of one head against the keys they see;
 //   keys   : 64 key positions of one kv head against the queries that see them, of all query heads
 //            that share it -- the gradient of a shared key or value is one sum.
-// With P and dS rounded to the inputs' type before their products (half a step each):
+// P is rounded to the inputs' type before its product (half a step); dS goes in as two such values, which costs
+// little here and halves the squared error of gq and gk:
 //   dS = P (scale g v - delta) x (derivative of the capped score), delta = scale g o,  gq = dS k, gk = dS^T q, gv = P^T g.
 // A masked pair's dS is set to 0, not multiplied by 0: its g v may be infinite.
 #pragma once
@@ -23,18 +24,14 @@ struct QueryMemory {
   static constexpr int kBytes = 6 * kTile;
 };
 
-template <typename T, int DP, bool GENERAL>
-__global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_constant__ Problem a) {
+template <typename T, int DP, int MODE>
+__global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_kernel(const __grid_constant__ Problem a) {
   extern __shared__ __align__(128) unsigned char smem[];
   using M = QueryMemory<DP>;
   const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
   const int pos0 = blockIdx.x * kBlock, last = min(a.n, pos0 + kBlock) - 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
-  if (any_flag(a, a.bad_k, kv, first_key, end_key)) {
-    plain_query_gradient<T>(a, pos0, kBlock, head);
-    return;
-  }
   const uint32_t base = smem_u32(smem);
   Loader<DP, kBlock> loader;
   loader.look_up(a, pos0, last + 1);
@@ -45,12 +42,17 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_c
   loader.template copy<T>(a, a.v, kv, base + M::kV);
   commit_copies();
   loader.look_up(a, first_key + kBlock, end_key);
+  if (any_flag(a, a.bad_k, kv, first_key, end_key)) {  // looked at while the first rows are on their way
+    wait_copies<0>();
+    plain_query_gradient<T>(a, pos0, kBlock, head);
+    return;
+  }
 
   const int row0 = warp * 16, i0 = pos0 + row0 + (lane >> 2), i1 = i0 + 8;
   const Bounds see0 = keys_of(a, i0), see1 = keys_of(a, i1);
   const int warp_begin = keys_of(a, pos0 + row0).begin, warp_last = min(last, pos0 + row0 + 15);
   const int warp_end = pos0 + row0 <= last ? keys_of(a, warp_last).end : 0;
-  const float slope = GENERAL ? slope_of(a, head) : 0.f;
+  const float slope = MODE != kPlain ? slope_of(a, head) : 0.f;
   const int64_t place = int64_t(head) * a.n;
   const float lse0 = i0 < a.n ? a.lse[place + i0] : 0.f, lse1 = i1 < a.n ? a.lse[place + i1] : 0.f;
   const float delta0 = i0 < a.n ? a.delta[place + i0] : 0.f, delta1 = i1 < a.n ? a.delta[place + i1] : 0.f;
@@ -76,14 +78,14 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = j0 + t * 8 + (lane & 3) * 2 + e;
-          const Score x0 = score_of<GENERAL>(a, s[t][e], slope, float(i0 - j)), x1 = score_of<GENERAL>(a, s[t][2 + e], slope, float(i1 - j));
+          const Score x0 = score_of<MODE>(a, s[t][e], slope, float(i0 - j)), x1 = score_of<MODE>(a, s[t][2 + e], slope, float(i1 - j));
           const float d0 = exp2_fast(x0.x - lse0) * fmaf(dp[t][e], a.scale, -delta0) * x0.slope;
           const float d1 = exp2_fast(x1.x - lse1) * fmaf(dp[t][2 + e], a.scale, -delta1) * x1.slope;
           dp[t][e] = j >= see0.begin && j < see0.end ? d0 : 0.f;
           dp[t][2 + e] = j >= see1.begin && j < see1.end ? d1 : 0.f;
         }
       }
-      product_probabilities<T, DP, NT>(gq, dp, base + M::kK + stage * M::kTile);
+      product_probabilities<T, DP, NT, true>(gq, dp, base + M::kK + stage * M::kTile);
     }
     __syncthreads();
     stage ^= 1;
@@ -104,8 +106,8 @@ struct KeyMemory {
   static constexpr int kBytes = kDelta + 2 * kRows * 4;
 };
 
-template <typename T, int DP, bool GENERAL>
-__global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_constant__ Problem a) {
+template <typename T, int DP, int MODE>
+__global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kernel(const __grid_constant__ Problem a) {
   extern __shared__ __align__(128) unsigned char smem[];
   using M = KeyMemory<DP>;
   constexpr int R = M::kRows, NT = R / 8;
@@ -113,12 +115,6 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
   const int pos0 = blockIdx.x * kBlock, last = min(a.n, pos0 + kBlock) - 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first_query = queries_of(a, pos0).begin, end_query = queries_of(a, last).end;
-  bool bad = false;
-  for (int head = kv * group; head < (kv + 1) * group; ++head) bad |= any_flag(a, a.bad_q, head, first_query, end_query);
-  if (bad) {
-    plain_key_gradients<T>(a, pos0, kBlock, kv);
-    return;
-  }
   const uint32_t base = smem_u32(smem);
   {
     Loader<DP, kBlock> keys;
@@ -143,6 +139,14 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
   loader.look_up(a, first_query, end_query);
   if (total > 0) fetch(kv * group, first_query, 0);
   commit_copies();
+  loader.look_up(a, first_query + (steps > 1 ? R : 0), end_query);
+  bool bad = false;  // looked at while the first rows are on their way
+  for (int h = kv * group; h < (kv + 1) * group; ++h) bad |= any_flag(a, a.bad_q, h, first_query, end_query);
+  if (bad) {
+    wait_copies<0>();
+    plain_key_gradients<T>(a, pos0, kBlock, kv);
+    return;
+  }
 
   const int row0 = warp * 16, j0 = pos0 + row0 + (lane >> 2), j1 = j0 + 8;
   const Bounds seen0 = queries_of(a, j0), seen1 = queries_of(a, j1);
@@ -158,15 +162,13 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
       next_step = 0;
       ++next_head;
     }
-    if (it + 1 < total) {
-      loader.look_up(a, first_query + next_step * R, end_query);
-      fetch(next_head, first_query + next_step * R, stage ^ 1);
-    }
+    if (it + 1 < total) fetch(next_head, first_query + next_step * R, stage ^ 1);
     commit_copies();
+    loader.look_up(a, first_query + (next_step + 1 == steps ? 0 : next_step + 1) * R, end_query);  // for the step after
     wait_copies<1>();
     __syncthreads();
     if (q0 + R > warp_begin && q0 < warp_end) {
-      const float slope = GENERAL ? slope_of(a, head) : 0.f;
+      const float slope = MODE != kPlain ? slope_of(a, head) : 0.f;
       const uint32_t tq = base + M::kQ + stage * M::kStep, tg = base + M::kG + stage * M::kStep;
       float p[NT][4] = {}, ds[NT][4] = {};
       product_rows<T, DP, NT>(p, base + M::kK, row0, tq);
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
         for (int e = 0; e < 2; ++e) {
           const int r = t * 8 + (lane & 3) * 2 + e, i = q0 + r;
           const float lse = s_lse[stage * R + r], delta = s_delta[stage * R + r];
-          const Score x0 = score_of<GENERAL>(a, p[t][e], slope, float(i - j0)), x1 = score_of<GENERAL>(a, p[t][2 + e], slope, float(i - j1));
+          const Score x0 = score_of<MODE>(a, p[t][e], slope, float(i - j0)), x1 = score_of<MODE>(a, p[t][2 + e], slope, float(i - j1));
           const bool on0 = i >= seen0.begin && i < seen0.end, on1 = i >= seen1.begin && i < seen1.end;
           p[t][e] = on0 ? exp2_fast(x0.x - lse) : 0.f;
           p[t][2 + e] = on1 ? exp2_fast(x1.x - lse) : 0.f;
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) key_gradients_kernel(const __grid_co
         }
       }
       product_probabilities<T, DP, NT>(gv, p, tg);
-      product_probabilities<T, DP, NT>(gk, ds, tq);
+      product_probabilities<T, DP, NT, true>(gk, ds, tq);
     }
     __syncthreads();
     stage ^= 1;
@@ -206,11 +208,11 @@ int prepare_kernel(K kernel, int bytes, const char* what) {
   return e == cudaSuccess ? TEXB_OK : fail(TEXB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, int MODE>
 int launch_backward(const Problem& a, cudaStream_t stream) {
   const unsigned tiles = unsigned((a.n + kBlock - 1) / kBlock);
-  auto queries = query_gradient_kernel<T, DP, GENERAL>;
-  auto keys = key_gradients_kernel<T, DP, GENERAL>;
+  auto queries = query_gradient_kernel<T, DP, MODE>;
+  auto keys = key_gradients_kernel<T, DP, MODE>;
   int st = prepare_kernel(queries, QueryMemory<DP>::kBytes, "attention query_gradient_kernel");
   if (st == TEXB_OK) st = prepare_kernel(keys, KeyMemory<DP>::kBytes, "attention key_gradients_kernel");
   if (st != TEXB_OK) return st;
@@ -222,10 +224,11 @@ int launch_backward(const Problem& a, cudaStream_t stream) {
 }
 
 template <int DP>
-int backward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
-  if (dtype == TEXB_BFLOAT16)
-    return general ? launch_backward<__nv_bfloat16, DP, true>(a, stream) : launch_backward<__nv_bfloat16, DP, false>(a, stream);
-  return general ? launch_backward<__half, DP, true>(a, stream) : launch_backward<__half, DP, false>(a, stream);
+int backward_by_type(const Problem& a, int dtype, int mode, cudaStream_t stream) {
+  const bool bf16 = dtype == TEXB_BFLOAT16;
+  if (mode == kCapped) return bf16 ? launch_backward<__nv_bfloat16, DP, kCapped>(a, stream) : launch_backward<__half, DP, kCapped>(a, stream);
+  if (mode == kBiased) return bf16 ? launch_backward<__nv_bfloat16, DP, kBiased>(a, stream) : launch_backward<__half, DP, kBiased>(a, stream);
+  return bf16 ? launch_backward<__nv_bfloat16, DP, kPlain>(a, stream) : launch_backward<__half, DP, kPlain>(a, stream);
 }
 
 }  // namespace attention

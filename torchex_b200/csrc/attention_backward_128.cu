@@ -2,6 +2,6 @@
 
 namespace texb {
 namespace attention {
-template int backward_by_type<128>(const Problem&, int, bool, cudaStream_t);
+template int backward_by_type<128>(const Problem&, int, int, cudaStream_t);
 }  // namespace attention
 }  // namespace texb

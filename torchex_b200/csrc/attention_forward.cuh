@@ -22,21 +22,14 @@ struct ForwardMemory {
   static constexpr int kBytes = 5 * kTile;
 };
 
-template <typename T, int DP, bool GENERAL>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Problem a) {
+template <typename T, int DP, int MODE>
+__global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(const __grid_constant__ Problem a) {
   extern __shared__ __align__(128) unsigned char smem[];
   using M = ForwardMemory<T, DP>;
   const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
   const int pos0 = blockIdx.x * kBlock, last = min(a.n, pos0 + kBlock) - 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
-
-  const bool bad = a.bad_v ? any_flag(a, a.bad_v, kv, first_key, end_key)
-                           : look_over<T>(a, a.v, kv, first_key, end_key);
-  if (bad) {
-    plain_forward<T>(a, pos0, kBlock, head);
-    return;
-  }
 
   const uint32_t base = smem_u32(smem), sq = base + M::kQ;
   Loader<DP, kBlock> loader;
@@ -47,6 +40,13 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   loader.template copy<T>(a, a.v, kv, base + M::kV);
   commit_copies();
   loader.look_up(a, first_key + kBlock, end_key);
+  // looked at while the first rows are on their way
+  const bool bad = a.bad_v ? any_flag(a, a.bad_v, kv, first_key, end_key) : look_over<T>(a, a.v, kv, first_key, end_key);
+  if (bad) {
+    wait_copies<0>();
+    plain_forward<T>(a, pos0, kBlock, head);
+    return;
+  }
 
   const int row0 = warp * 16, i0 = pos0 + row0 + (lane >> 2), i1 = i0 + 8;
   const Bounds see0 = keys_of(a, i0), see1 = keys_of(a, i1);
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   const Bounds tail = pos0 + row0 <= last ? keys_of(a, warp_last) : Bounds{0, 0};
   const int warp_end = tail.end;
   const int all_begin = tail.begin, all_end = pos0 + row0 + 15 <= last ? keys_of(a, pos0 + row0).end : 0;
-  const float slope = GENERAL ? slope_of(a, head) : 0.f;
+  const float slope = MODE != kPlain ? slope_of(a, head) : 0.f;
 
   float out[DP / 8][4] = {};
   float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = j0 + t * 8 + (lane & 3) * 2 + e;
-          s[t][e] = score_of<GENERAL>(a, s[t][e], slope, float(i0 - j)).x;
-          s[t][2 + e] = score_of<GENERAL>(a, s[t][2 + e], slope, float(i1 - j)).x;
+          s[t][e] = score_of<MODE>(a, s[t][e], slope, float(i0 - j)).x;
+          s[t][2 + e] = score_of<MODE>(a, s[t][2 + e], slope, float(i1 - j)).x;
           if (!whole) {
             if (j < see0.begin || j >= see0.end) s[t][e] = -INFINITY;
             if (j < see1.begin || j >= see1.end) s[t][2 + e] = -INFINITY;
@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   if (a.out_low.p) store_rows<T, DP, true>(a, a.out_low, head, pos0 + row0, out, factor0, factor1, smem + M::kQ, row0);
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, int MODE>
 int launch_forward(const Problem& a, cudaStream_t stream) {
-  auto kernel = forward_kernel<T, DP, GENERAL>;
+  auto kernel = forward_kernel<T, DP, MODE>;
   constexpr int bytes = ForwardMemory<T, DP>::kBytes;
   if (bytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -155,10 +155,11 @@ int launch_forward(const Problem& a, cudaStream_t stream) {
 }
 
 template <int DP>
-int forward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
-  if (dtype == TEXB_BFLOAT16)
-    return general ? launch_forward<__nv_bfloat16, DP, true>(a, stream) : launch_forward<__nv_bfloat16, DP, false>(a, stream);
-  return general ? launch_forward<__half, DP, true>(a, stream) : launch_forward<__half, DP, false>(a, stream);
+int forward_by_type(const Problem& a, int dtype, int mode, cudaStream_t stream) {
+  const bool bf16 = dtype == TEXB_BFLOAT16;
+  if (mode == kCapped) return bf16 ? launch_forward<__nv_bfloat16, DP, kCapped>(a, stream) : launch_forward<__half, DP, kCapped>(a, stream);
+  if (mode == kBiased) return bf16 ? launch_forward<__nv_bfloat16, DP, kBiased>(a, stream) : launch_forward<__half, DP, kBiased>(a, stream);
+  return bf16 ? launch_forward<__nv_bfloat16, DP, kPlain>(a, stream) : launch_forward<__half, DP, kPlain>(a, stream);
 }
 
 }  // namespace attention

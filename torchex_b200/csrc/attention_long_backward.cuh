@@ -31,7 +31,7 @@ struct LongBackwardMemory {
   static constexpr int kScores = 0, kSums = 256, kColumns = 512;  // tensor memory
 };
 
-template <typename T, int DP, bool GENERAL, bool KEYS>
+template <typename T, int DP, int MODE, bool KEYS>
 __global__ void __launch_bounds__(kLongThreads, 1)
 long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ Maps maps) {
   extern __shared__ unsigned char raw[];
@@ -112,7 +112,7 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
     }
     for (int u = buffer; u < total; u += 2) {
       const int p0 = first + step * N, stage = u % S;
-      const float slope = GENERAL ? slope_of(a, KEYS ? kv * group + head : own_head) : 0.f;
+      const float slope = MODE != kPlain ? slope_of(a, KEYS ? kv * group + head : own_head) : 0.f;
       if (KEYS) t5::warp_wait(bar(kFull + stage), (u / S) & 1, dead);  // lse and delta of the tile's queries
       t5::warp_wait(bar(kScoresFull + buffer), (u >> 1) & 1, dead);
       const float* lse = s_lse + stage * 2 * N;
@@ -141,9 +141,9 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
             const int k = e + h;
             const float2 l = h ? float2{l4.z, l4.w} : float2{l4.x, l4.y}, d = h ? float2{d4.z, d4.w} : float2{d4.x, d4.y};
             float2 x, bend = {1.f, 1.f};
-            if constexpr (GENERAL) {
+            if constexpr (MODE != kPlain) {
               const float away = float(pos - p0) - float(c + k);
-              const Score x0 = score_of<true>(a, s[k], slope, away), x1 = score_of<true>(a, s[k + 1], slope, away - 1.f);
+              const Score x0 = score_of<MODE>(a, s[k], slope, away), x1 = score_of<MODE>(a, s[k + 1], slope, away - 1.f);
               x = {x0.x - l.x, x1.x - l.y};
               bend = {x0.slope, x1.slope};
             } else {
@@ -151,7 +151,7 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
             }
             float2 p = {exp2_fast(x.x), exp2_fast(x.y)};
             float2 ds = t5::mul2(p, t5::fma2({g[k], g[k + 1]}, scale, {-d.x, -d.y}));
-            if constexpr (GENERAL) ds = t5::mul2(ds, bend);
+            if constexpr (MODE != kPlain) ds = t5::mul2(ds, bend);
             if (!whole) {  // set, not multiplied: a masked pair's product may be infinite
               const bool on0 = c + k >= from && c + k < to, on1 = c + k + 1 >= from && c + k + 1 < to;
               p = {on0 ? p.x : 0.f, on1 ? p.y : 0.f};
@@ -308,9 +308,9 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
   if (warp == 12) t5::tmem_free(tmem, M::kColumns);
 }
 
-template <typename T, int DP, bool GENERAL, bool KEYS>
+template <typename T, int DP, int MODE, bool KEYS>
 int launch_long_backward(const Problem& a, int dtype, cudaStream_t stream) {
-  auto kernel = long_backward_kernel<T, DP, GENERAL, KEYS>;
+  auto kernel = long_backward_kernel<T, DP, MODE, KEYS>;
   using M = LongBackwardMemory<DP>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kBytes);
   if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "attention long_backward_kernel: %s", cudaGetErrorString(e));
@@ -323,19 +323,18 @@ int launch_long_backward(const Problem& a, int dtype, cudaStream_t stream) {
   return check_launch("attention long_backward_kernel");
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, int MODE>
 int launch_long_backward_both(const Problem& a, int dtype, cudaStream_t stream) {
-  const int st = launch_long_backward<T, DP, GENERAL, false>(a, dtype, stream);
-  return st == TEXB_OK ? launch_long_backward<T, DP, GENERAL, true>(a, dtype, stream) : st;
+  const int st = launch_long_backward<T, DP, MODE, false>(a, dtype, stream);
+  return st == TEXB_OK ? launch_long_backward<T, DP, MODE, true>(a, dtype, stream) : st;
 }
 
 template <int DP>
-int long_backward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
-  if (dtype == TEXB_BFLOAT16)
-    return general ? launch_long_backward_both<__nv_bfloat16, DP, true>(a, dtype, stream)
-                   : launch_long_backward_both<__nv_bfloat16, DP, false>(a, dtype, stream);
-  return general ? launch_long_backward_both<__half, DP, true>(a, dtype, stream)
-                 : launch_long_backward_both<__half, DP, false>(a, dtype, stream);
+int long_backward_by_type(const Problem& a, int dtype, int mode, cudaStream_t stream) {
+  const bool bf16 = dtype == TEXB_BFLOAT16;
+  if (mode == kCapped) return bf16 ? launch_long_backward_both<__nv_bfloat16, DP, kCapped>(a, dtype, stream) : launch_long_backward_both<__half, DP, kCapped>(a, dtype, stream);
+  if (mode == kBiased) return bf16 ? launch_long_backward_both<__nv_bfloat16, DP, kBiased>(a, dtype, stream) : launch_long_backward_both<__half, DP, kBiased>(a, dtype, stream);
+  return bf16 ? launch_long_backward_both<__nv_bfloat16, DP, kPlain>(a, dtype, stream) : launch_long_backward_both<__half, DP, kPlain>(a, dtype, stream);
 }
 
 // Waits that gave up in this unit's kernels since the library was loaded.

@@ -44,7 +44,7 @@ __device__ __forceinline__ LongRange range_of(const Problem& a, int pos0) {
   return {f.begin, l.end, l.begin, f.end};
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, int MODE>
 __global__ void __launch_bounds__(kLongThreads, 1)
 long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ Maps maps) {
   extern __shared__ unsigned char raw[];
@@ -108,7 +108,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t sums = tmem + lanes + M::kOut + w * DP;
     const Bounds see = keys_of(a, i);
-    const float unit = a.unit, slope = GENERAL ? slope_of(a, head) : 0.f;
+    const float unit = a.unit, slope = MODE != kPlain ? slope_of(a, head) : 0.f;
     float top = -INFINITY;  // in units of log2
     float2 sum = {0.f, 0.f};
     int done = 0;           // tiles of this query tile so far
@@ -121,9 +121,9 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
       for (int c = 0; c < N; c += 32) t5::tmem_load32(scores + c, reinterpret_cast<float(&)[32]>(s[c]));
       t5::tmem_wait_loads();
       const int j0 = first_key + j * N;
-      if constexpr (GENERAL) {
+      if constexpr (MODE != kPlain) {
 #pragma unroll
-        for (int c = 0; c < N; ++c) s[c] = score_of<true>(a, s[c], slope, float(i - j0) - float(c)).x;
+        for (int c = 0; c < N; ++c) s[c] = score_of<MODE>(a, s[c], slope, float(i - j0) - float(c)).x;
       }
       if (!(j0 >= mine.all_begin && j0 + N <= mine.all_end)) {
         const int from = see.begin - j0, to = see.end - j0;
@@ -134,7 +134,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
 #pragma unroll
       for (int c = 4; c + 1 < N; c += 2) most[(c >> 1) & 3] = t5::max3(most[(c >> 1) & 3], s[c], s[c + 1]);
       float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-      if constexpr (!GENERAL) now *= unit;  // the scale is positive here
+      if constexpr (MODE == kPlain) now *= unit;  // the scale is positive here
       if (done == 0) {
         top = now;
       } else if (__any_sync(0xffffffffu, now > top + kStale)) {
@@ -157,7 +157,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
         }
       }
       const float less = top == -INFINITY ? 0.f : top;  // a row without a visible key so far: weights 0, not NaN
-      const float2 factor = {GENERAL ? 1.f : unit, GENERAL ? 1.f : unit}, shift = {-less, -less};
+      const float2 factor = {MODE != kPlain ? 1.f : unit, MODE != kPlain ? 1.f : unit}, shift = {-less, -less};
       float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int c = 0; c < N; c += 32) {
@@ -297,9 +297,9 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   if (warp == 12) t5::tmem_free(tmem, M::kColumns);
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, int MODE>
 int launch_long_forward(const Problem& a, int dtype, cudaStream_t stream) {
-  auto kernel = long_forward_kernel<T, DP, GENERAL>;
+  auto kernel = long_forward_kernel<T, DP, MODE>;
   constexpr int bytes = LongForwardMemory<DP>::kBytes;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "attention long_forward_kernel: %s", cudaGetErrorString(e));
@@ -313,11 +313,11 @@ int launch_long_forward(const Problem& a, int dtype, cudaStream_t stream) {
 }
 
 template <int DP>
-int long_forward_by_type(const Problem& a, int dtype, bool general, cudaStream_t stream) {
-  if (dtype == TEXB_BFLOAT16)
-    return general ? launch_long_forward<__nv_bfloat16, DP, true>(a, dtype, stream)
-                   : launch_long_forward<__nv_bfloat16, DP, false>(a, dtype, stream);
-  return general ? launch_long_forward<__half, DP, true>(a, dtype, stream) : launch_long_forward<__half, DP, false>(a, dtype, stream);
+int long_forward_by_type(const Problem& a, int dtype, int mode, cudaStream_t stream) {
+  const bool bf16 = dtype == TEXB_BFLOAT16;
+  if (mode == kCapped) return bf16 ? launch_long_forward<__nv_bfloat16, DP, kCapped>(a, dtype, stream) : launch_long_forward<__half, DP, kCapped>(a, dtype, stream);
+  if (mode == kBiased) return bf16 ? launch_long_forward<__nv_bfloat16, DP, kBiased>(a, dtype, stream) : launch_long_forward<__half, DP, kBiased>(a, dtype, stream);
+  return bf16 ? launch_long_forward<__nv_bfloat16, DP, kPlain>(a, dtype, stream) : launch_long_forward<__half, DP, kPlain>(a, dtype, stream);
 }
 
 // Waits that gave up in this unit's kernels since the library was loaded.
