@@ -19,9 +19,10 @@ namespace attention {
 
 template <int DP>
 struct QueryMemory {
+  static constexpr int kStages = DP <= 32 ? 4 : 2;
   static constexpr int kTile = kBlock * DP * 2;
-  static constexpr int kQ = 0, kG = kTile, kK = 2 * kTile, kV = 4 * kTile;  // two stages of keys and values
-  static constexpr int kBytes = 6 * kTile;
+  static constexpr int kQ = 0, kG = kTile, kK = 2 * kTile, kV = kK + kStages * kTile;
+  static constexpr int kBytes = (2 + 2 * kStages) * kTile;
 };
 
 template <typename T, int DP, int MODE>
@@ -33,15 +34,22 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
   const uint32_t base = smem_u32(smem);
-  Loader<DP, kBlock> loader;
-  loader.look_up(a, pos0, last + 1);
-  loader.template copy<T>(a, a.q, head, base + M::kQ);
-  loader.template copy<T>(a, a.g, head, base + M::kG);
-  loader.look_up(a, first_key, end_key);
-  loader.template copy<T>(a, a.k, kv, base + M::kK);
-  loader.template copy<T>(a, a.v, kv, base + M::kV);
-  commit_copies();
-  loader.look_up(a, first_key + kBlock, end_key);
+  constexpr int S = M::kStages;
+  Loader<DP, kBlock> queries, ahead[S - 1], loader;
+  queries.look_up(a, pos0, last + 1);
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_key + t * kBlock, end_key);
+  queries.template copy<T>(a, a.q, head, base + M::kQ);
+  queries.template copy<T>(a, a.g, head, base + M::kG);
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) {
+    if (first_key + t * kBlock < end_key) {
+      ahead[t].template copy<T>(a, a.k, kv, base + M::kK + t * M::kTile);
+      ahead[t].template copy<T>(a, a.v, kv, base + M::kV + t * M::kTile);
+    }
+    commit_copies();
+  }
+  loader.look_up(a, first_key + (S - 1) * kBlock, end_key);
   if (any_flag(a, a.bad_k, kv, first_key, end_key)) {  // looked at while the first rows are on their way
     wait_copies<0>();
     plain_query_gradient<T>(a, pos0, kBlock, head);
@@ -60,14 +68,15 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_ker
   float gq[DP / 8][4] = {};
   int stage = 0;
   for (int j0 = first_key; j0 < end_key; j0 += kBlock) {
-    if (j0 + kBlock < end_key) {
-      loader.template copy<T>(a, a.k, kv, base + M::kK + (stage ^ 1) * M::kTile);
-      loader.template copy<T>(a, a.v, kv, base + M::kV + (stage ^ 1) * M::kTile);
+    wait_copies<S - 2>();
+    __syncthreads();  // this tile is there, and the stage of the last one is free
+    if (j0 + (S - 1) * kBlock < end_key) {
+      const int free = stage == 0 ? S - 1 : stage - 1;
+      loader.template copy<T>(a, a.k, kv, base + M::kK + free * M::kTile);
+      loader.template copy<T>(a, a.v, kv, base + M::kV + free * M::kTile);
     }
     commit_copies();
-    loader.look_up(a, j0 + 2 * kBlock, end_key);
-    wait_copies<1>();
-    __syncthreads();
+    loader.look_up(a, j0 + S * kBlock, end_key);
     if (j0 + kBlock > warp_begin && j0 < warp_end) {
       constexpr int NT = kBlock / 8;
       float s[NT][4] = {}, dp[NT][4] = {};
@@ -87,8 +96,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_ker
       }
       product_probabilities<T, DP, NT, true>(gq, dp, base + M::kK + stage * M::kTile);
     }
-    __syncthreads();
-    stage ^= 1;
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
   wait_copies<0>();
   __syncwarp();
@@ -101,9 +109,10 @@ template <int DP>
 struct KeyMemory {
   static constexpr int kRows = DP == 128 ? 32 : 64;
   static constexpr int kTile = kBlock * DP * 2, kStep = kRows * DP * 2;
-  static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile, kG = kQ + 2 * kStep;  // two stages of queries and gradients
-  static constexpr int kLse = kG + 2 * kStep, kDelta = kLse + 2 * kRows * 4;
-  static constexpr int kBytes = kDelta + 2 * kRows * 4;
+  static constexpr int kStages = DP <= 32 ? 4 : 2;  // of queries and gradients
+  static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile, kG = kQ + kStages * kStep;
+  static constexpr int kLse = kG + kStages * kStep, kDelta = kLse + kStages * kRows * 4;
+  static constexpr int kBytes = kDelta + kStages * kRows * 4;
 };
 
 template <typename T, int DP, int MODE>
@@ -124,10 +133,10 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
   }
   float* s_lse = reinterpret_cast<float*>(smem + M::kLse);
   float* s_delta = reinterpret_cast<float*>(smem + M::kDelta);
-  Loader<DP, R> loader;
-  auto fetch = [&](int head, int q0, int stage) {
-    loader.template copy<T>(a, a.q, head, base + M::kQ + stage * M::kStep);
-    loader.template copy<T>(a, a.g, head, base + M::kG + stage * M::kStep);
+  constexpr int S = M::kStages;
+  auto fetch = [&](const Loader<DP, R>& rows, int head, int q0, int stage) {
+    rows.template copy<T>(a, a.q, head, base + M::kQ + stage * M::kStep);
+    rows.template copy<T>(a, a.g, head, base + M::kG + stage * M::kStep);
     for (int r = threadIdx.x; r < R; r += kThreads) {
       const bool real = q0 + r < end_query;
       const int64_t at = int64_t(head) * a.n + (real ? q0 + r : 0);
@@ -136,10 +145,26 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
     }
   };
   const int steps = (end_query - first_query + R - 1) / R, total = steps * group;
-  loader.look_up(a, first_query, end_query);
-  if (total > 0) fetch(kv * group, first_query, 0);
-  commit_copies();
-  loader.look_up(a, first_query + (steps > 1 ? R : 0), end_query);
+  // the steps of the first head, then of the next: what is fetched next, and its rows, looked up a step ahead
+  int fetch_step = 0, fetch_head = kv * group;
+  auto advance = [&] {
+    if (++fetch_step == steps) {
+      fetch_step = 0;
+      ++fetch_head;
+    }
+  };
+  Loader<DP, R> ahead[S - 1], loader;
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_query + (steps > 0 ? t % steps : 0) * R, end_query);
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) {
+    if (t < total) {
+      fetch(ahead[t], fetch_head, first_query + fetch_step * R, t);
+      advance();
+    }
+    commit_copies();
+  }
+  loader.look_up(a, first_query + fetch_step * R, end_query);
   bool bad = false;  // looked at while the first rows are on their way
   for (int h = kv * group; h < (kv + 1) * group; ++h) bad |= any_flag(a, a.bad_q, h, first_query, end_query);
   if (bad) {
@@ -157,16 +182,14 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
   int stage = 0, head = kv * group, step = 0;
   for (int it = 0; it < total; ++it) {
     const int q0 = first_query + step * R;
-    int next_step = step + 1, next_head = head;
-    if (next_step == steps) {
-      next_step = 0;
-      ++next_head;
+    wait_copies<S - 2>();
+    __syncthreads();  // this step's rows are there, and the stage of the last one is free
+    if (it + S - 1 < total) {
+      fetch(loader, fetch_head, first_query + fetch_step * R, stage == 0 ? S - 1 : stage - 1);
+      advance();
     }
-    if (it + 1 < total) fetch(next_head, first_query + next_step * R, stage ^ 1);
     commit_copies();
-    loader.look_up(a, first_query + (next_step + 1 == steps ? 0 : next_step + 1) * R, end_query);  // for the step after
-    wait_copies<1>();
-    __syncthreads();
+    loader.look_up(a, first_query + fetch_step * R, end_query);
     if (q0 + R > warp_begin && q0 < warp_end) {
       const float slope = MODE != kPlain ? slope_of(a, head) : 0.f;
       const uint32_t tq = base + M::kQ + stage * M::kStep, tg = base + M::kG + stage * M::kStep;
@@ -190,10 +213,11 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
       product_probabilities<T, DP, NT>(gv, p, tg);
       product_probabilities<T, DP, NT, true>(gk, ds, tq);
     }
-    __syncthreads();
-    stage ^= 1;
-    step = next_step;
-    head = next_head;
+    stage = stage + 1 == S ? 0 : stage + 1;
+    if (++step == steps) {
+      step = 0;
+      ++head;
+    }
   }
   wait_copies<0>();
   __syncthreads();  // the key tiles are written over below, by warps that read only their own rows of them

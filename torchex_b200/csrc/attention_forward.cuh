@@ -2,7 +2,7 @@
 //
 // A CTA of four warps owns 64 query positions of one head, 16 per warp, and walks the keys its rows
 // see in tiles of 64: scores, running maximum and sum (in units of log2), and the product with the
-// values stay in registers; keys and values are copied one tile ahead (cp.async, two stages).  A warp
+// values stay in registers; keys and values are copied ahead (cp.async, two to four stages).  A warp
 // passes over tiles that none of its 16 rows see, which is what keeps a tile of many short segments
 // cheap, and over the mask where all of its rows see the whole tile.  Probabilities are rounded to the
 // type of the values before the second product, which the matrix instructions require: half a step
@@ -16,10 +16,11 @@ namespace attention {
 
 template <typename T, int DP>
 struct ForwardMemory {
+  static constexpr int kStages = DP <= 32 ? 4 : 2;  // narrow rows: all keys of a tile of short segments at once
   static constexpr int kQ = 0;
   static constexpr int kTile = kBlock * DP * 2;
-  static constexpr int kK = kTile, kV = 3 * kTile;  // two stages each
-  static constexpr int kBytes = 5 * kTile;
+  static constexpr int kK = kTile, kV = kK + kStages * kTile;
+  static constexpr int kBytes = (1 + 2 * kStages) * kTile;
 };
 
 template <typename T, int DP, int MODE>
@@ -32,14 +33,21 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
 
   const uint32_t base = smem_u32(smem), sq = base + M::kQ;
-  Loader<DP, kBlock> loader;
-  loader.look_up(a, pos0, last + 1);
-  loader.template copy<T>(a, a.q, head, sq);
-  loader.look_up(a, first_key, end_key);
-  loader.template copy<T>(a, a.k, kv, base + M::kK);
-  loader.template copy<T>(a, a.v, kv, base + M::kV);
-  commit_copies();
-  loader.look_up(a, first_key + kBlock, end_key);
+  constexpr int S = M::kStages;
+  Loader<DP, kBlock> queries, ahead[S - 1], loader;
+  queries.look_up(a, pos0, last + 1);
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_key + t * kBlock, end_key);
+  queries.template copy<T>(a, a.q, head, sq);
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) {
+    if (first_key + t * kBlock < end_key) {
+      ahead[t].template copy<T>(a, a.k, kv, base + M::kK + t * M::kTile);
+      ahead[t].template copy<T>(a, a.v, kv, base + M::kV + t * M::kTile);
+    }
+    commit_copies();
+  }
+  loader.look_up(a, first_key + (S - 1) * kBlock, end_key);
   // looked at while the first rows are on their way
   const bool bad = a.bad_v ? any_flag(a, a.bad_v, kv, first_key, end_key) : look_over<T>(a, a.v, kv, first_key, end_key);
   if (bad) {
@@ -61,14 +69,15 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
   float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
   int stage = 0;
   for (int j0 = first_key; j0 < end_key; j0 += kBlock) {
-    if (j0 + kBlock < end_key) {
-      loader.template copy<T>(a, a.k, kv, base + M::kK + (stage ^ 1) * M::kTile);
-      loader.template copy<T>(a, a.v, kv, base + M::kV + (stage ^ 1) * M::kTile);
+    wait_copies<S - 2>();
+    __syncthreads();  // this tile is there, and the stage of the last one is free
+    if (j0 + (S - 1) * kBlock < end_key) {
+      const int free = stage == 0 ? S - 1 : stage - 1;
+      loader.template copy<T>(a, a.k, kv, base + M::kK + free * M::kTile);
+      loader.template copy<T>(a, a.v, kv, base + M::kV + free * M::kTile);
     }
     commit_copies();
-    loader.look_up(a, j0 + 2 * kBlock, end_key);
-    wait_copies<1>();
-    __syncthreads();
+    loader.look_up(a, j0 + S * kBlock, end_key);
     if (j0 + kBlock > warp_begin && j0 < warp_end) {
       constexpr int NT = kBlock / 8;
       float s[NT][4] = {};
@@ -121,8 +130,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
       }
       product_probabilities<T, DP, NT>(out, s, base + M::kV + stage * M::kTile);
     }
-    __syncthreads();
-    stage ^= 1;
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
   wait_copies<0>();
 #pragma unroll
