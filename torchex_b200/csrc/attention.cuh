@@ -64,10 +64,14 @@ __device__ __forceinline__ T* row_at(const Problem& a, const View& x, int head, 
   return static_cast<T*>(x.p) + row_of(a, pos) * x.row + head * x.head;
 }
 
-struct Bounds { int begin, end; };
+struct Bounds {
+  int begin, end;
+  __device__ __forceinline__ bool holds(int p) const { return unsigned(p - begin) < unsigned(end - begin); }  // begin <= end
+};
 __device__ __forceinline__ Bounds segment_of(const Problem& a, int pos) {
   const int s = min(max(__ldg(a.sid + pos), 0), a.segments - 1);
-  return {max(0, __ldg(a.offsets + s)), min(a.n, __ldg(a.offsets + s + 1))};
+  const int begin = max(0, __ldg(a.offsets + s));
+  return {begin, max(begin, min(a.n, __ldg(a.offsets + s + 1)))};
 }
 // Bounded waits of the kernels for long segments that gave up (part of texb_device_status).
 static __device__ int g_wait_timeouts = 0;
@@ -76,13 +80,13 @@ static __device__ int g_wait_timeouts = 0;
 __device__ __forceinline__ Bounds keys_of(const Problem& a, int pos) {
   if (pos >= a.n) return {0, 0};
   Bounds b = segment_of(a, pos);
-  if (a.causal) b.end = min(b.end, pos + 1);
+  if (a.causal) b.end = max(b.begin, min(b.end, pos + 1));
   return b;
 }
 __device__ __forceinline__ Bounds queries_of(const Problem& a, int pos) {
   if (pos >= a.n) return {0, 0};
   Bounds b = segment_of(a, pos);
-  if (a.causal) b.begin = max(b.begin, pos);
+  if (a.causal) b.begin = min(b.end, max(b.begin, pos));
   return b;
 }
 

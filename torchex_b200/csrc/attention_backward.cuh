@@ -19,14 +19,14 @@ namespace attention {
 
 template <int DP>
 struct QueryMemory {
-  static constexpr int kStages = DP <= 32 ? 4 : 2;
-  static constexpr int kTile = kBlock * DP * 2;
-  static constexpr int kQ = 0, kG = kTile, kK = 2 * kTile, kV = kK + kStages * kTile;
-  static constexpr int kBytes = (2 + 2 * kStages) * kTile;
+  static constexpr int kStages = DP <= 32 ? 4 : 2, kKeys = DP <= 32 ? 32 : 64;
+  static constexpr int kQueries = kBlock * DP * 2, kTile = kKeys * DP * 2;
+  static constexpr int kQ = 0, kG = kQueries, kK = 2 * kQueries, kV = kK + kStages * kTile;
+  static constexpr int kBytes = 2 * kQueries + 2 * kStages * kTile;
 };
 
 template <typename T, int DP, int MODE>
-__global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_kernel(const __grid_constant__ Problem a) {
+__global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) query_gradient_kernel(const __grid_constant__ Problem a) {
   extern __shared__ __align__(128) unsigned char smem[];
   using M = QueryMemory<DP>;
   const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
@@ -34,22 +34,23 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
   const uint32_t base = smem_u32(smem);
-  constexpr int S = M::kStages;
-  Loader<DP, kBlock> queries, ahead[S - 1], loader;
+  constexpr int S = M::kStages, N = M::kKeys;
+  Loader<DP, kBlock> queries;
+  Loader<DP, N> ahead[S - 1], loader;
   queries.look_up(a, pos0, last + 1);
 #pragma unroll
-  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_key + t * kBlock, end_key);
+  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_key + t * N, end_key);
   queries.template copy<T>(a, a.q, head, base + M::kQ);
   queries.template copy<T>(a, a.g, head, base + M::kG);
 #pragma unroll
   for (int t = 0; t < S - 1; ++t) {
-    if (first_key + t * kBlock < end_key) {
+    if (first_key + t * N < end_key) {
       ahead[t].template copy<T>(a, a.k, kv, base + M::kK + t * M::kTile);
       ahead[t].template copy<T>(a, a.v, kv, base + M::kV + t * M::kTile);
     }
     commit_copies();
   }
-  loader.look_up(a, first_key + (S - 1) * kBlock, end_key);
+  loader.look_up(a, first_key + (S - 1) * N, end_key);
   if (any_flag(a, a.bad_k, kv, first_key, end_key)) {  // looked at while the first rows are on their way
     wait_copies<0>();
     plain_query_gradient<T>(a, pos0, kBlock, head);
@@ -67,18 +68,18 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_ker
 
   float gq[DP / 8][4] = {};
   int stage = 0;
-  for (int j0 = first_key; j0 < end_key; j0 += kBlock) {
+  for (int j0 = first_key; j0 < end_key; j0 += N) {
     wait_copies<S - 2>();
     __syncthreads();  // this tile is there, and the stage of the last one is free
-    if (j0 + (S - 1) * kBlock < end_key) {
+    if (j0 + (S - 1) * N < end_key) {
       const int free = stage == 0 ? S - 1 : stage - 1;
       loader.template copy<T>(a, a.k, kv, base + M::kK + free * M::kTile);
       loader.template copy<T>(a, a.v, kv, base + M::kV + free * M::kTile);
     }
     commit_copies();
-    loader.look_up(a, j0 + S * kBlock, end_key);
-    if (j0 + kBlock > warp_begin && j0 < warp_end) {
-      constexpr int NT = kBlock / 8;
+    loader.look_up(a, j0 + S * N, end_key);
+    if (j0 + N > warp_begin && j0 < warp_end) {
+      constexpr int NT = N / 8;
       float s[NT][4] = {}, dp[NT][4] = {};
       product_rows<T, DP, NT>(s, base + M::kQ, row0, base + M::kK + stage * M::kTile);
       product_rows<T, DP, NT>(dp, base + M::kG, row0, base + M::kV + stage * M::kTile);
@@ -90,8 +91,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 5 : 1) query_gradient_ker
           const Score x0 = score_of<MODE>(a, s[t][e], slope, float(i0 - j)), x1 = score_of<MODE>(a, s[t][2 + e], slope, float(i1 - j));
           const float d0 = exp2_fast(x0.x - lse0) * fmaf(dp[t][e], a.scale, -delta0) * x0.slope;
           const float d1 = exp2_fast(x1.x - lse1) * fmaf(dp[t][2 + e], a.scale, -delta1) * x1.slope;
-          dp[t][e] = j >= see0.begin && j < see0.end ? d0 : 0.f;
-          dp[t][2 + e] = j >= see1.begin && j < see1.end ? d1 : 0.f;
+          dp[t][e] = see0.holds(j) ? d0 : 0.f;
+          dp[t][2 + e] = see1.holds(j) ? d1 : 0.f;
         }
       }
       product_probabilities<T, DP, NT, true>(gq, dp, base + M::kK + stage * M::kTile);
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
           const int r = t * 8 + (lane & 3) * 2 + e, i = q0 + r;
           const float lse = s_lse[stage * R + r], delta = s_delta[stage * R + r];
           const Score x0 = score_of<MODE>(a, p[t][e], slope, float(i - j0)), x1 = score_of<MODE>(a, p[t][2 + e], slope, float(i - j1));
-          const bool on0 = i >= seen0.begin && i < seen0.end, on1 = i >= seen1.begin && i < seen1.end;
+          const bool on0 = seen0.holds(i), on1 = seen1.holds(i);
           p[t][e] = on0 ? exp2_fast(x0.x - lse) : 0.f;
           p[t][2 + e] = on1 ? exp2_fast(x1.x - lse) : 0.f;
           ds[t][e] = on0 ? p[t][e] * fmaf(ds[t][e], a.scale, -delta) * x0.slope : 0.f;

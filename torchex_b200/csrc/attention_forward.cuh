@@ -1,7 +1,7 @@
 // Forward kernel of the attention within segments; instantiated by the attention_forward_*.cu files.
 //
 // A CTA of four warps owns 64 query positions of one head, 16 per warp, and walks the keys its rows
-// see in tiles of 64: scores, running maximum and sum (in units of log2), and the product with the
+// see in tiles of 64 (32 for narrow rows): scores, running maximum and sum (in units of log2), and the product with the
 // values stay in registers; keys and values are copied ahead (cp.async, two to four stages).  A warp
 // passes over tiles that none of its 16 rows see, which is what keeps a tile of many short segments
 // cheap, and over the mask where all of its rows see the whole tile.  Probabilities are rounded to the
@@ -16,11 +16,12 @@ namespace attention {
 
 template <typename T, int DP>
 struct ForwardMemory {
-  static constexpr int kStages = DP <= 32 ? 4 : 2;  // narrow rows: all keys of a tile of short segments at once
-  static constexpr int kQ = 0;
-  static constexpr int kTile = kBlock * DP * 2;
-  static constexpr int kK = kTile, kV = kK + kStages * kTile;
-  static constexpr int kBytes = (1 + 2 * kStages) * kTile;
+  static constexpr int kStages = DP <= 32 ? 4 : 2;  // narrow rows: most keys of a tile of short segments at once
+  static constexpr int kKeys = DP <= 32 ? 32 : 64;  // of a stage; fewer where most of a tile of 64 would be masked
+  static constexpr int kQ = 0, kQueries = kBlock * DP * 2;
+  static constexpr int kTile = kKeys * DP * 2;
+  static constexpr int kK = kQueries, kV = kK + kStages * kTile;
+  static constexpr int kBytes = kQueries + 2 * kStages * kTile;
 };
 
 template <typename T, int DP, int MODE>
@@ -33,21 +34,22 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
   const int first_key = keys_of(a, pos0).begin, end_key = keys_of(a, last).end;
 
   const uint32_t base = smem_u32(smem), sq = base + M::kQ;
-  constexpr int S = M::kStages;
-  Loader<DP, kBlock> queries, ahead[S - 1], loader;
+  constexpr int S = M::kStages, N = M::kKeys;
+  Loader<DP, kBlock> queries;
+  Loader<DP, N> ahead[S - 1], loader;
   queries.look_up(a, pos0, last + 1);
 #pragma unroll
-  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_key + t * kBlock, end_key);
+  for (int t = 0; t < S - 1; ++t) ahead[t].look_up(a, first_key + t * N, end_key);
   queries.template copy<T>(a, a.q, head, sq);
 #pragma unroll
   for (int t = 0; t < S - 1; ++t) {
-    if (first_key + t * kBlock < end_key) {
+    if (first_key + t * N < end_key) {
       ahead[t].template copy<T>(a, a.k, kv, base + M::kK + t * M::kTile);
       ahead[t].template copy<T>(a, a.v, kv, base + M::kV + t * M::kTile);
     }
     commit_copies();
   }
-  loader.look_up(a, first_key + (S - 1) * kBlock, end_key);
+  loader.look_up(a, first_key + (S - 1) * N, end_key);
   // looked at while the first rows are on their way
   const bool bad = a.bad_v ? any_flag(a, a.bad_v, kv, first_key, end_key) : look_over<T>(a, a.v, kv, first_key, end_key);
   if (bad) {
@@ -68,21 +70,21 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
   float out[DP / 8][4] = {};
   float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
   int stage = 0;
-  for (int j0 = first_key; j0 < end_key; j0 += kBlock) {
+  for (int j0 = first_key; j0 < end_key; j0 += N) {
     wait_copies<S - 2>();
     __syncthreads();  // this tile is there, and the stage of the last one is free
-    if (j0 + (S - 1) * kBlock < end_key) {
+    if (j0 + (S - 1) * N < end_key) {
       const int free = stage == 0 ? S - 1 : stage - 1;
       loader.template copy<T>(a, a.k, kv, base + M::kK + free * M::kTile);
       loader.template copy<T>(a, a.v, kv, base + M::kV + free * M::kTile);
     }
     commit_copies();
-    loader.look_up(a, j0 + S * kBlock, end_key);
-    if (j0 + kBlock > warp_begin && j0 < warp_end) {
-      constexpr int NT = kBlock / 8;
+    loader.look_up(a, j0 + S * N, end_key);
+    if (j0 + N > warp_begin && j0 < warp_end) {
+      constexpr int NT = N / 8;
       float s[NT][4] = {};
       product_rows<T, DP, NT>(s, sq, row0, base + M::kK + stage * M::kTile);
-      const bool whole = j0 >= all_begin && j0 + kBlock <= all_end;
+      const bool whole = j0 >= all_begin && j0 + N <= all_end;
       float top0_new = top0, top1_new = top1;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -92,8 +94,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
           s[t][e] = score_of<MODE>(a, s[t][e], slope, float(i0 - j)).x;
           s[t][2 + e] = score_of<MODE>(a, s[t][2 + e], slope, float(i1 - j)).x;
           if (!whole) {
-            if (j < see0.begin || j >= see0.end) s[t][e] = -INFINITY;
-            if (j < see1.begin || j >= see1.end) s[t][2 + e] = -INFINITY;
+            if (!see0.holds(j)) s[t][e] = -INFINITY;
+            if (!see1.holds(j)) s[t][2 + e] = -INFINITY;
           }
           top0_new = fmaxf(top0_new, s[t][e]);
           top1_new = fmaxf(top1_new, s[t][2 + e]);

@@ -118,7 +118,7 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
       const float* lse = s_lse + stage * 2 * N;
       const float* delta = lse + N;
       const bool whole = p0 >= all_begin && p0 + N <= all_end;
-      const int from = see.begin - p0, to = see.end - p0;
+      const unsigned from = unsigned(see.begin - p0), count = unsigned(see.end - see.begin);
 #pragma unroll
       for (int c = 0; c < N; c += 32) {
         float s[32], g[32];
@@ -153,7 +153,7 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
             float2 ds = t5::mul2(p, t5::fma2({g[k], g[k + 1]}, scale, {-d.x, -d.y}));
             if constexpr (MODE != kPlain) ds = t5::mul2(ds, bend);
             if (!whole) {  // set, not multiplied: a masked pair's product may be infinite
-              const bool on0 = c + k >= from && c + k < to, on1 = c + k + 1 >= from && c + k + 1 < to;
+              const bool on0 = unsigned(c + k) - from < count, on1 = unsigned(c + k + 1) - from < count;
               p = {on0 ? p.x : 0.f, on1 ? p.y : 0.f};
               ds = {on0 ? ds.x : 0.f, on1 ? ds.y : 0.f};
             }

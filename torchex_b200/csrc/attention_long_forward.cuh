@@ -126,9 +126,9 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
         for (int c = 0; c < N; ++c) s[c] = score_of<MODE>(a, s[c], slope, float(i - j0) - float(c)).x;
       }
       if (!(j0 >= mine.all_begin && j0 + N <= mine.all_end)) {
-        const int from = see.begin - j0, to = see.end - j0;
+        const unsigned from = unsigned(see.begin - j0), count = unsigned(see.end - see.begin);
 #pragma unroll
-        for (int c = 0; c < N; ++c) s[c] = c >= from && c < to ? s[c] : -INFINITY;
+        for (int c = 0; c < N; ++c) s[c] = unsigned(c) - from < count ? s[c] : -INFINITY;
       }
       float most[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
