@@ -488,7 +488,8 @@ typedef struct texb_attention_problem {
   float* lse;                      /* [heads, n]: written by forward (NULL: not wanted), read by backward */
   const void* g;                   /* backward: gradient of out */
   int64_t g_strides[2];
-  void *g_q, *g_k, *g_v;           /* backward: contiguous gradients, every row written */
+  void *g_q, *g_k, *g_v;           /* backward: contiguous gradients, every row written; NULL: not wanted (g_k and
+                                      g_v together) */
 } texb_attention_problem;
 size_t texb_attention_workspace_bytes(int64_t n, int heads, int kv_heads, int backward);
 int texb_attention_forward(const texb_attention_problem* problem, void* workspace, size_t workspace_bytes, void* stream);

@@ -32,7 +32,7 @@ def test_c_abi_rejects_bad_arguments():
                 (2, dict(dtype=0)), (2, dict(dtype=7)), (1, dict(n=-1)), (2, dict(n=1 << 31)), (1, dict(num_segments=-1)),
                 (1, dict(num_segments=0)), (1, dict(heads=0)), (1, dict(kv_heads=0)), (1, dict(kv_heads=3)), (1, dict(dim=0)),
                 (2, dict(dim=12)), (2, dict(dim=136)), (1, dict(softcap=-1.0)), (1, dict(softcap=float("nan"))),
-                (1, dict(scale=float("nan"))), (1, dict(q=None)), (1, dict(v=None)), (1, dict(sid=None)), (1, dict(offsets=None)),
+                (1, dict(scale=float("nan"))), (1, dict(scale=float("inf"))), (1, dict(softcap=float("inf"))), (1, dict(q=None)), (1, dict(v=None)), (1, dict(sid=None)), (1, dict(offsets=None)),
                 (1, dict(out=None)), (2, dict(k=4104)), (2, dict(q_strides=(132, 32))), (2, dict(v_strides=(64, 30))),
                 (2, dict(heads=65535, kv_heads=65535))]:
             assert call(_problem(**changes), 4096, nbytes, None) == status, changes
@@ -40,7 +40,7 @@ def test_c_abi_rejects_bad_arguments():
         assert call(_problem(), None, 0, None) == 3 and call(_problem(), 4096, nbytes - 1, None) == 3
         assert call(_problem(n=0), None, 0, None) == 0  # nothing to do
     assert lib.texb_attention_backward(_problem(lse=None), 4096, need, None) == 1
-    assert lib.texb_attention_backward(_problem(g_k=None), 4096, need, None) == 1
+    assert lib.texb_attention_backward(_problem(g_k=None), 4096, need, None) == 1  # without g_v
 
 
 class _NoPlan:

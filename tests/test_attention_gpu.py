@@ -299,6 +299,18 @@ def test_streams_graphs_and_an_eager_graph_beside():
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+@pytest.mark.parametrize("lens", [[30, 40, 7], [300, 200]])
+def test_gradients_that_are_not_wanted(lens):
+    ids, data = _plan(lens, False)
+    q, k, v, g = _inputs(sum(lens), 2, 1, 64, torch.bfloat16, 6)
+    full = _step(q, k, v, g, data)
+    for wanted in ((0,), (1,), (2,), (0, 2)):
+        ins = [x.detach().clone().requires_grad_(i in wanted) for i, x in enumerate((q, k, v))]
+        out = segment_attention(*ins, data)
+        grads = torch.autograd.grad(out, [ins[i] for i in wanted], g)
+        assert all(torch.equal(a, full[1 + i]) for i, a in zip(wanted, grads))
+
+
 def test_empty_batch_and_refusals():
     data = ScatterData(torch.zeros(0, dtype=torch.int64, device=DEV), torch.zeros(0, dtype=torch.int64, device=DEV))
     e = torch.zeros(0, 2, 16, device=DEV, dtype=torch.float16, requires_grad=True)
@@ -314,6 +326,7 @@ def test_empty_batch_and_refusals():
             ("multiple of 8", tuple(torch.zeros(10, 1, 136, device=DEV, dtype=torch.bfloat16) for _ in range(3)), {}),
             ("evenly", (q[:, :3], kv, kv), {}), ("different numbers", (q, kv, q), {}), ("built for", (q[:9], kv[:9], kv[:9]), {}),
             ("head dimension", (q, kv[..., :8], kv), {}), ("softcap", (q, kv, kv), {"softcap": -1.0}),
+            ("softcap", (q, kv, kv), {"softcap": float("inf")}), ("scale", (q, kv, kv), {"scale": float("nan")}),
             ("per query head", (q, kv, kv), {"slopes": torch.zeros(2, device=DEV)}),
             ("dtype", (q, kv, kv), {"slopes": torch.zeros(4, device=DEV, dtype=torch.float16)}),
             ("no gradient", (q, kv, kv), {"slopes": torch.zeros(4, device=DEV, requires_grad=True)}),

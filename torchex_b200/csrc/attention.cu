@@ -3,6 +3,8 @@
 
 #include "attention_long.cuh"
 
+#include <cmath>
+
 namespace texb {
 namespace attention {
 
@@ -123,11 +125,14 @@ int check(const Problem& a, int dtype, bool backward) {
   if (a.dim % 8 != 0 || a.dim > 128)
     return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: head dimension %d is not a multiple of 8 up to 128", a.dim);
   if (a.heads + a.kv_heads > 65535) return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: too many heads");
-  if (!(a.cap >= 0.f) || !(a.scale == a.scale)) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: bad scale or softcap");
+  if (!(a.cap >= 0.f && a.cap < INFINITY) || !(fabsf(a.scale) < INFINITY))
+    return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: bad scale or softcap");
   if (a.n == 0) return TEXB_OK;
   if (!a.sid || !a.offsets || a.segments == 0) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: NULL plan");
   const View* views[] = {&a.q, &a.k, &a.v, &a.out, &a.g, &a.gq, &a.gk, &a.gv};
+  if (backward && (!a.gk.p != !a.gv.p)) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: g_k and g_v are wanted together");
   for (int i = 0; i < (backward ? 8 : 4); ++i) {
+    if (!views[i]->p && i >= 5) continue;  // a gradient that is not wanted
     if (!views[i]->p) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: NULL pointer");
     if (reinterpret_cast<uintptr_t>(views[i]->p) % 16 != 0 || views[i]->row % 8 != 0 || views[i]->head % 8 != 0)
       return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: rows must be 16-byte aligned");
@@ -143,9 +148,15 @@ inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kFlag)); }  // of
 // doing it: at most three tiles of keys.
 constexpr int kShortSegment = 64;
 
-// Segments so long, on average, that tiles of 128 positions mostly hold one: then the products are matrix
-// products of some size, and run on the 5th-generation tensor cores.
-inline bool long_segments(const Problem& a) { return a.n >= int64_t(a.segments) * 128; }
+// Whether the 5th-generation tensor cores' kernels are used: where segments are long enough, on average, for tiles of
+// 128 rows to be worth it.  Narrow rows are padded to 64 columns there, which takes longer segments to pay.
+// Measured on 16 384 rows, 8 heads, training step, general / long kernels in us: dim 128, average 32: 321 / 258,
+// 64: 383 / 241, 1024: 2543 / 709; dim 64, 32: 215 / 209, 64: 241 / 205; dim 32, 192: 238 / 221 (causal 169 / 189), 512: 449 / 323
+// (280 / 240); dim 16, 512: 311 / 314 (204 / 231), 1024: 562 / 497 (342 / 320).
+inline bool long_segments(const Problem& a) {
+  const int64_t average = a.dim <= 16 ? 768 : a.dim <= 32 ? 256 : 32;
+  return a.n >= a.segments * average;
+}
 
 }  // namespace
 }  // namespace attention

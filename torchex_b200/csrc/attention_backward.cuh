@@ -241,9 +241,11 @@ int launch_backward(const Problem& a, cudaStream_t stream) {
   int st = prepare_kernel(queries, QueryMemory<DP>::kBytes, "attention query_gradient_kernel");
   if (st == TEXB_OK) st = prepare_kernel(keys, KeyMemory<DP>::kBytes, "attention key_gradients_kernel");
   if (st != TEXB_OK) return st;
-  queries<<<dim3(tiles, unsigned(a.heads)), kThreads, QueryMemory<DP>::kBytes, stream>>>(a);
-  st = check_launch("attention query_gradient_kernel");
-  if (st != TEXB_OK) return st;
+  if (a.gq.p) {
+    queries<<<dim3(tiles, unsigned(a.heads)), kThreads, QueryMemory<DP>::kBytes, stream>>>(a);
+    st = check_launch("attention query_gradient_kernel");
+  }
+  if (st != TEXB_OK || !a.gk.p) return st;
   keys<<<dim3(tiles, unsigned(a.kv_heads)), kThreads, KeyMemory<DP>::kBytes, stream>>>(a);
   return check_launch("attention key_gradients_kernel");
 }

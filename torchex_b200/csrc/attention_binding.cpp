@@ -3,6 +3,7 @@
 
 #include "binding.h"
 
+#include <cmath>
 #include <tuple>
 
 namespace texb_binding {
@@ -107,7 +108,13 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     const c10::cuda::CUDAGuard guard(s[0].device());
     const at::Tensor q = readable_rows(s[0]), k = readable_rows(s[1]), v = readable_rows(s[2]), g = readable_rows(grads[0]);
     const at::Tensor out = s[7].contiguous(), low = s[8], lse = s[9];
-    at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
+    const bool want_q = ctx->needs_input_grad(0), want_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    at::Tensor gq, gk, gv;
+    if (want_q) gq = at::empty(q.sizes(), q.options());
+    if (want_kv) {
+      gk = at::empty(k.sizes(), k.options());
+      gv = at::empty(v.sizes(), v.options());
+    }
     texb_attention_problem p = problem_of(q, k, v, s[3], s[4], s[5], s[6], o);
     p.out = out.data_ptr();
     p.out_low = low.data_ptr();
@@ -115,9 +122,9 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     p.g = g.data_ptr();
     p.g_strides[0] = g.stride(0);
     p.g_strides[1] = g.stride(1);
-    p.g_q = gq.data_ptr();
-    p.g_k = gk.data_ptr();
-    p.g_v = gv.data_ptr();
+    p.g_q = want_q ? gq.data_ptr() : nullptr;
+    p.g_k = want_kv ? gk.data_ptr() : nullptr;
+    p.g_v = want_kv ? gv.data_ptr() : nullptr;
     const at::Tensor ws = scratch(texb_attention_workspace_bytes(p.n, p.heads, p.kv_heads, 1), q);
     check_status(texb_attention_backward(&p, ws.data_ptr(), size_t(ws.numel()), stream_of(q)), "texb_attention_backward");
     torch::autograd::variable_list r(12);
@@ -140,7 +147,8 @@ at::Tensor segment_attention(const Plan& plan, const at::Tensor& q, const at::Te
               " key / value heads evenly");
   TORCH_CHECK(q.size(2) >= 8 && q.size(2) <= kMaxDim && q.size(2) % 8 == 0, "the head dimension must be a multiple of 8 up to ",
               kMaxDim, ", got ", q.size(2));
-  TORCH_CHECK(softcap >= 0, "softcap must not be negative, got ", softcap);
+  TORCH_CHECK(softcap >= 0 && std::isfinite(softcap), "softcap must be finite and not negative, got ", softcap);
+  TORCH_CHECK(std::isfinite(scale), "scale must be finite, got ", scale);
   at::Tensor slopes;
   if (slopes_given.has_value() && slopes_given->defined()) {
     TORCH_CHECK(slopes_given->dim() == 1 && slopes_given->size(0) == q.size(1), "slopes must hold one value per query head");

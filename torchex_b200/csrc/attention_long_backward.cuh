@@ -325,8 +325,8 @@ int launch_long_backward(const Problem& a, int dtype, cudaStream_t stream) {
 
 template <typename T, int DP, int MODE>
 int launch_long_backward_both(const Problem& a, int dtype, cudaStream_t stream) {
-  const int st = launch_long_backward<T, DP, MODE, false>(a, dtype, stream);
-  return st == TEXB_OK ? launch_long_backward<T, DP, MODE, true>(a, dtype, stream) : st;
+  const int st = a.gq.p ? launch_long_backward<T, DP, MODE, false>(a, dtype, stream) : TEXB_OK;
+  return st == TEXB_OK && a.gk.p ? launch_long_backward<T, DP, MODE, true>(a, dtype, stream) : st;
 }
 
 template <int DP>

@@ -184,7 +184,8 @@ std::tuple<std::vector<at::Tensor>, at::Tensor> clip_grads(const std::vector<at:
                                size_t(ws.numel()), stream_of(norm)),
                "texb_clip_grads");
   if (given.has_value())
-    for (const at::Tensor& o : outs) torch::autograd::impl::bump_version(o);
+    for (const at::Tensor& o : outs)
+      if (!o.is_inference()) torch::autograd::impl::bump_version(o);
   return {outs, norm};
 }
 
