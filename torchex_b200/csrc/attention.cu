@@ -54,14 +54,59 @@ inline Spread spread_of(int dim, int heads) {
   return s;
 }
 
+// The order in which the long kernels take their tiles of `rows` positions: by falling length of the rows that a
+// tile walks, in 64 classes, so that no long tile begins when the others are done (in order of position a training
+// step of packed documents took an eighth longer).  One CTA; which tile of a class comes first does not matter.
+struct Order {
+  int rows, tiles;
+  int32_t *order, *length;  // both [tiles]
+};
+template <bool KEYS>
+__device__ void order_tiles(const Problem& a, const Order& o) {
+  constexpr int kClasses = 64;
+  __shared__ int s_count[kClasses], s_longest;
+  if (threadIdx.x < kClasses) s_count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s_longest = 1;
+  __syncthreads();
+  int longest = 1;
+  for (int t = threadIdx.x; t < o.tiles; t += kThreads) {
+    const int pos0 = t * o.rows, last = min(a.n, pos0 + o.rows) - 1;
+    const Bounds f = KEYS ? queries_of(a, pos0) : keys_of(a, pos0), l = KEYS ? queries_of(a, last) : keys_of(a, last);
+    const int length = max(1, (l.end - f.begin + 63) / 64);
+    o.length[t] = length;
+    longest = max(longest, length);
+  }
+  atomicMax(&s_longest, longest);
+  __syncthreads();
+  auto class_of = [&](int t) { return kClasses - 1 - int(int64_t(o.length[t]) * (kClasses - 1) / s_longest); };
+  for (int t = threadIdx.x; t < o.tiles; t += kThreads) atomicAdd(&s_count[class_of(t)], 1);  // its own entries of `length`
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int before = 0;
+    for (int c = 0; c < kClasses; ++c) {
+      const int n = s_count[c];
+      s_count[c] = before;
+      before += n;
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < o.tiles; t += kThreads) o.order[atomicAdd(&s_count[class_of(t)], 1)] = t;
+}
+
 // The flags of the blocks of the values (forward: Q_ROWS false, the CTAs along y are groups of kv heads), or, for
 // the backward pass, delta_i = scale g_i . o_i and the flags of the queries or gradients of each head (the first
 // CTAs along y) and of the keys of each kv head.  Bound by HBM: every row is read once.
 template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads)
 look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_spread, int q_groups, float* __restrict__ delta,
-                 uint8_t* __restrict__ bad_q, uint8_t* __restrict__ bad_k) {
+                 uint8_t* __restrict__ bad_q, uint8_t* __restrict__ bad_k, Order queries, Order keys_order) {
   __shared__ int s_bad[kThreads];  // by head of the CTA
+  const int blocks = (a.n + kFlag - 1) / kFlag;
+  if (int(blockIdx.x) >= blocks) {  // one or two CTAs more, for the long kernels
+    if (blockIdx.y == 0) order_tiles<false>(a, queries);
+    else if (BACKWARD && blockIdx.y == 1) order_tiles<true>(a, keys_order);
+    return;
+  }
   const int pos0 = blockIdx.x * kFlag, end = min(a.n, pos0 + kFlag);
   const bool keys = !BACKWARD || int(blockIdx.y) >= q_groups;
   const Spread sp = keys ? k_spread : q_spread;
@@ -112,7 +157,7 @@ look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_sp
   if (bad) s_bad[mine] = 1;
   __syncthreads();
   if (int(threadIdx.x) < sp.heads && first_head + int(threadIdx.x) < heads)
-    (keys ? bad_k : bad_q)[int64_t(first_head + threadIdx.x) * gridDim.x + blockIdx.x] = uint8_t(s_bad[threadIdx.x]);
+    (keys ? bad_k : bad_q)[int64_t(first_head + threadIdx.x) * blocks + blockIdx.x] = uint8_t(s_bad[threadIdx.x]);
 }
 
 int check(const Problem& a, int dtype, bool backward) {
@@ -174,12 +219,42 @@ int attention_timeouts_impl(int* count) {
   return TEXB_OK;
 }
 
+namespace attention {
+namespace {
+struct Workspace {
+  uint8_t *flags, *flags_q;  // of values, or keys; of queries and gradients
+  float* delta;
+  Order queries, keys;
+  size_t bytes;
+};
+Workspace carve(void* ws, int64_t n, int heads, int kv_heads, bool backward) {
+  Workspace w = {};
+  const uintptr_t base = align_up(reinterpret_cast<uintptr_t>(ws), 256);
+  size_t at = 0;
+  auto take = [&](size_t bytes) { void* p = reinterpret_cast<void*>(base + at); at += align_up(bytes, 256); return p; };
+  auto order = [&](int rows) {
+    const size_t tiles = size_t(ceil_div(n, rows));
+    Order o = {rows, int(tiles), nullptr, nullptr};
+    o.order = static_cast<int32_t*>(take(tiles * sizeof(int32_t)));
+    o.length = static_cast<int32_t*>(take(tiles * sizeof(int32_t)));
+    return o;
+  };
+  w.flags = static_cast<uint8_t*>(take(blocks_of(n) * size_t(kv_heads)));
+  w.queries = order(backward ? kLongTile : kLongRows);
+  if (backward) {
+    w.keys = order(kLongTile);
+    w.flags_q = static_cast<uint8_t*>(take(blocks_of(n) * size_t(heads)));
+    w.delta = static_cast<float*>(take(size_t(n) * size_t(heads) * sizeof(float)));
+  }
+  w.bytes = at + 256;
+  return w;
+}
+}  // namespace
+}  // namespace attention
+
 size_t attention_workspace_bytes_impl(int64_t n, int heads, int kv_heads, int backward) {
   if (n < 0 || heads < 1 || kv_heads < 1) return 0;
-  const size_t blocks = attention::blocks_of(n);
-  size_t bytes = align_up(blocks * size_t(kv_heads), 256) + 256;
-  if (backward) bytes += align_up(blocks * size_t(heads), 256) + align_up(size_t(n) * size_t(heads) * sizeof(float), 256);
-  return bytes;
+  return attention::carve(nullptr, n, heads, kv_heads, backward != 0).bytes;
 }
 
 namespace attention {
@@ -241,17 +316,17 @@ int attention_forward_impl(const texb_attention_problem* t, void* workspace, siz
   if (st != TEXB_OK || a.n == 0) return st;
   a.bad_v = nullptr;
   if (t->max_count < 0 || t->max_count > kShortSegment) {
-    const size_t need = attention_workspace_bytes_impl(a.n, a.heads, a.kv_heads, 0);
-    if (!workspace || workspace_bytes < need)
-      return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", need, workspace_bytes);
-    uint8_t* flags = static_cast<uint8_t*>(workspace);
+    const Workspace w = carve(workspace, a.n, a.heads, a.kv_heads, false);
+    if (!workspace || workspace_bytes < w.bytes)
+      return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", w.bytes, workspace_bytes);
     const Spread ks = spread_of(a.dim, a.kv_heads);
-    const dim3 grid(unsigned(blocks_of(a.n)), unsigned(ceil_div(a.kv_heads, ks.heads)));
+    const dim3 grid(unsigned(blocks_of(a.n)) + (long_segments(a) ? 1u : 0u), unsigned(ceil_div(a.kv_heads, ks.heads)));
     auto look = dtype == TEXB_BFLOAT16 ? look_over_kernel<__nv_bfloat16, false> : look_over_kernel<__half, false>;
-    look<<<grid, kThreads, 0, stream>>>(a, ks, ks, 0, nullptr, nullptr, flags);
+    look<<<grid, kThreads, 0, stream>>>(a, ks, ks, 0, nullptr, nullptr, w.flags, w.queries, w.queries);
     st = check_launch("attention look_over_kernel");
     if (st != TEXB_OK) return st;
-    a.bad_v = flags;
+    a.bad_v = w.flags;
+    a.query_order = w.queries.order;
   }
   const int mode = mode_of(a);
   if (a.bad_v && long_segments(a)) {
@@ -272,22 +347,19 @@ int attention_backward_impl(const texb_attention_problem* t, void* workspace, si
   const int dtype = t->dtype;
   st = check(a, dtype, true);
   if (st != TEXB_OK || a.n == 0) return st;
-  const size_t need = attention_workspace_bytes_impl(a.n, a.heads, a.kv_heads, 1);
-  const uintptr_t base = align_up(reinterpret_cast<uintptr_t>(workspace), 256);
-  if (!workspace || workspace_bytes < need)
-    return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", need, workspace_bytes);
-  const size_t blocks = blocks_of(a.n);
-  float* delta = reinterpret_cast<float*>(base);
-  uint8_t* bad_q = reinterpret_cast<uint8_t*>(base + align_up(size_t(a.n) * size_t(a.heads) * sizeof(float), 256));
-  uint8_t* bad_k = bad_q + align_up(blocks * size_t(a.heads), 256);
-  a.delta = delta;
-  a.bad_q = bad_q;
-  a.bad_k = bad_k;
+  const Workspace w = carve(workspace, a.n, a.heads, a.kv_heads, true);
+  if (!workspace || workspace_bytes < w.bytes)
+    return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", w.bytes, workspace_bytes);
+  a.delta = w.delta;
+  a.bad_q = w.flags_q;
+  a.bad_k = w.flags;
+  a.query_order = w.queries.order;
+  a.key_order = w.keys.order;
   const Spread qs = spread_of(a.dim, a.heads), ks = spread_of(a.dim, a.kv_heads);
-  const int q_groups = int(ceil_div(a.heads, qs.heads));
-  const dim3 grid(unsigned(blocks), unsigned(q_groups + ceil_div(a.kv_heads, ks.heads)));
+  const int q_groups = int(ceil_div(a.heads, qs.heads));  // and at least one group of kv heads: two CTAs along y
+  const dim3 grid(unsigned(blocks_of(a.n)) + (long_segments(a) ? 1u : 0u), unsigned(q_groups + ceil_div(a.kv_heads, ks.heads)));
   auto look = dtype == TEXB_BFLOAT16 ? look_over_kernel<__nv_bfloat16, true> : look_over_kernel<__half, true>;
-  look<<<grid, kThreads, 0, stream>>>(a, qs, ks, q_groups, delta, bad_q, bad_k);
+  look<<<grid, kThreads, 0, stream>>>(a, qs, ks, q_groups, w.delta, w.flags_q, w.flags, w.queries, w.keys);
   st = check_launch("attention look_over_kernel");
   if (st != TEXB_OK) return st;
   const int mode = mode_of(a);

@@ -52,6 +52,8 @@ struct Problem {
   // flags of blocks with a value that is not finite, [.., ceil(n / kFlag)]; NULL: look for oneself
   const uint8_t *bad_v, *bad_k;  // per kv head
   const uint8_t* bad_q;          // per head: in q or g
+  // long kernels: the tiles of queries, and of keys, by falling length of what they walk
+  const int32_t *query_order, *key_order;
 };
 
 __device__ __forceinline__ int row_of(const Problem& a, int pos) {

@@ -41,10 +41,10 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;
   const int group = a.heads / a.kv_heads;
-  const int own_head = blockIdx.y;
+  // the heads of a tile side by side, since they share rows; the longest tiles first
+  const int own_heads = KEYS ? a.kv_heads : a.heads, own_head = blockIdx.x % own_heads;
   const int kv = KEYS ? own_head : own_head / group;
-  // the CTAs with the longest streams first: the last queries, or the first keys, of a causal segment
-  const int pos0 = (a.causal && !KEYS ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * kLongTile;
+  const int pos0 = __ldg((KEYS ? a.key_order : a.query_order) + blockIdx.x / own_heads) * kLongTile;
   const int last = min(a.n, pos0 + kLongTile) - 1;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   auto seen_by = [&](int pos) { return KEYS ? queries_of(a, pos) : keys_of(a, pos); };
@@ -318,8 +318,9 @@ int launch_long_backward(const Problem& a, int dtype, cudaStream_t stream) {
   const int query_rows = KEYS ? M::kRows : kLongTile, key_rows = KEYS ? kLongTile : M::kRows;
   maps.used = a.perm == nullptr && make_map(&maps.q, a, a.q, a.heads, query_rows, dtype) && make_map(&maps.g, a, a.g, a.heads, query_rows, dtype) &&
               make_map(&maps.k, a, a.k, a.kv_heads, key_rows, dtype) && make_map(&maps.v, a, a.v, a.kv_heads, key_rows, dtype);
-  const dim3 grid(unsigned((a.n + kLongTile - 1) / kLongTile), unsigned(KEYS ? a.kv_heads : a.heads));
-  kernel<<<grid, kLongThreads, M::kBytes, stream>>>(a, maps);
+  const int64_t grid = ceil_div(a.n, kLongTile) * (KEYS ? a.kv_heads : a.heads);
+  if (grid > INT_MAX) return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: too many rows and heads");
+  kernel<<<unsigned(grid), kLongThreads, M::kBytes, stream>>>(a, maps);
   return check_launch("attention long_backward_kernel");
 }
 

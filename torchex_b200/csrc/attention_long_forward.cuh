@@ -53,9 +53,9 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   unsigned char* smem = raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023);
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;
-  const int head = blockIdx.y, kv = head / (a.heads / a.kv_heads);
-  // the last tiles of a causal segment see the most keys: begin with them
-  const int pos0 = (a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * kLongRows;
+  // the heads of a tile side by side, since they share keys and values; the longest tiles first
+  const int head = blockIdx.x % a.heads, kv = head / (a.heads / a.kv_heads);
+  const int pos0 = __ldg(a.query_order + blockIdx.x / a.heads) * kLongRows;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
   const LongRange range[2] = {range_of(a, pos0), range_of(a, pos0 + kLongTile)};
   const int first_key = range[0].begin, end_key = max(range[0].end, range[1].end);
@@ -307,8 +307,9 @@ int launch_long_forward(const Problem& a, int dtype, cudaStream_t stream) {
   constexpr int keys = LongForwardMemory<DP>::kKeys;
   maps.used = a.perm == nullptr && make_map(&maps.q, a, a.q, a.heads, kLongTile, dtype) && make_map(&maps.k, a, a.k, a.kv_heads, keys, dtype) &&
               make_map(&maps.v, a, a.v, a.kv_heads, keys, dtype);
-  const dim3 grid(unsigned((a.n + kLongRows - 1) / kLongRows), unsigned(a.heads));
-  kernel<<<grid, kLongThreads, bytes, stream>>>(a, maps);
+  const int64_t grid = ceil_div(a.n, kLongRows) * a.heads;
+  if (grid > INT_MAX) return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: too many rows and heads");
+  kernel<<<unsigned(grid), kLongThreads, bytes, stream>>>(a, maps);
   return check_launch("attention long_forward_kernel");
 }
 
