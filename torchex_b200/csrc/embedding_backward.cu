@@ -610,8 +610,10 @@ join_runs_kernel(const int32_t* __restrict__ sid, Tiles t, T* __restrict__ g_wei
 
 // Positions of a tile: 128 where that still gives some 380 threads per SM a tile, less for fewer
 // tokens or narrower rows, down to 8.  Larger tiles mean fewer partial sums through HBM (up to two
-// fp32 rows per tile), smaller ones more rows in flight.
+// fp32 rows per tile), smaller ones more rows in flight.  A batch that fits one tile takes one, which saves
+// joining them, a launch: what a small step costs is its launches.
 inline int tile_positions(int64_t n, int dim) {
+  if (n <= 128) return 128;
   const int64_t threads = ceil_div(dim, 8);  // eight values per lane
   int tile = 128;
   while (tile > 8 && ceil_div(n, tile) * threads < 148 * 384) tile /= 2;

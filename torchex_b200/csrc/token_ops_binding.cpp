@@ -5,7 +5,13 @@
 
 #include "binding.h"
 
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
 #include <algorithm>
+#include <memory>
+#include <mutex>
+#include <string>
 #include <tuple>
 
 namespace texb_binding {
@@ -66,31 +72,45 @@ at::Tensor embedding_backward(const at::Tensor& tokens_in, const at::Tensor& g_i
   return out;
 }
 
-// The autograd node of the lookup.  Compiled: a node written in Python costs more host time per step
-// than the kernels of a small batch take.
-struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
-  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& weight,
-                            double scale, int64_t padding_idx) {
-    ctx->save_for_backward({tokens});
-    ctx->saved_data["vocab"] = weight.dim() == 2 ? weight.size(0) : int64_t(0);
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["padding_idx"] = padding_idx;
-    return embedding_forward(tokens, weight, scale);
-  }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
-                                                 torch::autograd::variable_list g) {
+// The autograd node of the lookup.  A node of its own, set up by hand: a training step on a small batch costs
+// more host time than its kernels take, and the general wrappers (Python's above all) would add to that.
+struct EmbeddingBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable tokens;
+  int64_t vocab = 0, padding_idx = -1;
+  double scale = 1.0;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     TORCH_CHECK(!at::GradMode::is_enabled(), "embedding is differentiable once (create_graph is not supported)");
-    const auto saved = ctx->get_saved_variables();
-    return {at::Tensor(),
-            embedding_backward(saved[0], g[0], ctx->saved_data["vocab"].toInt(), ctx->saved_data["scale"].toDouble(),
-                               ctx->saved_data["padding_idx"].toInt()),
-            at::Tensor(), at::Tensor()};
+    if (!grads[0].defined()) return {at::Tensor()};
+    at::Tensor t;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      t = tokens.unpack();
+    }
+    return {embedding_backward(t, grads[0], vocab, scale, padding_idx)};
   }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    tokens.reset_data();
+  }
+  std::string name() const override { return "EmbeddingBackward"; }
 };
 
 at::Tensor embedding(const at::Tensor& tokens, const at::Tensor& weight, double scale, int64_t padding_idx) {
-  if (at::GradMode::is_enabled() && weight.requires_grad()) return EmbeddingNode::apply(tokens, weight, scale, padding_idx);
-  return embedding_forward(tokens, weight, scale);
+  if (!at::GradMode::is_enabled() || !weight.requires_grad()) return embedding_forward(tokens, weight, scale);
+  at::Tensor out;
+  {
+    const at::NoGradGuard no_grad;
+    out = embedding_forward(tokens, weight, scale);
+  }
+  auto node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(weight));
+  node->tokens = torch::autograd::SavedVariable(tokens, /*is_output=*/false);
+  node->vocab = weight.size(0);
+  node->scale = scale;
+  node->padding_idx = padding_idx;
+  torch::autograd::set_history(out, node);
+  return out;
 }
 
 // ---- gradient clipping -----------------------------------------------------------------
