@@ -40,38 +40,12 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
   unsigned char* smem = raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023);
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;
-  const int group = a.heads / a.kv_heads;
-  // the heads of a tile side by side, since they share rows; the longest tiles first
-  const int own_heads = KEYS ? a.kv_heads : a.heads, own_head = blockIdx.x % own_heads;
-  const int kv = KEYS ? own_head : own_head / group;
-  const int pos0 = __ldg((KEYS ? a.key_order : a.query_order) + blockIdx.x / own_heads) * kLongTile;
-  const int last = min(a.n, pos0 + kLongTile) - 1;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-  auto seen_by = [&](int pos) { return KEYS ? queries_of(a, pos) : keys_of(a, pos); };
-  const Bounds head_bounds = seen_by(pos0), tail_bounds = seen_by(last);
-  const int first = head_bounds.begin, end = tail_bounds.end;
-  // positions that all rows see: between the last beginning and the first end
-  const int all_begin = tail_bounds.begin, all_end = head_bounds.end;
-  const int steps = (end - first + N - 1) / N;  // tiles of one head's stream
-  const int heads = KEYS ? group : 1, total = steps * heads;
-  if (steps <= 0) return;  // a plan without the row itself in its segment
-  bool bad = false;
-  const int looked = min(a.n, first + steps * N);  // tiles are copied whole
-  if (KEYS) {
-    for (int h = 0; h < heads; ++h) bad |= any_flag(a, a.bad_q, kv * group + h, first, looked);
-  } else {
-    bad = any_flag(a, a.bad_k, kv, first, looked);
-  }
-  if (bad) {
-    if (KEYS) plain_key_gradients<T>(a, pos0, kLongTile, kv);
-    else plain_query_gradient<T>(a, pos0, kLongTile, own_head);
-    return;
-  }
   const uint32_t base = t5::smem_u32(smem);
   auto bar = [&](int i) { return base + M::kBarriers + i * 8; };
   enum { kOwnFull = 0, kFull = 1, kEmpty = kFull + S, kScoresFull = kEmpty + S, kWeightsFull = kScoresFull + 2, kDone = kWeightsFull + 2,
          kSettle = kDone + 1 };
   static_assert((kSettle + 1) * 8 <= 128, "room for the barriers");
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   if (threadIdx.x == 0) {
     s_dead = 0;
     t5::barrier_init(bar(kOwnFull), maps.used ? 1 : 4);
@@ -87,11 +61,68 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) t5::tmem_alloc(t5::smem_u32(&s_tmem), M::kColumns);
+  const int group = a.heads / a.kv_heads;
+  // the heads of a tile side by side, since they share rows; the longest tiles first
+  const int own_heads = KEYS ? a.kv_heads : a.heads, own_head = blockIdx.x % own_heads;
+  const int kv = KEYS ? own_head : own_head / group;
+  const int pos0 = __ldg((KEYS ? a.key_order : a.query_order) + blockIdx.x / own_heads) * kLongTile;
+  const int last = min(a.n, pos0 + kLongTile) - 1;
+  auto seen_by = [&](int pos) { return KEYS ? queries_of(a, pos) : keys_of(a, pos); };
+  const Bounds head_bounds = seen_by(pos0), tail_bounds = seen_by(last);
+  const int first = head_bounds.begin, end = tail_bounds.end;
+  // positions that all rows see: between the last beginning and the first end
+  const int all_begin = tail_bounds.begin, all_end = head_bounds.end;
+  const int steps = max(0, (end - first + N - 1) / N);  // tiles of one head's stream
+  const int heads = KEYS ? group : 1, total = steps * heads;
   t5::fence_before_sync();
   __syncthreads();
   t5::fence_after_sync();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   volatile int* dead = &s_dead;
+
+  // Rows in segment order are fetched by the copy engine, the CTA's own and the first of the stream before
+  // anything else.
+  auto stream_head = [&](int h) { return KEYS ? kv * group + h : kv; };
+  auto part = [&](int stage, int which) { return base + M::kStream + (stage * 2 + which) * M::kPart; };
+  auto box = [&](const CUtensorMap& map, uint32_t to, int rows, int full, int h, int pos) {
+#pragma unroll
+    for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (rows * 128), &map, bar(full), b * 64, h, pos);
+  };
+  auto fetch = [&](int u, int step, int head) {
+    const int stage = u % S;
+    t5::barrier_arrive_expect(bar(kFull + stage), 2 * M::kPart);
+    box(KEYS ? maps.q : maps.k, part(stage, 0), N, kFull + stage, stream_head(head), first + step * N);
+    box(KEYS ? maps.g : maps.v, part(stage, 1), N, kFull + stage, stream_head(head), first + step * N);
+  };
+  const int early = min(total, S);
+  if (maps.used && warp == 8 && t5::elect_one() && total > 0) {
+    t5::barrier_arrive_expect(bar(kOwnFull), 2 * M::kOwn);
+    box(KEYS ? maps.k : maps.q, base + M::kOwn1, kLongTile, kOwnFull, own_head, pos0);
+    box(KEYS ? maps.v : maps.g, base + M::kOwn2, kLongTile, kOwnFull, own_head, pos0);
+    for (int u = 0; u < early; ++u) fetch(u, u % steps, u / steps);
+  }
+  bool bad = false;
+  const int looked = steps > 0 ? min(a.n, first + steps * N) : first;  // tiles are copied whole
+  if (KEYS) {
+    for (int h = 0; h < heads; ++h) bad |= any_flag(a, a.bad_q, kv * group + h, first, looked);
+  } else {
+    bad = any_flag(a, a.bad_k, kv, first, looked);
+  }
+  if (bad || total == 0) {
+    if (maps.used && warp == 8 && t5::elect_one() && total > 0) {  // nothing may be under way when this memory is given up
+      t5::barrier_wait(bar(kOwnFull), 0, dead);
+      for (int u = 0; u < early; ++u) {
+        if (KEYS) t5::barrier_arrive(bar(kFull + u));  // in place of lse and delta
+        t5::barrier_wait(bar(kFull + u), 0, dead);
+      }
+    }
+    __syncthreads();
+    if (warp == 12) t5::tmem_free(__shfl_sync(0xffffffffu, s_tmem, 0), M::kColumns);
+    if (total == 0) return;  // a plan without the row itself in its segment
+    if (KEYS) plain_key_gradients<T>(a, pos0, kLongTile, kv);
+    else plain_query_gradient<T>(a, pos0, kLongTile, own_head);
+    return;
+  }
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   const float* s_lse = reinterpret_cast<const float*>(smem + M::kLse);
 
   if (warp < 8) {  // ---- probabilities and gradients of scores
@@ -196,25 +227,12 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
     }
   } else if (warp < 12) {  // ---- copies
     const View &own1 = KEYS ? a.k : a.q, &own2 = KEYS ? a.v : a.g, &stream1 = KEYS ? a.q : a.k, &stream2 = KEYS ? a.g : a.v;
-    auto stream_head = [&](int h) { return KEYS ? kv * group + h : kv; };
-    auto part = [&](int stage, int which) { return base + M::kStream + (stage * 2 + which) * M::kPart; };
     if (maps.used) {
       if (warp == 8 && t5::elect_one()) {
-        const CUtensorMap &o1 = KEYS ? maps.k : maps.q, &o2 = KEYS ? maps.v : maps.g, &s1 = KEYS ? maps.q : maps.k, &s2 = KEYS ? maps.g : maps.v;
-        auto box = [&](const CUtensorMap& map, uint32_t to, int rows, int full, int h, int pos) {
-#pragma unroll
-          for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (rows * 128), &map, bar(full), b * 64, h, pos);
-        };
-        t5::barrier_arrive_expect(bar(kOwnFull), 2 * M::kOwn);
-        box(o1, base + M::kOwn1, kLongTile, kOwnFull, own_head, pos0);
-        box(o2, base + M::kOwn2, kLongTile, kOwnFull, own_head, pos0);
-        int step = 0, head = 0;
-        for (int u = 0; u < total; ++u) {
-          const int stage = u % S;
-          if (u >= S) t5::barrier_wait(bar(kEmpty + stage), (u / S - 1) & 1, dead);
-          t5::barrier_arrive_expect(bar(kFull + stage), 2 * M::kPart);
-          box(s1, part(stage, 0), N, kFull + stage, stream_head(head), first + step * N);
-          box(s2, part(stage, 1), N, kFull + stage, stream_head(head), first + step * N);
+        int step = early % steps, head = early / steps;
+        for (int u = early; u < total; ++u) {
+          t5::barrier_wait(bar(kEmpty + u % S), (u / S - 1) & 1, dead);
+          fetch(u, step, head);
           if (++step == steps) {
             step = 0;
             ++head;
@@ -279,12 +297,11 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
   } else if (warp == 12 && t5::elect_one()) {  // ---- products
     constexpr uint32_t score_instr = t5::instruction<T>(128, N, false), sum_instr = t5::instruction<T>(128, DP, true);
     auto scores_of = [&](int u) { return tmem + M::kScores + (u & 1) * 2 * N; };
-    auto part = [&](int u, int which) { return base + M::kStream + ((u % S) * 2 + which) * M::kPart; };
     auto score = [&](int u) {
       t5::barrier_wait(bar(kFull + u % S), (u / S) & 1, dead);
       t5::fence_after_sync();
-      t5::multiply_columns<DP>(scores_of(u), base + M::kOwn1, kLongTile, part(u, 0), N, score_instr);
-      t5::multiply_columns<DP>(scores_of(u) + N, base + M::kOwn2, kLongTile, part(u, 1), N, score_instr);
+      t5::multiply_columns<DP>(scores_of(u), base + M::kOwn1, kLongTile, part(u % S, 0), N, score_instr);
+      t5::multiply_columns<DP>(scores_of(u) + N, base + M::kOwn2, kLongTile, part(u % S, 1), N, score_instr);
       t5::commit(bar(kScoresFull + (u & 1)));
     };
     t5::barrier_wait(bar(kOwnFull), 0, dead);
@@ -292,8 +309,8 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
     for (int u = 0; u < total; ++u) {
       t5::barrier_wait(bar(kWeightsFull + (u & 1)), (u >> 1) & 1, dead);
       t5::fence_after_sync();
-      if (KEYS) t5::multiply_rows<N>(tmem + M::kSums + DP, scores_of(u), part(u, 1), sum_instr, u > 0);
-      t5::multiply_rows<N>(tmem + M::kSums, scores_of(u) + N, part(u, 0), sum_instr, u > 0);
+      if (KEYS) t5::multiply_rows<N>(tmem + M::kSums + DP, scores_of(u), part(u % S, 1), sum_instr, u > 0);
+      t5::multiply_rows<N>(tmem + M::kSums, scores_of(u) + N, part(u % S, 0), sum_instr, u > 0);
       if (u + S < total) t5::commit(bar(kEmpty + u % S));  // only stages that are filled again
       if (u + 1 == total) t5::commit(bar(kDone));
       // products are done in the order of their issue: new scores may overwrite what these sums read

@@ -53,19 +53,6 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   unsigned char* smem = raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023);
   __shared__ uint32_t s_tmem;
   __shared__ int s_dead;
-  // the heads of a tile side by side, since they share keys and values; the longest tiles first
-  const int head = blockIdx.x % a.heads, kv = head / (a.heads / a.kv_heads);
-  const int pos0 = __ldg(a.query_order + blockIdx.x / a.heads) * kLongRows;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
-  const LongRange range[2] = {range_of(a, pos0), range_of(a, pos0 + kLongTile)};
-  const int first_key = range[0].begin, end_key = max(range[0].end, range[1].end);
-  const int tiles = (end_key - first_key + N - 1) / N;
-  if (tiles <= 0) return;  // a plan without the row itself in its segment
-  // boxes are copied whole: the last one may hold rows behind the last key, which must be finite as well
-  if (any_flag(a, a.bad_v, kv, first_key, min(a.n, first_key + tiles * N))) {
-    plain_forward<T>(a, pos0, kLongRows, head);
-    return;
-  }
   const uint32_t base = t5::smem_u32(smem);
   auto bar = [&](int i) { return base + M::kBarriers + i * 8; };
   // barriers by stage: keys full, keys empty, values full, values empty; by query tile and buffer: scores full,
@@ -73,6 +60,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   enum { kQueries = 0, kKeysFull = 1, kKeysEmpty = kKeysFull + S, kValuesFull = kKeysEmpty + S, kValuesEmpty = kValuesFull + S,
          kScoresFull = kValuesEmpty + S, kWeightsFull = kScoresFull + 4, kDone = kWeightsFull + 4, kSettle = kDone + 4 };
   static_assert((kSettle + 2) * 8 <= 256, "room for the barriers");
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
   if (threadIdx.x == 0) {
     s_dead = 0;
     const int copiers = maps.used ? 1 : 4;
@@ -91,11 +79,48 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) t5::tmem_alloc(t5::smem_u32(&s_tmem), M::kColumns);
+  // the heads of a tile side by side, since they share keys and values; the longest tiles first
+  const int head = blockIdx.x % a.heads, kv = head / (a.heads / a.kv_heads);
+  const int pos0 = __ldg(a.query_order + blockIdx.x / a.heads) * kLongRows;
+  const LongRange range[2] = {range_of(a, pos0), range_of(a, pos0 + kLongTile)};
+  const int first_key = range[0].begin, end_key = max(range[0].end, range[1].end);
+  const int tiles = max(0, (end_key - first_key + N - 1) / N);
   t5::fence_before_sync();
   __syncthreads();
   t5::fence_after_sync();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   volatile int* dead = &s_dead;
+
+  // Rows in segment order are fetched by the copy engine: item 0 queries and keys of tile 0, item 2 j + 1 values of
+  // tile j, item 2 j keys of tile j.  The first of them before anything else.
+  const int items = 2 * tiles, early = min(items, 2 * S);
+  auto fetch = [&](int item) {
+    const int j = item >> 1, stage = j % S, pos = first_key + j * N, full = (item & 1 ? kValuesFull : kKeysFull) + stage;
+    auto box = [&](const CUtensorMap& map, uint32_t to, int rows, int arrival, int h, int p) {
+#pragma unroll
+      for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (rows * 128), &map, bar(arrival), b * 64, h, p);
+    };
+    if (item == 0) {
+      t5::barrier_arrive_expect(bar(kQueries), 2 * M::kTile);
+      for (int t = 0; t < 2; ++t) box(maps.q, base + M::kQ + t * M::kTile, kLongTile, kQueries, head, pos0 + t * kLongTile);
+    }
+    t5::barrier_arrive_expect(bar(full), M::kStage);
+    if (item & 1) box(maps.v, base + M::kV + stage * M::kStage, N, full, kv, pos);
+    else box(maps.k, base + M::kK + stage * M::kStage, N, full, kv, pos);
+  };
+  if (maps.used && warp == 8 && t5::elect_one())
+    for (int item = 0; item < early; ++item) fetch(item);
+  // boxes are copied whole: the last one may hold rows behind the last key, which must be finite as well
+  if (any_flag(a, a.bad_v, kv, first_key, tiles > 0 ? min(a.n, first_key + tiles * N) : first_key) || tiles == 0) {
+    if (maps.used && warp == 8 && t5::elect_one() && tiles > 0) {  // nothing may be under way when this memory is given up
+      t5::barrier_wait(bar(kQueries), 0, dead);
+      for (int item = 0; item < early; ++item) t5::barrier_wait(bar((item & 1 ? kValuesFull : kKeysFull) + (item >> 1)), 0, dead);
+    }
+    __syncthreads();
+    if (warp == 12) t5::tmem_free(__shfl_sync(0xffffffffu, s_tmem, 0), M::kColumns);
+    if (tiles > 0) plain_forward<T>(a, pos0, kLongRows, head);  // (no tiles: a plan without the row itself in its segment)
+    return;
+  }
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   // This warp's query tile, and the tiles of keys that some row of it sees: from `from` on, before `until`.  In
   // registers: looked up by an index in the loops below they took 400 cycles of every 2000.
   const int w = warp < 8 ? warp >> 2 : warp & 1;
@@ -207,30 +232,16 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
       }
     }
   } else if (warp < 12) {  // ---- copies: queries and the first keys, then values and keys in turn
-    // item 0: queries and keys of tile 0; item 2 j + 1: values of tile j; item 2 j: keys of tile j
     auto announce = [&](int item) {
       t5::fence_copies();
       if (item == 0) t5::warp_arrive(bar(kQueries));
       t5::warp_arrive(bar((item & 1 ? kValuesFull : kKeysFull) + (item >> 1) % S));
     };
-    const int items = 2 * tiles;
-    if (maps.used) {
-      if (warp == 8 && t5::elect_one()) {
-        auto box = [&](const CUtensorMap& map, uint32_t to, int rows, int full, int h, int pos) {
-#pragma unroll
-          for (int b = 0; b < DP / 64; ++b) t5::copy_box(to + b * (rows * 128), &map, bar(full), b * 64, h, pos);
-        };
-        for (int item = 0; item < items; ++item) {
-          const int j = item >> 1, stage = j % S, pos = first_key + j * N, full = (item & 1 ? kValuesFull : kKeysFull) + stage;
-          if (j >= S) t5::barrier_wait(bar((item & 1 ? kValuesEmpty : kKeysEmpty) + stage), (j / S - 1) & 1, dead);
-          if (item == 0) {
-            t5::barrier_arrive_expect(bar(kQueries), 2 * M::kTile);
-            for (int t = 0; t < 2; ++t) box(maps.q, base + M::kQ + t * M::kTile, kLongTile, kQueries, head, pos0 + t * kLongTile);
-          }
-          t5::barrier_arrive_expect(bar(full), M::kStage);
-          if (item & 1) box(maps.v, base + M::kV + stage * M::kStage, N, full, kv, pos);
-          else box(maps.k, base + M::kK + stage * M::kStage, N, full, kv, pos);
-        }
+    if (maps.used && warp == 8 && t5::elect_one()) {
+      for (int item = early; item < items; ++item) {
+        const int j = item >> 1;
+        t5::barrier_wait(bar((item & 1 ? kValuesEmpty : kKeysEmpty) + j % S), (j / S - 1) & 1, dead);
+        fetch(item);
       }
     }
     constexpr int kLag = 4;  // items under way
