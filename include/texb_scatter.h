@@ -77,11 +77,13 @@ const char* texb_last_error(void);
  * device.  No counterpart in the reference.
  *   wait_timeouts: bounded device-side waits that expired.  The reduce kernels
  *     wait for their bulk copies with an iteration limit; when it runs out they
- *     count the event and return instead of hanging.
+ *     count the event and return instead of hanging (the attention kernels
+ *     likewise: their results are then wrong).
  *   bad_indices: indices found outside their range in a plan handed to the
  *     reduce kernels (a perm entry outside [0, n), a segment id outside
  *     [0, num_segments), a balance cut outside [0, n]).  The access is skipped or
- *     redirected and counted instead of faulting; the output is then wrong. */
+ *     redirected and counted instead of faulting; the output is then wrong.
+ *     Also tokens outside their table (texb_embedding_*). */
 int texb_device_status(int* wait_timeouts, int* bad_indices);
 
 /* Tuning knobs for experiments: "rows_per_cta" (0 = one wave of CTAs),

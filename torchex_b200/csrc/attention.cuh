@@ -333,8 +333,8 @@ template <typename T>
 __device__ __forceinline__ bool look_over(const Problem& a, const View& x, int head, int begin, int end) {
   const int pieces = a.dim / 8;
   bool bad = false;
-  for (int c = threadIdx.x; c < (end - begin) * pieces; c += kThreads) {
-    const int pos = begin + c / pieces;
+  for (int64_t c = threadIdx.x; c < int64_t(end - begin) * pieces; c += kThreads) {
+    const int pos = begin + int(c / pieces);
     bad |= not_finite<T>(*reinterpret_cast<const uint4*>(row_at<T>(a, x, head, pos) + (c % pieces) * 8));
   }
   return __syncthreads_or(bad);

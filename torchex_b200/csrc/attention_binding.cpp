@@ -142,6 +142,7 @@ at::Tensor segment_attention(const Plan& plan, const at::Tensor& q, const at::Te
   check_rows(q, "q", plan.sid, q);
   check_rows(k, "k", plan.sid, q);
   check_rows(v, "v", plan.sid, q);
+  TORCH_CHECK(q.size(1) + k.size(1) <= 65535, "too many heads");
   TORCH_CHECK(k.size(1) == v.size(1), "k and v have different numbers of heads");
   TORCH_CHECK(q.size(1) >= 1 && k.size(1) >= 1 && q.size(1) % k.size(1) == 0, q.size(1), " query heads do not share ", k.size(1),
               " key / value heads evenly");

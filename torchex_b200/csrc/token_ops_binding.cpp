@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
+#include <climits>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -37,7 +38,7 @@ at::Tensor embedding_forward(const at::Tensor& tokens_in, const at::Tensor& weig
   const at::Tensor tokens = checked_tokens(tokens_in);
   TORCH_CHECK(weight_in.device().is_cuda(), "weight must be a CUDAtensor ");
   TORCH_CHECK(weight_in.dim() == 2, "weight must be [vocab, dim]");
-  TORCH_CHECK(weight_in.size(1) >= 1, "weight needs at least one column");
+  TORCH_CHECK(weight_in.size(1) >= 1 && weight_in.size(1) <= INT_MAX, "weight needs between one and 2^31 - 1 columns");
   TORCH_CHECK(weight_in.device() == tokens.device(), "tokens and weight live on different devices");
   const int dtype = dtype_code(weight_in, "weight");
   const c10::cuda::CUDAGuard guard(tokens.device());
@@ -62,7 +63,7 @@ at::Tensor embedding_backward(const at::Tensor& tokens_in, const at::Tensor& g_i
   const c10::cuda::CUDAGuard guard(tokens.device());
   const at::Tensor g = g_in.contiguous();
   const int64_t n = tokens.numel(), dim = g.size(-1);
-  TORCH_CHECK(dim >= 1, "the gradient needs at least one column");
+  TORCH_CHECK(dim >= 1 && dim <= INT_MAX, "the gradient needs between one and 2^31 - 1 columns");
   at::Tensor out = at::empty({vocab, dim}, g.options());
   const at::Tensor ws = scratch(texb_embedding_backward_workspace_bytes(n, vocab, int(dim)), tokens);
   check_status(texb_embedding_backward(tokens.data_ptr(), int(tokens.element_size()), n, g.data_ptr(), dtype, vocab,
@@ -136,7 +137,7 @@ Tensors gather(const std::vector<at::Tensor>& grads) {
 }
 
 at::Tensor grad_norm(const std::vector<at::Tensor>& grads) {
-  TORCH_CHECK(!grads.empty(), "grad_norm needs at least one tensor");
+  TORCH_CHECK(!grads.empty() && grads.size() <= size_t(INT_MAX), "grad_norm needs at least one tensor");
   const Tensors t = gather(grads);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
@@ -170,7 +171,7 @@ void check_apart(const Tensors& t, const std::vector<at::Tensor>& grads, const s
 
 std::tuple<std::vector<at::Tensor>, at::Tensor> clip_grads(const std::vector<at::Tensor>& grads, double max_norm,
                                                            c10::optional<std::vector<at::Tensor>> given) {
-  TORCH_CHECK(!grads.empty(), "clip_grads needs at least one tensor");
+  TORCH_CHECK(!grads.empty() && grads.size() <= size_t(INT_MAX), "clip_grads needs at least one tensor");
   TORCH_CHECK(max_norm >= 0, "max_norm must not be negative, got ", max_norm);
   const Tensors t = gather(grads);
   const c10::cuda::CUDAGuard guard(grads[0].device());
