@@ -206,25 +206,12 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
     }
     // the sums: one warpgroup writes the keys' gradient, the other the values', or each half of the queries'
     t5::warp_wait(bar(kDone), 0, dead);
-    const bool there = pos < a.n;
+    // all products are done: the CTA's own rows in shared memory are free
+    constexpr int kWritten = KEYS ? DP : DP / 2;
+    unsigned char* rows = smem + (buffer ? M::kOwn2 : M::kOwn1) + (warp & 3) * (32 * kWritten * 2);
     const View& view = !KEYS ? a.gq : buffer ? a.gv : a.gk;
-    T* to = row_at<T>(a, view, own_head, min(pos, a.n - 1));
-    const int c0 = KEYS ? 0 : buffer * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
-    const uint32_t sums = tmem + lanes + M::kSums + (KEYS ? buffer * DP : 0);
-    for (int c = c0; c < c1; c += 32) {
-      float o[32];
-      t5::tmem_load32(sums + c, o);
-      t5::tmem_wait_loads();
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        if (there && c + e < a.dim) {
-          Chunk<T, 16> out;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) out.v[x] = narrow<T>(o[e + x]);
-          store_chunk<T, 16>(to + c + e, out);
-        }
-      }
-    }
+    store_sums<T, kWritten>(a, view, own_head, pos0 + (warp & 3) * 32, tmem + lanes + M::kSums + (KEYS ? buffer * DP : 0),
+                            KEYS ? 0 : buffer * kWritten, rows);
   } else if (warp < 12) {  // ---- copies
     const View &own1 = KEYS ? a.k : a.q, &own2 = KEYS ? a.v : a.g, &stream1 = KEYS ? a.q : a.k, &stream2 = KEYS ? a.g : a.v;
     if (maps.used) {
