@@ -93,7 +93,7 @@ __device__ void order_tiles(const Problem& a, const Order& o) {
   for (int t = threadIdx.x; t < o.tiles; t += kThreads) o.order[atomicAdd(&s_count[class_of(t)], 1)] = t;
 }
 
-// The flags of the blocks of the values (forward: Q_ROWS false, the CTAs along y are groups of kv heads), or, for
+// The flags of the blocks of the values (forward: BACKWARD false, the CTAs along y are groups of kv heads), or, for
 // the backward pass, delta_i = scale g_i . o_i and the flags of the queries or gradients of each head (the first
 // CTAs along y) and of the keys of each kv head.  Bound by HBM: every row is read once.
 template <typename T, bool BACKWARD>

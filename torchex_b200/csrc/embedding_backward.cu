@@ -83,8 +83,7 @@ struct SortLayout {  // shared memory of a sorting CTA, in bytes
   static constexpr int kCounts = 0;                                       // uint16 [kSortWarps][kMaxBins]
   static constexpr int kTotals = kCounts + kSortWarps * kMaxBins * 2;     // uint32 [kMaxCluster][kMaxBins]
   static constexpr int kBase = kTotals + kMaxCluster * kMaxBins * 4;      // uint32 [kMaxBins]
-  static constexpr int kStart = kBase + kMaxBins * 4;                     // uint32 [kMaxBins]
-  static constexpr int kScan = kStart + kMaxBins * 4;                     // uint32 [32]
+  static constexpr int kScan = kBase + kMaxBins * 4;                      // uint32 [32]
   static constexpr int kItems = kScan + 128;                              // uint2 [items of the CTA]
 };
 
@@ -161,7 +160,6 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
   uint16_t(*counts)[kMaxBins] = reinterpret_cast<uint16_t(*)[kMaxBins]>(smem + SortLayout::kCounts);
   uint32_t(*totals)[kMaxBins] = reinterpret_cast<uint32_t(*)[kMaxBins]>(smem + SortLayout::kTotals);
   uint32_t* base = reinterpret_cast<uint32_t*>(smem + SortLayout::kBase);
-  uint32_t* local_start = reinterpret_cast<uint32_t*>(smem + SortLayout::kStart);
   uint32_t* scan = reinterpret_cast<uint32_t*>(smem + SortLayout::kScan);
   uint2* buffer = reinterpret_cast<uint2*>(smem + SortLayout::kItems);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -218,23 +216,6 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
       }
       for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(&totals[rank][d], r)[0] = run;
     }
-    uint32_t start = exclusive_scan(run, scan);
-    if (d < bins) local_start[d] = start;
-    __syncthreads();
-    // The share is first put into digit order in this CTA's own memory (nobody writes into it before
-    // the next cluster barrier), so that the stores into the other CTAs' memory run along consecutive
-    // words: 8-byte stores to scattered places of the cluster took 25 of a pass's 32 us at 131 072 tokens.
-#pragma unroll
-    for (int k = 0; k < kMaxItems; ++k) {
-      if (k < items && mine + k * 32 < share) {
-        const uint32_t dg = (item[k].x >> shift) & (bins - 1);
-        buffer[local_start[dg] + counts[warp][dg] + order[k]] = item[k];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kMaxItems; ++k)
-      if (k < items && k * kSortThreads + int(threadIdx.x) < share) item[k] = buffer[k * kSortThreads + threadIdx.x];
     cluster.sync();
     // place of this CTA's first item of each digit: all items of smaller digits, and those of this
     // digit in earlier CTAs
@@ -246,14 +227,17 @@ sort_and_clear_kernel(const IdT* __restrict__ tokens, int n, int64_t vocab, int6
         all += t;
       }
     }
-    start = exclusive_scan(all, scan);
-    if (d < bins) base[d] = start + earlier - local_start[d];
+    const uint32_t start = exclusive_scan(all, scan);
+    if (d < bins) base[d] = start + earlier;
     __syncthreads();
+    // Straight to their places in the cluster's memory.  Putting the share into digit order in the CTA's own
+    // memory first, so that these stores run along consecutive words, took longer: 25 us instead of 23 for the
+    // whole gradient of 1024 tokens (32768 rows of 8 columns), 79 instead of 75 for 131072 (131072 rows of 8).
 #pragma unroll
     for (int k = 0; k < kMaxItems; ++k) {
-      const int at = k * kSortThreads + int(threadIdx.x);  // place in the CTA's digit order
-      if (k < items && at < share) {
-        const uint32_t to = base[(item[k].x >> shift) & (bins - 1)] + uint32_t(at);  // < n <= ranks * per_cta
+      if (k < items && mine + k * 32 < share) {
+        const uint32_t dg = (item[k].x >> shift) & (bins - 1);
+        const uint32_t to = base[dg] + counts[warp][dg] + order[k];  // < n <= ranks * per_cta
         cluster.map_shared_rank(buffer, to >> shift_cta)[to & (per_cta - 1)] = item[k];
       }
     }
@@ -433,7 +417,7 @@ __device__ __forceinline__ void fetch(Chunk<T, BYTES>* to, const T* from) {
 // three batches deep, in which every lane reads only what it copied itself -- so the copies need no
 // barrier, and a run's end does not hold back the loads behind it.  Walking the rows of a batch is a
 // loop, not unrolled: eight copies of the code that closes a run (division of the work between row and
-// slot, stores) overflowed the instruction cache, and took 27 us instead of 9 for 16 384 rows of 1024.
+// slot, stores) overflowed the instruction cache: 27 us instead of 16 for 16 384 rows of 1024.
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(kSumThreads)
 sum_tiles_kernel(const T* __restrict__ g, const int32_t* __restrict__ sid, const int32_t* __restrict__ perm, Tiles t,
@@ -699,7 +683,7 @@ int launch_sort_and_clear(const IdT* tokens, int64_t n, int64_t vocab, int64_t p
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   // Clearing CTAs: at least 64 KB of table each, and no more than run beside the sort at once -- a
-  // cluster that had to wait for a free one doubled the time (239 us instead of 105 for 0.7 GB).
+  // cluster that had to wait for a free one starts when the others end (239 us instead of 143 for 0.7 GB).
   int64_t workers = ceil_div(vocab * row_words * int64_t(sizeof(W)), 65536);
   cfg.gridDim = dim3(unsigned(ranks) * 2);
   const int clusters = resident_clusters(kernel, cfg, ranks, items);
