@@ -55,3 +55,13 @@ def test_operator_rejects_bad_arguments():
     with pytest.raises(TypeError):
         segment_attention(q, q, q, _NoPlan())
     assert callable(scatter_ext.segment_attention)
+
+
+def test_c_abi_rejects_caps_out_of_range():
+    """A cap whose factors (2 scale / cap, cap, each in units of log2) leave fp32 would turn scores of 0 into NaN."""
+    lib = _native.lib()
+    need = lib.texb_attention_workspace_bytes(10, 4, 2, 1)
+    for changes in (dict(softcap=1e-45), dict(softcap=3e38), dict(softcap=1e-30, scale=1e10)):
+        assert lib.texb_attention_forward(_problem(**changes), 4096, need, None) == 2, changes
+        assert lib.texb_attention_backward(_problem(**changes), 4096, need, None) == 2, changes
+        assert "softcap" in _native.last_error()

@@ -337,3 +337,24 @@ def test_empty_batch_and_refusals():
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(segment_attention(x, kv, kv, data).sum(), x, create_graph=True)
     assert not segment_attention(x.detach(), kv, kv, data).requires_grad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,dim", [([70, 1, 200], 16), ([200, 150], 64), ([200, 150], 128)])
+def test_cap_far_above_the_scores(dtype, lens, dim):
+    """A cap of a million leaves scores of a few units what they are (cap tanh(x / cap) = x to 1e-11), so the formulas
+    without a cap hold.  Beside the roundings that their bound counts for a score x, (dim + 4 + 4) 2^-24 |x| at least,
+    the cap has nine: two factors, two products with them, five of the series; so twice the bound is enough, and a
+    hundredth for its curvature."""
+    ids, data = _plan(lens, True, 3)
+    q, k, v, g = _inputs(sum(lens), 4, 2, dim, dtype, 7)
+    want = [(value, 2.01 * bound) for value, bound in _definition(q, k, v, g, ids, len(lens), dim ** -0.5, False, 0.0, None)]
+    _check(_step(q, k, v, g, data, softcap=1e6), want)
+
+
+def test_caps_out_of_range_are_refused():
+    ids, data = _plan([4, 6], False)
+    q = torch.zeros(10, 4, 16, device=DEV, dtype=torch.bfloat16)
+    for cap in (1e-300, 1e-42, 3e38):
+        with pytest.raises(RuntimeError, match="softcap"):
+            segment_attention(q, q, q, data, softcap=cap)

@@ -3,6 +3,7 @@
 
 #include "attention_long.cuh"
 
+#include <cfloat>
 #include <cmath>
 
 namespace texb {
@@ -172,6 +173,9 @@ int check(const Problem& a, int dtype, bool backward) {
   if (a.heads + a.kv_heads > 65535) return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: too many heads");
   if (!(a.cap >= 0.f && a.cap < INFINITY) || !(fabsf(a.scale) < INFINITY))
     return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: bad scale or softcap");
+  // 0 times an infinite factor would be NaN, not a score of 0
+  if (a.cap > 0.f && !(a.cap >= FLT_MIN && fabsf(a.bend_in) < INFINITY && a.bend_out < INFINITY))
+    return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: softcap %g is out of range for scale %g", a.cap, a.scale);
   if (a.n == 0) return TEXB_OK;
   if (!a.sid || !a.offsets || a.segments == 0) return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: NULL plan");
   const View* views[] = {&a.q, &a.k, &a.v, &a.out, &a.g, &a.gq, &a.gk, &a.gv};

@@ -105,7 +105,9 @@ __device__ __forceinline__ float reciprocal_fast(float x) {  // 1 unit in the la
 
 // The score in units of log2, from the plain product of a query and a key, and its derivative by scale *
 // product.  tanh y = 1 - 2 / (exp(2 y) + 1), off by a few 2^-24 whatever y is: the exponential is infinite or 0
-// for large |y|, and tanh then +-1.  `slope` is the head's, in units of log2.
+// for large |y|, and tanh then +-1.  Where |y| is small, that error is no small part of tanh y (a cap far above the
+// scores would lose them), and y - y^3 / 3 is taken: the next term of the series is below 2^-23 of it for |y| < 0.03.
+// `slope` is the head's, in units of log2.
 struct Score { float x, slope; };
 // How scores are formed: scaled (by a positive factor) and nothing else; with a bias by distance, or any factor;
 // capped, with or without that.  A template parameter: the choice made per score took a third of the capped kernels' time.
@@ -115,7 +117,11 @@ template <int MODE>
 __device__ __forceinline__ Score score_of(const Problem& a, float product, float slope, float distance) {
   if constexpr (MODE == kPlain) return {product * a.unit, 1.f};
   if constexpr (MODE == kBiased) return {fmaf(-slope, fabsf(distance), product * a.unit), 1.f};
-  const float t = fmaf(-2.f, reciprocal_fast(exp2_fast(product * a.bend_in) + 1.f), 1.f);
+  constexpr float kUnit = 0.34657359f;  // y = z log(2) / 2
+  const float z = product * a.bend_in, z2 = z * z;
+  const float small = z * fmaf(z2, -1.f / 3.f * kUnit * kUnit * kUnit, kUnit);
+  const float large = fmaf(-2.f, reciprocal_fast(exp2_fast(z) + 1.f), 1.f);
+  const float t = z2 < 0.0075f ? small : large;
   return {fmaf(-slope, fabsf(distance), a.bend_out * t), fmaf(-t, t, 1.f)};
 }
 __device__ __forceinline__ Score any_score(const Problem& a, float product, float slope, float distance) {

@@ -149,6 +149,7 @@ at::Tensor segment_attention(const Plan& plan, const at::Tensor& q, const at::Te
   TORCH_CHECK(q.size(2) >= 8 && q.size(2) <= kMaxDim && q.size(2) % 8 == 0, "the head dimension must be a multiple of 8 up to ",
               kMaxDim, ", got ", q.size(2));
   TORCH_CHECK(softcap >= 0 && std::isfinite(softcap), "softcap must be finite and not negative, got ", softcap);
+  TORCH_CHECK(softcap == 0 || float(softcap) > 0.f, "softcap ", softcap, " is out of the range of float32");
   TORCH_CHECK(std::isfinite(scale), "scale must be finite, got ", scale);
   at::Tensor slopes;
   if (slopes_given.has_value() && slopes_given->defined()) {
