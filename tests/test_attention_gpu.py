@@ -358,3 +358,16 @@ def test_caps_out_of_range_are_refused():
     for cap in (1e-300, 1e-42, 3e38):
         with pytest.raises(RuntimeError, match="softcap"):
             segment_attention(q, q, q, data, softcap=cap)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    ids, data = _plan([4, 6], False)
+    q = torch.zeros(10, 4, 16, device=DEV, dtype=torch.bfloat16)
+    with fwd.dual_level():
+        for i in range(3):
+            args = [q, q, q]
+            args[i] = fwd.make_dual(q, torch.ones_like(q))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                segment_attention(*args, data)

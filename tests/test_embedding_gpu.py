@@ -220,3 +220,15 @@ def test_gradient_only_where_it_is_wanted():
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(out, w, create_graph=True)
     assert math.isfinite(out.item())
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    w, tok = torch.randn(9, 4, device=DEV), torch.tensor([1, 2], device=DEV)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            embedding(tok, fwd.make_dual(w, torch.ones_like(w)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            embedding(tok, fwd.make_dual(w.clone().requires_grad_(True), torch.ones_like(w)))
+        assert embedding(tok, w).shape == (2, 4)

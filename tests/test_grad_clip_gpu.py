@@ -206,3 +206,20 @@ def test_streams_and_graph_replay():
     for h, (outs, n) in zip(held, results):
         ref, nr = clip_grads(h, 1.5)
         assert torch.equal(n, nr) and all(torch.equal(a, b) for a, b in zip(outs, ref))
+
+
+def test_tensors_that_require_a_gradient():
+    """Neither result has a gradient, so it is not taken from tensors that would record one."""
+    p = torch.nn.Parameter(torch.full((16,), 2.0, device=DEV))
+    x = torch.ones(16, device=DEV)
+    for call in (lambda: grad_norm([p]), lambda: clip_grads([p], 1.0), lambda: clip_grads([x], 1.0, out=[p]),
+                 lambda: grad_norm([p * 2])):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call()
+    assert (p == 2).all()
+    with torch.no_grad():
+        assert grad_norm([p]).item() == 8.0
+    p.grad, = torch.autograd.grad((p * p).sum(), p, create_graph=True)  # 2 p
+    assert p.grad.requires_grad
+    assert clip_grad_norm_(p, 8.0).item() == 16.0
+    assert torch.allclose(p.grad, torch.full_like(x, 2.0))

@@ -62,6 +62,7 @@ void check_rows(const at::Tensor& t, const char* name, const at::Tensor& sid, co
   TORCH_CHECK(t.device() == sid.device(), name, " and ScatterData live on different devices");
   TORCH_CHECK(t.size(0) == sid.numel(), name, " has ", t.size(0), " rows but ScatterData was built for ", sid.numel());
   TORCH_CHECK(t.size(2) == q.size(2), name, " has another head dimension than q");
+  check_no_tangent(t, name);
 }
 
 // out and, where a gradient will be wanted, what rounding took from it and the log-sums of the rows

@@ -21,6 +21,11 @@ namespace texb_binding {
 #define TEXB_CHECK_DTYPE(x, t) \
   TORCH_CHECK((x).scalar_type() == (t), #x, " must have dtype ", (t), ", got ", (x).scalar_type())
 
+// Forward-mode derivatives are not computed: a tensor that carries one is refused, not read as a constant.
+inline void check_no_tangent(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name, " carries a forward-mode derivative, which is not supported");
+}
+
 inline void check_status(int status, const char* what) {
   TORCH_CHECK(status == TEXB_OK, what, " failed with status ", status, ": ", texb_last_error());
 }

@@ -38,6 +38,7 @@ at::Tensor embedding_forward(const at::Tensor& tokens_in, const at::Tensor& weig
   const at::Tensor tokens = checked_tokens(tokens_in);
   TORCH_CHECK(weight_in.device().is_cuda(), "weight must be a CUDAtensor ");
   TORCH_CHECK(weight_in.dim() == 2, "weight must be [vocab, dim]");
+  check_no_tangent(weight_in, "weight");
   TORCH_CHECK(weight_in.size(1) >= 1 && weight_in.size(1) <= INT_MAX, "weight needs between one and 2^31 - 1 columns");
   TORCH_CHECK(weight_in.device() == tokens.device(), "tokens and weight live on different devices");
   const int dtype = dtype_code(weight_in, "weight");
@@ -136,8 +137,17 @@ Tensors gather(const std::vector<at::Tensor>& grads) {
   return r;
 }
 
+// The norm and the scaled tensors have no gradient: where one would be recorded, the call is refused, so that a
+// penalty on the norm does not silently lose its own.
+void check_no_gradient(const std::vector<at::Tensor>& tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor& t : tensors)
+    TORCH_CHECK(!t.requires_grad(), "grad_norm and clip_grads are not differentiable: detach the tensors, or call them under torch.no_grad()");
+}
+
 at::Tensor grad_norm(const std::vector<at::Tensor>& grads) {
   TORCH_CHECK(!grads.empty() && grads.size() <= size_t(INT_MAX), "grad_norm needs at least one tensor");
+  check_no_gradient(grads);
   const Tensors t = gather(grads);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
@@ -173,11 +183,13 @@ std::tuple<std::vector<at::Tensor>, at::Tensor> clip_grads(const std::vector<at:
                                                            c10::optional<std::vector<at::Tensor>> given) {
   TORCH_CHECK(!grads.empty() && grads.size() <= size_t(INT_MAX), "clip_grads needs at least one tensor");
   TORCH_CHECK(max_norm >= 0, "max_norm must not be negative, got ", max_norm);
+  check_no_gradient(grads);
   const Tensors t = gather(grads);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   std::vector<at::Tensor> outs;
   if (given.has_value()) {
     outs = std::move(*given);
+    check_no_gradient(outs);
     TORCH_CHECK(outs.size() == grads.size(), "out has ", outs.size(), " tensors for ", grads.size(), " gradients");
     for (size_t i = 0; i < outs.size(); ++i) {
       const at::Tensor &o = outs[i], &g = grads[i];

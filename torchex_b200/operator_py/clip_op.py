@@ -13,7 +13,8 @@ from .. import scatter_ext as _ext
 
 def grad_norm(grads) -> torch.Tensor:
     """2-norm over all values of a sequence of tensors (float32, bfloat16 or float16, dense in
-    memory, on one device): a float32 tensor without axes on that device.  Does not synchronise."""
+    memory, on one device): a float32 tensor without axes on that device.  Does not synchronise.
+    Not differentiable: tensors that require a gradient are taken under ``torch.no_grad()`` only."""
     return _ext.grad_norm(list(grads))
 
 
@@ -24,7 +25,7 @@ def clip_grads(grads, max_norm: float, out=None):
     ``out`` (a sequence, one tensor per gradient, of the same shape and strides) receives the
     results: new tensors if it is None, ``grads`` itself for scaling in place, or for instance the
     float32 gradients that an optimizer keeps beside 16-bit ones (each output has the dtype of its
-    gradient or float32).  Outputs overlap neither each other nor another gradient.  Does not
+    gradient or float32).  Not differentiable, as ``grad_norm``.  Outputs overlap neither each other nor another gradient.  Does not
     synchronise; an infinite or NaN norm shows in the results as it does in
     ``torch.nn.utils.clip_grad_norm_`` with ``error_if_nonfinite=False``."""
     if not max_norm >= 0:
@@ -41,4 +42,5 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    return clip_grads(grads, max_norm, out=grads)[1]
+    with torch.no_grad():  # gradients of a backward pass with create_graph require one themselves
+        return clip_grads(grads, max_norm, out=grads)[1]
