@@ -371,3 +371,20 @@ def test_forward_mode_is_refused():
             args[i] = fwd.make_dual(q, torch.ones_like(q))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 segment_attention(*args, data)
+
+
+@pytest.mark.parametrize("n,heads", [(70, 1), (1, 3), (1, 1)])
+def test_strides_of_axes_of_one(n, heads):
+    """The stride of an axis of size one says nothing, whatever it is."""
+    ids, data = _plan([n], False)
+    q, k, v, g = _inputs(n, heads, heads, 16, torch.bfloat16, 4)
+    want = _step(q, k, v, g, data)
+
+    def odd(x):
+        strides = [1 if size == 1 else stride for size, stride in zip(x.shape, x.stride())]
+        y = x.as_strided(x.shape, strides)
+        assert y.is_contiguous() and torch.equal(x, y)
+        return y
+
+    for a, b in zip(_step(odd(q), odd(k), odd(v), odd(g), data), want):
+        assert torch.equal(a, b)

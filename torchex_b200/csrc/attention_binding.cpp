@@ -14,9 +14,15 @@ constexpr int64_t kMaxDim = 128;
 // Rows that the kernels can read where they are: contiguous along the head dimension, every row of every
 // head on a 16-byte boundary (a slice of a fused projection qualifies).  Others are copied.
 at::Tensor readable_rows(const at::Tensor& t) {
-  const bool fine = (t.size(2) == 1 || t.stride(2) == 1) && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0;
+  const bool fine = t.stride(2) == 1 && (t.size(0) == 1 || t.stride(0) % 8 == 0) && (t.size(1) == 1 || t.stride(1) % 8 == 0);
   const at::Tensor r = fine ? t : t.contiguous();
   return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
+// Strides of the rows and heads; torch leaves that of an axis of size one open.
+void strides_of(const at::Tensor& t, int64_t* to) {
+  to[0] = t.size(0) == 1 ? t.size(1) * t.size(2) : t.stride(0);
+  to[1] = t.size(1) == 1 ? t.size(2) : t.stride(1);
 }
 
 struct Options {
@@ -31,11 +37,9 @@ texb_attention_problem problem_of(const at::Tensor& q, const at::Tensor& k, cons
   p.q = q.data_ptr();
   p.k = k.data_ptr();
   p.v = v.data_ptr();
-  for (int i = 0; i < 2; ++i) {
-    p.q_strides[i] = q.stride(i);
-    p.k_strides[i] = k.stride(i);
-    p.v_strides[i] = v.stride(i);
-  }
+  strides_of(q, p.q_strides);
+  strides_of(k, p.k_strides);
+  strides_of(v, p.v_strides);
   p.dtype = q.scalar_type() == at::kBFloat16 ? TEXB_BFLOAT16 : TEXB_FLOAT16;
   p.sid = sid.data_ptr<int>();
   p.perm = perm.defined() ? perm.data_ptr<int>() : nullptr;
@@ -121,8 +125,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     p.out_low = low.data_ptr();
     p.lse = lse.data_ptr<float>();
     p.g = g.data_ptr();
-    p.g_strides[0] = g.stride(0);
-    p.g_strides[1] = g.stride(1);
+    strides_of(g, p.g_strides);
     p.g_q = want_q ? gq.data_ptr() : nullptr;
     p.g_k = want_kv ? gk.data_ptr() : nullptr;
     p.g_v = want_kv ? gv.data_ptr() : nullptr;
