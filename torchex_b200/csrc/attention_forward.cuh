@@ -7,6 +7,8 @@
 // cheap, and over the mask where all of its rows see the whole tile.  Probabilities are rounded to the
 // type of the values before the second product, which the matrix instructions require: half a step
 // of that type each (2^-8 for bf16), averaged over the keys.
+// Bound: instruction issue (masks and exponentials; for heads of 16 columns there are eight multiply-adds to each).
+// Measured: 20 000 rows, 8 heads of 16, segments up to 128: 30 us, issue slots 58 % busy.
 #pragma once
 
 #include "attention.cuh"

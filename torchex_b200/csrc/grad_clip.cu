@@ -5,9 +5,11 @@
 // A list is one launch per pass, whatever the number and sizes of its tensors: pointers and sizes
 // travel in the kernel's parameters (no copy to the device, so the call can be captured in a
 // graph), the tensors are cut into chunks of 16 KB, and one resident wave of CTAs walks the
-// chunks with 64 bytes of loads in flight per thread.  The second pass walks them from the last to the first, so that what the first pass
-// read last still comes from L2, and stores past it; it reads the coefficient's partial sums itself,
-// which saves a launch, and leaves tensors that are scaled in place alone when the coefficient is 1.
+// chunks with 64 bytes of loads in flight per thread.  The second pass walks them from the last to the first,
+// so that what the first pass read last still comes from L2, and stores past it; it reads the coefficient's
+// partial sums itself, which saves a launch, and leaves tensors that are scaled in place alone when the
+// coefficient is 1.  Measured: 100 M bf16 values in 60 tensors, read twice and written once, 104 us (5.8 TB/s of
+// all bytes moved); 400 M into fp32 559 us; 60 000 values 10.6 us, which is the two launches.
 //
 // The squares of eight values are added in fp32, everything above that in fp64: the result is
 // within a few 2^-24 of the exact norm whatever the number of values.  A group of eight whose sum
