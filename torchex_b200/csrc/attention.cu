@@ -194,7 +194,8 @@ int check(const Problem& a, int dtype, bool backward) {
 inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kFlag)); }  // of flags
 
 // Segments short enough that a tile looks at the values of its keys itself instead of a pass of its own
-// doing it: at most three tiles of keys.
+// doing it: at most three tiles of keys.  Either way the same blocks of positions decide, and the kernels are chosen by
+// `long_segments` alone: whether the host knows the longest segment yet does not show in the results.
 constexpr int kShortSegment = 64;
 
 // Whether the 5th-generation tensor cores' kernels are used: where segments are long enough, on average, for tiles of
@@ -319,12 +320,13 @@ int attention_forward_impl(const texb_attention_problem* t, void* workspace, siz
   st = check(a, dtype, false);
   if (st != TEXB_OK || a.n == 0) return st;
   a.bad_v = nullptr;
-  if (t->max_count < 0 || t->max_count > kShortSegment) {
+  const bool use_long = long_segments(a);
+  if (use_long || t->max_count < 0 || t->max_count > kShortSegment) {
     const Workspace w = carve(workspace, a.n, a.heads, a.kv_heads, false);
     if (!workspace || workspace_bytes < w.bytes)
       return fail(TEXB_ERR_WORKSPACE, "segment_attention workspace: need %zu bytes, got %zu", w.bytes, workspace_bytes);
     const Spread ks = spread_of(a.dim, a.kv_heads);
-    const dim3 grid(unsigned(blocks_of(a.n)) + (long_segments(a) ? 1u : 0u), unsigned(ceil_div(a.kv_heads, ks.heads)));
+    const dim3 grid(unsigned(blocks_of(a.n)) + (use_long ? 1u : 0u), unsigned(ceil_div(a.kv_heads, ks.heads)));
     auto look = dtype == TEXB_BFLOAT16 ? look_over_kernel<__nv_bfloat16, false> : look_over_kernel<__half, false>;
     look<<<grid, kThreads, 0, stream>>>(a, ks, ks, 0, nullptr, nullptr, w.flags, w.queries, w.queries);
     st = check_launch("attention look_over_kernel");
@@ -333,7 +335,7 @@ int attention_forward_impl(const texb_attention_problem* t, void* workspace, siz
     a.query_order = w.queries.order;
   }
   const int mode = mode_of(a);
-  if (a.bad_v && long_segments(a)) {
+  if (use_long) {
     if (a.dim <= 64) return long_forward_by_type<64>(a, dtype, mode, stream);
     return long_forward_by_type<128>(a, dtype, mode, stream);
   }

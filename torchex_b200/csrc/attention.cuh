@@ -334,11 +334,16 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return bad;
 }
 
-// Whether positions [begin, end) of head `head` hold one; called by the whole CTA.
+// Whether positions [begin, end) of head `head`, or others of the blocks of kFlag that they lie in, hold one: what
+// `any_flag` says from the flags of the blocks.  Called by the whole CTA.
 template <typename T>
 __device__ __forceinline__ bool look_over(const Problem& a, const View& x, int head, int begin, int end) {
   const int pieces = a.dim / 8;
   bool bad = false;
+  if (begin < end) {
+    begin = begin / kFlag * kFlag;
+    end = min(a.n, (end + kFlag - 1) / kFlag * kFlag);
+  }
   for (int64_t c = threadIdx.x; c < int64_t(end - begin) * pieces; c += kThreads) {
     const int pos = begin + int(c / pieces);
     bad |= not_finite<T>(*reinterpret_cast<const uint4*>(row_at<T>(a, x, head, pos) + (c % pieces) * 8));
