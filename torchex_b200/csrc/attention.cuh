@@ -17,6 +17,7 @@
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include "vector_io.cuh"
 
@@ -156,6 +157,20 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return reinterpret_cast<const uint32_t&>(v);
 }
 
+// How far probabilities are lifted before they are rounded to T: 2^LIFT times, by subtracting as much less from the
+// scores, which costs nothing, and sums of them alike.  fp16's normal numbers end at 2^-14, and below 2^-25 it has none:
+// a row of keys that each take 2^-20 of the weight would lose most of it.  Its largest is 65504, so a probability of
+// 2^(15 - LIFT) may be lifted; for scores beyond 2^24, whose steps in fp32 are more than 1, it may come out as 2^16 and
+// is held at the largest number (a NaN stays one).  bf16 has fp32's exponents.
+template <typename T> constexpr bool kShortRange = std::is_same<T, __half>::value;
+template <typename T, int LIFT> constexpr float kLifted = kShortRange<T> ? float(LIFT) : 0.f;
+template <typename T> __device__ __forceinline__ uint32_t pack_lifted(float lo, float hi) {
+  if constexpr (!kShortRange<T>) return pack2<T>(lo, hi);
+  uint32_t v;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -256,7 +271,8 @@ __device__ __forceinline__ void product_rows(float (&acc)[NT][4], uint32_t a, in
 }
 
 // acc [16 x DP] += P (16 x 8 NT, rounded to T) times NT * 8 rows of tile b.  SPLIT: what the rounding takes from P
-// is multiplied as well, so that the products are those of some twice as many bits.
+// is multiplied as well, so that the products are those of some twice as many bits; P then holds gradients
+// of scores, otherwise (lifted) probabilities.
 template <typename T, int DP, int NT, bool SPLIT = false>
 __device__ __forceinline__ void product_probabilities(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b) {
   auto rest = [](float x) {
@@ -266,7 +282,8 @@ __device__ __forceinline__ void product_probabilities(float (&acc)[DP / 8][4], c
 #pragma unroll
   for (int k = 0; k < NT / 2; ++k) {
     const float (&x)[4] = p[2 * k], (&y)[4] = p[2 * k + 1];
-    const uint32_t fa[4] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+    auto pack = [](float lo, float hi) { return SPLIT ? pack2<T>(lo, hi) : pack_lifted<T>(lo, hi); };
+    const uint32_t fa[4] = {pack(x[0], x[1]), pack(x[2], x[3]), pack(y[0], y[1]), pack(y[2], y[3])};
     uint32_t fr[4];
     if constexpr (SPLIT) {
       fr[0] = pack2<T>(rest(x[0]), rest(x[1]));

@@ -6,7 +6,7 @@
 // passes over tiles that none of its 16 rows see, which is what keeps a tile of many short segments
 // cheap, and over the mask where all of its rows see the whole tile.  Probabilities are rounded to the
 // type of the values before the second product, which the matrix instructions require: half a step
-// of that type each (2^-8 for bf16), averaged over the keys.
+// of that type each (2^-8 for bf16, 2^-11 for fp16), averaged over the keys.
 // Bound: instruction issue (masks and exponentials; for heads of 16 columns there are eight multiply-adds to each).
 // Measured: 20 000 rows, 8 heads of 16, segments up to 128: 30 us, issue slots 58 % busy.
 #pragma once
@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
   const int all_begin = tail.begin, all_end = pos0 + row0 + 15 <= last ? keys_of(a, pos0 + row0).end : 0;
   const float slope = MODE != kPlain ? slope_of(a, head) : 0.f;
 
+  constexpr float kLift = kLifted<T, 15>;  // no probability is above 1
   float out[DP / 8][4] = {};
   float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
   int stage = 0;
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
       }
       // no visible key so far: subtract 0, so that the weights become 0 and not NaN
       const float base0 = top0_new == -INFINITY ? 0.f : top0_new, base1 = top1_new == -INFINITY ? 0.f : top1_new;
+      const float less0 = base0 - kLift, less1 = base1 - kLift;
       const float shrink0 = exp2_fast(top0 - base0), shrink1 = exp2_fast(top1 - base1);
       top0 = top0_new;
       top1 = top1_new;
@@ -119,8 +121,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[t][e] = exp2_fast(s[t][e] - base0);
-          s[t][2 + e] = exp2_fast(s[t][2 + e] - base1);
+          s[t][e] = exp2_fast(s[t][e] - less0);
+          s[t][2 + e] = exp2_fast(s[t][2 + e] - less1);
           sum0 += s[t][e];
           sum1 += s[t][2 + e];
         }
@@ -145,8 +147,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) forward_kernel(con
   // a row sees itself, so only rows behind the last position have an empty sum
   const bool none0 = see0.end <= see0.begin, none1 = see1.end <= see1.begin;
   if (a.lse && (lane & 3) == 0) {
-    if (i0 < a.n) a.lse[int64_t(head) * a.n + i0] = none0 ? 0.f : top0 + log2f(sum0);
-    if (i1 < a.n) a.lse[int64_t(head) * a.n + i1] = none1 ? 0.f : top1 + log2f(sum1);
+    if (i0 < a.n) a.lse[int64_t(head) * a.n + i0] = none0 ? 0.f : top0 - kLift + log2f(sum0);
+    if (i1 < a.n) a.lse[int64_t(head) * a.n + i1] = none1 ? 0.f : top1 - kLift + log2f(sum1);
   }
   const float factor0 = none0 ? 0.f : 1.f / sum0, factor1 = none1 ? 0.f : 1.f / sum1;
   store_rows<T, DP>(a, a.out, head, pos0 + row0, out, factor0, factor1, smem + M::kQ, row0);

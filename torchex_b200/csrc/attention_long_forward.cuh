@@ -134,6 +134,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t sums = tmem + lanes + M::kOut + w * DP;
     const Bounds see = keys_of(a, i);
+    constexpr float kLift = kLifted<T, 7>;  // the largest probability is 2^kStale
     const float unit = a.unit, slope = MODE != kPlain ? slope_of(a, head) : 0.f;
     float top = -INFINITY;  // in units of log2
     float2 sum = {0.f, 0.f};
@@ -182,7 +183,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
           t5::tmem_store16(sums + c, reinterpret_cast<const uint32_t*>(o));
         }
       }
-      const float less = top == -INFINITY ? 0.f : top;  // a row without a visible key so far: weights 0, not NaN
+      const float less = (top == -INFINITY ? 0.f : top) - kLift;  // a row without a visible key so far: weights 0, not NaN
       const float2 factor = {MODE != kPlain ? 1.f : unit, MODE != kPlain ? 1.f : unit}, shift = {-less, -less};
       float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
@@ -193,7 +194,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
           const float2 x = t5::fma2({s[c + e], s[c + e + 1]}, factor, shift);
           const float2 y = {exp2_fast(x.x), exp2_fast(x.y)};
           part[(e >> 1) & 1] = t5::add2(part[(e >> 1) & 1], y);
-          p[e / 2] = pack2<T>(y.x, y.y);
+          p[e / 2] = pack_lifted<T>(y.x, y.y);
         }
         t5::tmem_store16(scores + c / 2, p);
       }
@@ -208,7 +209,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
       t5::warp_wait(bar(kDone + 2 * w + (last & 1)), (last >> 1) & 1, dead);
       const bool there = i < a.n;
       const float total = sum.x + sum.y, factor = see.end > see.begin ? 1.f / total : 0.f;
-      if (there && a.lse) a.lse[int64_t(head) * a.n + i] = see.end > see.begin ? top + log2f(total) : 0.f;
+      if (there && a.lse) a.lse[int64_t(head) * a.n + i] = see.end > see.begin ? top - kLift + log2f(total) : 0.f;
       T* to = row_at<T>(a, a.out, head, min(i, a.n - 1));
       T* low = a.out_low.p ? row_at<T>(a, a.out_low, head, min(i, a.n - 1)) : nullptr;
 #pragma unroll
