@@ -467,7 +467,8 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
  *   out_i = sum_j softmax_j(x_ij) v_j over the rows j of i's segment, up to i if causal.
  * Query heads share key / value heads in consecutive groups of heads / kv_heads.
  * Scores, softmax statistics and sums are fp32; probabilities and the gradients of
- * scores are rounded to the tensors' type before they are multiplied.  A row that a query
+ * scores are rounded to the tensors' type before they are multiplied, in fp16 after a
+ * power of two has brought them into its range.  A row that a query
  * does not see has no influence on it, whatever it holds (NaN and infinities included).
  * No atomics: bit-reproducible run to run.  Nothing synchronises.
  *   Limits: TEXB_BFLOAT16 or TEXB_FLOAT16; dim a multiple of 8 up to 128; pointers and

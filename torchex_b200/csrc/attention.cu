@@ -94,14 +94,28 @@ __device__ void order_tiles(const Problem& a, const Order& o) {
   for (int t = threadIdx.x; t < o.tiles; t += kThreads) o.order[atomicAdd(&s_count[class_of(t)], 1)] = t;
 }
 
+// Raises a word that holds the bits of a float that is not negative.  The order does not matter: the largest stays.
+__device__ __forceinline__ void raise(float* to, float value) {
+  if (!(value < INFINITY)) return;  // rows that are not finite
+  int* word = reinterpret_cast<int*>(to);
+  if (__float_as_int(value) > *static_cast<volatile int*>(word)) atomicMax(word, __float_as_int(value));
+}
+
+__device__ __forceinline__ float* word_of(const Problem& a, bool keys, int head, int first) {
+  return keys ? a.v_most + int64_t(head) * a.n + first : a.g_most + int64_t(head / (a.heads / a.kv_heads)) * a.n + first;
+}
+
 // The flags of the blocks of the values (forward: BACKWARD false, the CTAs along y are groups of kv heads), or, for
 // the backward pass, delta_i = scale g_i . o_i and the flags of the queries or gradients of each head (the first
-// CTAs along y) and of the keys of each kv head.  Bound by HBM: every row is read once.
+// CTAs along y) and of the keys of each kv head, and for fp16 the sizes of the gradients and values.  Bound by HBM:
+// every row is read once.
 template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads)
 look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_spread, int q_groups, float* __restrict__ delta,
                  uint8_t* __restrict__ bad_q, uint8_t* __restrict__ bad_k, Order queries, Order keys_order) {
+  constexpr bool kSized = BACKWARD && kShortRange<T>;
   __shared__ int s_bad[kThreads];  // by head of the CTA
+  __shared__ float s_square[kSized ? kFlag * kThreads : 1];  // by row, then by head of the CTA
   const int blocks = (a.n + kFlag - 1) / kFlag;
   if (int(blockIdx.x) >= blocks) {  // one or two CTAs more, for the long kernels
     if (blockIdx.y == 0) order_tiles<false>(a, queries);
@@ -114,9 +128,9 @@ look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_sp
   const int first_head = (keys ? blockIdx.y - q_groups : blockIdx.y) * sp.heads, heads = keys ? a.kv_heads : a.heads;
   const int sub = threadIdx.x & (sp.lanes - 1), slot = threadIdx.x / sp.lanes, mine = slot % sp.heads, head = first_head + mine;
   const bool active = slot < sp.heads * sp.rows && head < heads && sub < a.dim / 8;
+  constexpr int kInFlight = 4;  // rows of a thread whose loads are issued together
   s_bad[threadIdx.x] = 0;
   __syncthreads();
-  constexpr int kInFlight = 4;  // rows of a thread whose loads are issued together
   bool bad = false;
   for (int r0 = slot / sp.heads; r0 < kFlag; r0 += sp.rows * kInFlight) {
     uint4 q[kInFlight], g[kInFlight], o[kInFlight], low[kInFlight];
@@ -130,6 +144,7 @@ look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_sp
           return __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(x.p) + row * x.row + head * x.head + sub * 8));
         };
         q[k] = piece(!BACKWARD ? a.v : keys ? a.k : a.q);
+        if (kSized && keys) g[k] = piece(a.v);
         if (!keys) {
           g[k] = piece(a.g);
           o[k] = piece(a.out);
@@ -139,7 +154,22 @@ look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_sp
     }
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
-      bad |= not_finite<T>(q[k]) || not_finite<T>(g[k]);
+      bad |= not_finite<T>(q[k]) || (!keys && not_finite<T>(g[k]));
+      const int pos = pos0 + r0 + k * sp.rows;
+      const bool writes = active && sub == 0 && pos < end && r0 + k * sp.rows < kFlag;
+      if constexpr (kSized) {
+        float square = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = widen<T>(reinterpret_cast<const Chunk<T, 16>&>(g[k]).v[e]);
+          square = fmaf(x, x, square);
+        }
+        for (int x = sp.lanes / 2; x > 0; x >>= 1) square += __shfl_xor_sync(0xffffffffu, square, x);
+        if (writes) {
+          s_square[(pos - pos0) * sp.heads + mine] = square;
+          if (!keys) a.g_size[int64_t(head) * a.n + pos] = square;
+        }
+      }
       if (keys) continue;
       // out itself is rounded: without the rest, delta's error would reach every dS of the row
       float sum = 0.f;
@@ -151,14 +181,29 @@ look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_sp
         sum = fmaf(widen<T>(gv.v[e]), widen<T>(lv.v[e]), sum);
       }
       for (int x = sp.lanes / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      const int pos = pos0 + r0 + k * sp.rows;
-      if (active && sub == 0 && pos < end && r0 + k * sp.rows < kFlag) delta[int64_t(head) * a.n + pos] = sum * a.scale;
+      if (writes) delta[int64_t(head) * a.n + pos] = sum * a.scale;
     }
   }
   if (bad) s_bad[mine] = 1;
   __syncthreads();
   if (int(threadIdx.x) < sp.heads && first_head + int(threadIdx.x) < heads)
     (keys ? bad_k : bad_q)[int64_t(first_head + threadIdx.x) * blocks + blockIdx.x] = uint8_t(s_bad[threadIdx.x]);
+  if constexpr (kSized) {
+    const int there = min(sp.heads, heads - first_head), first = first_of(a, pos0);
+    if (first == first_of(a, end - 1)) {  // a block within one segment raises each word once
+      if (int(threadIdx.x) < there) {
+        float most = 0.f;
+        for (int r = 0; r < end - pos0; ++r) {
+          const float square = s_square[r * sp.heads + threadIdx.x];
+          if (square < INFINITY) most = fmaxf(most, square);
+        }
+        raise(word_of(a, keys, first_head + threadIdx.x, first), most);
+      }
+    } else {
+      for (int i = threadIdx.x; i < (end - pos0) * there; i += kThreads)
+        raise(word_of(a, keys, first_head + i % there, first_of(a, pos0 + i / there)), s_square[i / there * sp.heads + i % there]);
+    }
+  }
 }
 
 int check(const Problem& a, int dtype, bool backward) {
@@ -228,7 +273,7 @@ namespace attention {
 namespace {
 struct Workspace {
   uint8_t *flags, *flags_q;  // of values, or keys; of queries and gradients
-  float* delta;
+  float *delta, *g_size, *most;  // most: of the values, then of the gradients
   Order queries, keys;
   size_t bytes;
 };
@@ -250,6 +295,8 @@ Workspace carve(void* ws, int64_t n, int heads, int kv_heads, bool backward) {
     w.keys = order(kLongTile);
     w.flags_q = static_cast<uint8_t*>(take(blocks_of(n) * size_t(heads)));
     w.delta = static_cast<float*>(take(size_t(n) * size_t(heads) * sizeof(float)));
+    w.g_size = static_cast<float*>(take(size_t(n) * size_t(heads) * sizeof(float)));
+    w.most = static_cast<float*>(take(2 * size_t(n) * size_t(kv_heads) * sizeof(float)));
   }
   w.bytes = at + 256;
   return w;
@@ -361,6 +408,13 @@ int attention_backward_impl(const texb_attention_problem* t, void* workspace, si
   a.bad_k = w.flags;
   a.query_order = w.queries.order;
   a.key_order = w.keys.order;
+  a.g_size = w.g_size;
+  a.v_most = w.most;
+  a.g_most = w.most + int64_t(a.n) * a.kv_heads;
+  if (dtype == TEXB_FLOAT16) {
+    const cudaError_t e = cudaMemsetAsync(w.most, 0, 2 * size_t(a.n) * size_t(a.kv_heads) * sizeof(float), stream);
+    if (e != cudaSuccess) return fail(TEXB_ERR_CUDA, "segment_attention: %s", cudaGetErrorString(e));
+  }
   const Spread qs = spread_of(a.dim, a.heads), ks = spread_of(a.dim, a.kv_heads);
   const int q_groups = int(ceil_div(a.heads, qs.heads));  // and at least one group of kv heads: two CTAs along y
   const dim3 grid(unsigned(blocks_of(a.n)) + (long_segments(a) ? 1u : 0u), unsigned(q_groups + ceil_div(a.kv_heads, ks.heads)));

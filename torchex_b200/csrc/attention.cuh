@@ -50,6 +50,9 @@ struct Problem {
   View g;                    // gradient of out
   const float* delta;        // [heads, n] by position: scale * g_i . o_i
   View gq, gk, gv;
+  // fp16 only, squares of norms: of each row of g, [heads, n]; of the largest finite row of v, and of g (of all heads that
+  // share the kv head), of each segment, [kv_heads, n] at the segment's first position
+  float *g_size, *v_most, *g_most;
   // flags of blocks with a value that is not finite, [.., ceil(n / kFlag)]; NULL: look for oneself
   const uint8_t *bad_v, *bad_k;  // per kv head
   const uint8_t* bad_q;          // per head: in q or g
@@ -76,6 +79,7 @@ __device__ __forceinline__ Bounds segment_of(const Problem& a, int pos) {
   const int begin = max(0, __ldg(a.offsets + s));
   return {begin, max(begin, min(a.n, __ldg(a.offsets + s + 1)))};
 }
+__device__ __forceinline__ int first_of(const Problem& a, int pos) { return min(segment_of(a, pos).begin, a.n - 1); }
 // Bounded waits of the kernels for long segments that gave up (part of texb_device_status).
 static __device__ int g_wait_timeouts = 0;
 
@@ -170,6 +174,27 @@ template <typename T> __device__ __forceinline__ uint32_t pack_lifted(float lo, 
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
   return v;
 }
+
+// Gradients of scores are lifted in fp16 as well, by the largest power of two, from 1 to 2^100, that keeps what bounds
+// them below 2^15: |dS| = P |scale (g v - g o)| <= 2 |scale| |g| |v|, v the largest row of the segment.  They are as
+// small as the gradients, which is about g over the length of the segment: for g of 2^-10 and 2048 rows the unlifted
+// ones were off by 2 %.  A row has one factor for all that is added up for it, and its sum is divided by it.
+__device__ __forceinline__ int gradient_lift(const Problem& a, float g_square, float v_square) {
+  const float bound = 2.f * fabsf(a.scale) * sqrtf(g_square) * sqrtf(v_square);
+  return min(100, max(0, 14 - (int(__float_as_uint(bound) >> 23) - 127)));
+}
+// of a row of queries and of a row of keys
+__device__ __forceinline__ int query_lift(const Problem& a, int head, int kv, int pos) {
+  if (pos >= a.n) return 0;
+  return gradient_lift(a, a.g_size[int64_t(head) * a.n + pos], a.v_most[int64_t(kv) * a.n + first_of(a, pos)]);
+}
+__device__ __forceinline__ int key_lift(const Problem& a, int kv, int pos) {
+  if (pos >= a.n) return 0;
+  const int64_t at = int64_t(kv) * a.n + first_of(a, pos);
+  return gradient_lift(a, a.g_most[at], a.v_most[at]);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
+constexpr int kGradientWeights = 15;  // lift of the probabilities of the backward pass: none is above 1
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {

@@ -9,6 +9,7 @@
 // P is rounded to the inputs' type before its product (half a step); dS goes in as two such values, which costs
 // little here and halves the squared error of gq and gk:
 //   dS = P (scale g v - delta) x (derivative of the capped score), delta = scale g o,  gq = dS k, gk = dS^T q, gv = P^T g.
+// In fp16 both are lifted first (attention.cuh), so that values far below its smallest normal number keep their bits.
 // A masked pair's dS is set to 0, not multiplied by 0: its g v may be infinite.
 // Bound as the forward kernel.  Measured: 20 000 rows, 8 heads of 16, segments up to 128: 31 us for the queries, 42
 // for the keys and values.
@@ -66,7 +67,13 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) query_gradient_ker
   const float slope = MODE != kPlain ? slope_of(a, head) : 0.f;
   const int64_t place = int64_t(head) * a.n;
   const float lse0 = i0 < a.n ? a.lse[place + i0] : 0.f, lse1 = i1 < a.n ? a.lse[place + i1] : 0.f;
-  const float delta0 = i0 < a.n ? a.delta[place + i0] : 0.f, delta1 = i1 < a.n ? a.delta[place + i1] : 0.f;
+  int lift0 = 0, lift1 = 0;
+  if constexpr (kShortRange<T>) {
+    lift0 = query_lift(a, head, kv, i0);
+    lift1 = query_lift(a, head, kv, i1);
+  }
+  const float up0 = power_of_two(lift0), up1 = power_of_two(lift1), scale0 = a.scale * up0, scale1 = a.scale * up1;
+  const float delta0 = i0 < a.n ? a.delta[place + i0] * up0 : 0.f, delta1 = i1 < a.n ? a.delta[place + i1] * up1 : 0.f;
 
   float gq[DP / 8][4] = {};
   int stage = 0;
@@ -91,8 +98,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) query_gradient_ker
         for (int e = 0; e < 2; ++e) {
           const int j = j0 + t * 8 + (lane & 3) * 2 + e;
           const Score x0 = score_of<MODE>(a, s[t][e], slope, float(i0 - j)), x1 = score_of<MODE>(a, s[t][2 + e], slope, float(i1 - j));
-          const float d0 = exp2_fast(x0.x - lse0) * fmaf(dp[t][e], a.scale, -delta0) * x0.slope;
-          const float d1 = exp2_fast(x1.x - lse1) * fmaf(dp[t][2 + e], a.scale, -delta1) * x1.slope;
+          const float d0 = exp2_fast(x0.x - lse0) * fmaf(dp[t][e], scale0, -delta0) * x0.slope;
+          const float d1 = exp2_fast(x1.x - lse1) * fmaf(dp[t][2 + e], scale1, -delta1) * x1.slope;
           dp[t][e] = see0.holds(j) ? d0 : 0.f;
           dp[t][2 + e] = see1.holds(j) ? d1 : 0.f;
         }
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 6 : 1) query_gradient_ker
   }
   wait_copies<0>();
   __syncwarp();
-  store_rows<T, DP>(a, a.gq, head, pos0 + row0, gq, 1.f, 1.f, smem + M::kQ, row0);
+  store_rows<T, DP>(a, a.gq, head, pos0 + row0, gq, power_of_two(-lift0), power_of_two(-lift1), smem + M::kQ, row0);
 }
 
 // Queries per step of the key kernel: 32 for the widest rows, whose two accumulators of 64 registers
@@ -181,6 +188,15 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
   const int warp_begin = pos0 + row0 <= last ? queries_of(a, pos0 + row0).begin : INT_MAX;
   const int warp_end = pos0 + row0 <= last ? queries_of(a, min(last, pos0 + row0 + 15)).end : 0;
 
+  constexpr float kLift = kLifted<T, kGradientWeights>;
+  int lift0 = 0, lift1 = 0;
+  float up0 = 1.f, up1 = 1.f;  // of the gradients of scores, whose probabilities are lifted already
+  if constexpr (kShortRange<T>) {
+    lift0 = key_lift(a, kv, j0);
+    lift1 = key_lift(a, kv, j1);
+    up0 = power_of_two(lift0 - kGradientWeights);
+    up1 = power_of_two(lift1 - kGradientWeights);
+  }
   float gk[DP / 8][4] = {}, gv[DP / 8][4] = {};
   int stage = 0, head = kv * group, step = 0;
   for (int it = 0; it < total; ++it) {
@@ -204,13 +220,13 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = t * 8 + (lane & 3) * 2 + e, i = q0 + r;
-          const float lse = s_lse[stage * R + r], delta = s_delta[stage * R + r];
+          const float lse = s_lse[stage * R + r] - kLift, delta = s_delta[stage * R + r];
           const Score x0 = score_of<MODE>(a, p[t][e], slope, float(i - j0)), x1 = score_of<MODE>(a, p[t][2 + e], slope, float(i - j1));
           const bool on0 = seen0.holds(i), on1 = seen1.holds(i);
           p[t][e] = on0 ? exp2_fast(x0.x - lse) : 0.f;
           p[t][2 + e] = on1 ? exp2_fast(x1.x - lse) : 0.f;
-          ds[t][e] = on0 ? p[t][e] * fmaf(ds[t][e], a.scale, -delta) * x0.slope : 0.f;
-          ds[t][2 + e] = on1 ? p[t][2 + e] * fmaf(ds[t][2 + e], a.scale, -delta) * x1.slope : 0.f;
+          ds[t][e] = on0 ? p[t][e] * fmaf(ds[t][e], a.scale, -delta) * x0.slope * up0 : 0.f;
+          ds[t][2 + e] = on1 ? p[t][2 + e] * fmaf(ds[t][2 + e], a.scale, -delta) * x1.slope * up1 : 0.f;
         }
       }
       product_probabilities<T, DP, NT>(gv, p, tg);
@@ -224,8 +240,9 @@ __global__ void __launch_bounds__(kThreads, DP <= 32 ? 4 : 1) key_gradients_kern
   }
   wait_copies<0>();
   __syncthreads();  // the key tiles are written over below, by warps that read only their own rows of them
-  store_rows<T, DP>(a, a.gk, kv, pos0 + row0, gk, 1.f, 1.f, smem + M::kK, row0);
-  store_rows<T, DP>(a, a.gv, kv, pos0 + row0, gv, 1.f, 1.f, smem + M::kV, row0);
+  constexpr float kUnlift = kShortRange<T> ? 1.f / (1 << kGradientWeights) : 1.f;
+  store_rows<T, DP>(a, a.gk, kv, pos0 + row0, gk, power_of_two(-lift0), power_of_two(-lift1), smem + M::kK, row0);
+  store_rows<T, DP>(a, a.gv, kv, pos0 + row0, gv, kUnlift, kUnlift, smem + M::kV, row0);
 }
 
 template <typename K>

@@ -42,7 +42,8 @@ __device__ __forceinline__ void copy_long_tile(const Problem& a, const View& x, 
   }
 }
 
-// Writes columns c0 .. c0 + COLUMNS - 1 of a warp's 32 rows of sums (tensor memory) to rows of a tensor: through
+// Writes columns c0 .. c0 + COLUMNS - 1 of a warp's 32 rows of sums (tensor memory), for fp16 times `factor`, each row
+// (lane) its own, to rows of a tensor: through
 // `rows`, 32 * COLUMNS * 2 bytes of shared memory that nothing else uses any more, so that a row is written by
 // neighbouring lanes.  One row per lane, 16 bytes at a time, touches 32 half sectors per store: the gradients of 8192
 // positions, 16 heads of 128 columns, up to 2048 keys take 343.5 us with the forward pass this way and 350 that way.
@@ -50,7 +51,7 @@ __device__ __forceinline__ void copy_long_tile(const Problem& a, const View& x, 
 // 32768 positions, 8 heads of 128 columns, up to 4096 keys).
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void store_sums(const Problem& a, const View& x, int head, int pos0, uint32_t sums, int c0,
-                                           unsigned char* rows) {
+                                           float factor, unsigned char* rows) {
   constexpr int kPieces = COLUMNS / 8, kMask = kPieces < 8 ? kPieces - 1 : 7;
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -58,6 +59,10 @@ __device__ __forceinline__ void store_sums(const Problem& a, const View& x, int 
     float o[32];
     t5::tmem_load32(sums + c0 + c, o);
     t5::tmem_wait_loads();
+    if constexpr (kShortRange<T>) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] *= factor;
+    }
 #pragma unroll
     for (int e = 0; e < 32; e += 8) {
       const uint4 piece = {pack2<T>(o[e], o[e + 1]), pack2<T>(o[e + 2], o[e + 3]),

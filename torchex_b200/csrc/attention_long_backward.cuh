@@ -9,12 +9,14 @@
 //   S = own1 stream1^T,  G = own2 stream2^T,  P = exp(S - lse),  dS = P (G - delta) scale slope,
 //   queries: g_q += dS K;   keys: g_v += P^T g, g_k += dS^T Q   (S and G transposed: rows are keys),
 // all in tensor memory: two buffers of 64 + 64 columns for S and G, over which P and dS are written in 16 bits, and
-// the sums.  Two warpgroups take the tiles in turn, one row per thread; warps 8 to 11 copy rows, one thread of warp
-// 12 issues all products, those of one buffer while the other one's exponentials are taken.
+// the sums.  In fp16 both are lifted by powers of two first (attention.cuh).  Two warpgroups take the tiles in turn,
+// one row per thread; warps 8 to 11 copy rows, one thread of warp 12 issues all products, those of one buffer while the
+// other one's exponentials are taken.
 // Bound: matrix products.  A tile of 64 takes 390 cycles for each of S and G (an operand of 64 rows runs at three
 // quarters of the rate of one of 128, for which tensor memory has no room) and 262 for each sum.
 // Measured with cold caches: 8192 rows, 16 heads that share 4, of 128 columns, up to 2048 keys, causal, 118 us for the
-// queries and 120 for the keys and values; the tensor pipe is 36 and 52 % busy over the launch.
+// queries and 120 for the keys and values; the tensor pipe is 36 and 52 % busy over the launch.  With warm caches
+// 104 and 105 in bf16, 106 and 109 in fp16, whose lifted gradients take a product more in the keys' form.
 #pragma once
 
 #include "attention_long.cuh"
@@ -137,7 +139,17 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
       row_lse = a.lse[int64_t(own_head) * a.n + pos];
       row_delta = a.delta[int64_t(own_head) * a.n + pos];
     }
-    const float2 unit = {a.unit, a.unit}, scale = {a.scale, a.scale};
+    // fp16: the row's factors.  The probabilities of the keys' form are lifted, and so are the gradients that they enter.
+    constexpr float kLift = KEYS ? kLifted<T, kGradientWeights> : 0.f;
+    int lift = 0;
+    float2 up = {1.f, 1.f};
+    if constexpr (kShortRange<T>) {
+      lift = KEYS ? key_lift(a, kv, pos) : query_lift(a, own_head, kv, pos);
+      up.x = up.y = power_of_two(lift - (KEYS ? kGradientWeights : 0));
+      if (!KEYS) row_delta *= up.x;
+    }
+    const float own_scale = KEYS ? a.scale : a.scale * up.x;
+    const float2 unit = {a.unit, a.unit}, scale = {own_scale, own_scale};
     int step = buffer, head = 0;  // of tile u = buffer, buffer + 2, ...
     while (step >= steps) {
       step -= steps;
@@ -177,20 +189,21 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
             if constexpr (MODE != kPlain) {
               const float away = float(pos - p0) - float(c + k);
               const Score x0 = score_of<MODE>(a, s[k], slope, away), x1 = score_of<MODE>(a, s[k + 1], slope, away - 1.f);
-              x = {x0.x - l.x, x1.x - l.y};
+              x = {x0.x - (l.x - kLift), x1.x - (l.y - kLift)};
               bend = {x0.slope, x1.slope};
             } else {
-              x = t5::fma2({s[k], s[k + 1]}, unit, {-l.x, -l.y});
+              x = t5::fma2({s[k], s[k + 1]}, unit, kLift > 0.f ? float2{kLift - l.x, kLift - l.y} : float2{-l.x, -l.y});
             }
             float2 p = {exp2_fast(x.x), exp2_fast(x.y)};
             float2 ds = t5::mul2(p, t5::fma2({g[k], g[k + 1]}, scale, {-d.x, -d.y}));
             if constexpr (MODE != kPlain) ds = t5::mul2(ds, bend);
+            if constexpr (KEYS && kShortRange<T>) ds = t5::mul2(ds, up);
             if (!whole) {  // set, not multiplied: a masked pair's product may be infinite
               const bool on0 = unsigned(c + k) - from < count, on1 = unsigned(c + k + 1) - from < count;
               p = {on0 ? p.x : 0.f, on1 ? p.y : 0.f};
               ds = {on0 ? ds.x : 0.f, on1 ? ds.y : 0.f};
             }
-            if (KEYS) p16[k / 2] = pack2<T>(p.x, p.y);
+            if (KEYS) p16[k / 2] = pack_lifted<T>(p.x, p.y);
             d16[k / 2] = pack2<T>(ds.x, ds.y);
           }
         }
@@ -213,7 +226,7 @@ long_backward_kernel(const __grid_constant__ Problem a, const __grid_constant__ 
     unsigned char* rows = smem + (buffer ? M::kOwn2 : M::kOwn1) + (warp & 3) * (32 * kWritten * 2);
     const View& view = !KEYS ? a.gq : buffer ? a.gv : a.gk;
     store_sums<T, kWritten>(a, view, own_head, pos0 + (warp & 3) * 32, tmem + lanes + M::kSums + (KEYS ? buffer * DP : 0),
-                            KEYS ? 0 : buffer * kWritten, rows);
+                            KEYS ? 0 : buffer * kWritten, power_of_two(KEYS && buffer ? -kGradientWeights : -lift), rows);
   } else if (warp < 12) {  // ---- copies
     const View &own1 = KEYS ? a.k : a.q, &own2 = KEYS ? a.v : a.g, &stream1 = KEYS ? a.q : a.k, &stream2 = KEYS ? a.g : a.v;
     if (maps.used) {

@@ -26,7 +26,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, data, s
     by ``slopes[head] * distance``, the distance counted in rows of the segment.
 
     Differentiable once, by q, k and v.  Statistics and sums are fp32; probabilities and
-    gradients of scores are rounded to the dtype of q before they are multiplied.  Results are
+    gradients of scores are rounded to the dtype of q before they are multiplied (float16: after a
+    power of two has brought them into its range, so that small gradients keep their bits).  Results are
     bit-reproducible, and independent of rows that a query does not see, whatever those hold."""
     if data._pending is not None:
         data._poll()
