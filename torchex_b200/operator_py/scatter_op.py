@@ -119,13 +119,15 @@ class ScatterData:
     def _poll(self, wait: bool = False) -> None:
         """Takes over the plan statistics once their copy to the host has finished
         (``wait``: block until it has).  From then on the host also knows that the plan
-        arrays are complete, which lets the reduce kernels read them early."""
+        arrays are complete, which lets the reduce kernels read them early.  While a stream
+        is captured the event must not be asked (that would end the capture), so the
+        statistics stay unknown to the captured calls."""
         if self._pending is None:
             return
         host, done = self._pending
         if wait:
             done.synchronize()
-        elif not done.query():
+        elif torch.cuda.is_current_stream_capturing() or not done.query():
             return
         max_cnt, num_empty, _bad, _ = host.tolist()
         self._pending = None
