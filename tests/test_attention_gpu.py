@@ -388,3 +388,18 @@ def test_strides_of_axes_of_one(n, heads):
 
     for a, b in zip(_step(odd(q), odd(k), odd(v), odd(g), data), want):
         assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused_for_slopes_and_gradients():
+    import torch.autograd.forward_ad as fwd
+
+    ids, data = _plan([4, 6], False)
+    q = torch.zeros(10, 4, 16, device=DEV, dtype=torch.bfloat16)
+    x = q.clone().requires_grad_(True)
+    out = segment_attention(x, q, q, data)
+    slopes = torch.zeros(4, device=DEV)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            segment_attention(q, q, q, data, slopes=fwd.make_dual(slopes, torch.ones_like(slopes)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, x, fwd.make_dual(q, torch.ones_like(q)))

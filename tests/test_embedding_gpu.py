@@ -232,3 +232,14 @@ def test_forward_mode_is_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             embedding(tok, fwd.make_dual(w.clone().requires_grad_(True), torch.ones_like(w)))
         assert embedding(tok, w).shape == (2, 4)
+
+
+def test_forward_mode_through_the_gradient_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    w, tok = torch.randn(9, 4, device=DEV, requires_grad=True), torch.tensor([1, 2], device=DEV)
+    out = embedding(tok, w)
+    with fwd.dual_level():
+        g = fwd.make_dual(torch.ones(2, 4, device=DEV), torch.ones(2, 4, device=DEV))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, w, g)

@@ -56,3 +56,14 @@ def test_operators_reject_bad_arguments():
         with pytest.raises(ValueError, match="max_norm"):
             clip_grads([x], bad)
     assert clip_grad_norm_([torch.nn.Parameter(x)], 1.0).item() == 0.0  # no gradient anywhere
+
+
+def test_forward_mode_is_refused():
+    """A norm or a clipped tensor without its derivative would be taken for a constant."""
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level():
+        dual = fwd.make_dual(torch.ones(3), torch.ones(3))
+        for call in (lambda: grad_norm([dual]), lambda: clip_grads([dual], 1.0), lambda: clip_grads([dual], 1.0, out=[torch.ones(3)])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

@@ -223,3 +223,16 @@ def test_tensors_that_require_a_gradient():
     assert p.grad.requires_grad
     assert clip_grad_norm_(p, 8.0).item() == 16.0
     assert torch.allclose(p.grad, torch.full_like(x, 2.0))
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level():
+        x, y = torch.ones(3, device=DEV), torch.empty(3, device=DEV)
+        dual = fwd.make_dual(torch.ones(3, device=DEV), torch.ones(3, device=DEV))
+        for call in (lambda: grad_norm([x, dual]), lambda: clip_grads([dual], 1.0), lambda: clip_grads([x, dual], 1.0, out=[y, x]),
+                     lambda: clip_grads([x], 1.0, out=[dual])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert float(grad_norm([x])) == pytest.approx(3 ** 0.5)

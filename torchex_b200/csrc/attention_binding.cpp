@@ -107,6 +107,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "segment_attention is differentiable once (create_graph is not supported)");
+    check_no_tangent(grads[0], "the gradient");
     const auto s = ctx->get_saved_variables();
     const Options o = {ctx->saved_data["scale"].toDouble(), ctx->saved_data["softcap"].toDouble(), ctx->saved_data["causal"].toBool(),
                        ctx->saved_data["num_segments"].toInt(), ctx->saved_data["max_count"].toInt()};
@@ -161,6 +162,7 @@ at::Tensor segment_attention(const Plan& plan, const at::Tensor& q, const at::Te
     TORCH_CHECK(slopes_given->device() == q.device(), "slopes and q live on different devices");
     TORCH_CHECK(!slopes_given->requires_grad() || !at::GradMode::is_enabled(), "slopes take no gradient: pass slopes.detach()");
     TEXB_CHECK_DTYPE((*slopes_given), at::kFloat);
+    check_no_tangent(*slopes_given, "slopes");
     slopes = slopes_given->contiguous();
   }
   const Options o = {scale, softcap, causal, plan.num_segments, plan.max_cnt};

@@ -60,6 +60,7 @@ at::Tensor embedding_backward(const at::Tensor& tokens_in, const at::Tensor& g_i
   TORCH_CHECK(g_in.device() == tokens.device(), "tokens and the gradient live on different devices");
   TORCH_CHECK(g_in.dim() == tokens.dim() + 1 && g_in.sizes().slice(0, tokens.dim()) == tokens.sizes(),
               "the gradient must have the shape of tokens and one more axis");
+  check_no_tangent(g_in, "the gradient");
   const int dtype = dtype_code(g_in, "the gradient");
   const c10::cuda::CUDAGuard guard(tokens.device());
   const at::Tensor g = g_in.contiguous();
@@ -126,6 +127,7 @@ struct Tensors {  // the host arrays of the C ABI
 Tensors gather(const std::vector<at::Tensor>& grads) {
   Tensors r;
   for (const at::Tensor& g : grads) {
+    check_no_tangent(g, "a gradient");
     TORCH_CHECK(g.layout() == at::kStrided, "gradients must be dense tensors, got a sparse one");
     TORCH_CHECK(g.device().is_cuda(), "gradients must be CUDAtensors ");
     TORCH_CHECK(g.device() == grads[0].device(), "gradients live on different devices");
@@ -193,6 +195,7 @@ std::tuple<std::vector<at::Tensor>, at::Tensor> clip_grads(const std::vector<at:
     TORCH_CHECK(outs.size() == grads.size(), "out has ", outs.size(), " tensors for ", grads.size(), " gradients");
     for (size_t i = 0; i < outs.size(); ++i) {
       const at::Tensor &o = outs[i], &g = grads[i];
+      check_no_tangent(o, "an output");
       TORCH_CHECK(o.device() == g.device(), "out[", i, "] lives on another device than its gradient");
       TORCH_CHECK(o.sizes() == g.sizes(), "out[", i, "] has another shape than its gradient");
       TORCH_CHECK(o.layout() == at::kStrided && ((o.is_contiguous() && g.is_contiguous()) || o.strides() == g.strides()),
