@@ -647,7 +647,7 @@ int resident_clusters(K kernel, const cudaLaunchConfig_t& cfg, int ranks, int it
   }
   // the largest shared memory that any shape asks for: the attribute stays with the kernel
   constexpr int kMost = SortLayout::kItems + kSortThreads * kMaxItems * int(sizeof(uint2));
-  static_assert(kMost >= kMarkBits / 8 + 8, "the marks fit as well");
+  static_assert(kMost >= kMarkBits / 8, "the marks fit as well");
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return 0;
   int count = 0;
   if (cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess || count < 2) {
@@ -670,9 +670,10 @@ int launch_sort_and_clear(const IdT* tokens, int64_t n, int64_t vocab, int64_t p
   const int passes = n > 1 ? int(ceil_div(bits, kMaxDigitBits)) : 0;
   const int digit_bits = passes ? int(ceil_div(bits, passes)) : 1;
   const int lanes = lanes_of(row_words);
+  // for the items of a sorting CTA or the marks of a clearing one, whatever the table: the number of clusters that fit is
+  // remembered by ranks and items
   size_t smem = SortLayout::kItems + size_t(kSortThreads) * items * sizeof(uint2);
-  const size_t marks = size_t((vocab < kMarkBits ? vocab : kMarkBits) / 8 + 8);
-  if (smem < marks) smem = marks;
+  if (smem < size_t(kMarkBits / 8)) smem = size_t(kMarkBits / 8);
   cudaError_t e = cudaSuccess;
   auto kernel = sort_and_clear_kernel<IdT, W>;
   cudaLaunchConfig_t cfg = {};
