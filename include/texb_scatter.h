@@ -473,8 +473,9 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
  * No atomics: bit-reproducible run to run.  Nothing synchronises.
  *   Limits: TEXB_BFLOAT16 or TEXB_FLOAT16; dim a multiple of 8 up to 128; pointers and
  *   strides (in values) such that rows start on 16-byte boundaries; heads a multiple of
- *   kv_heads; n < 2^31 - 65536; softcap 0, or at least 2^-126 and such that
- *   2 scale / softcap and softcap, each times log2(e), are finite in fp32. */
+ *   kv_heads; n < 2^31 - 65536; softcap 0 and scale times log2(e) finite in fp32, or
+ *   softcap at least 2^-126 and such that 2 scale / softcap and softcap, each times
+ *   log2(e), are. */
 typedef struct texb_attention_problem {
   const void *q, *k, *v;           /* [n, heads, dim], [n, kv_heads, dim] twice */
   int64_t q_strides[2], k_strides[2], v_strides[2]; /* values from row to row, from head to head */

@@ -65,3 +65,13 @@ def test_c_abi_rejects_caps_out_of_range():
         assert lib.texb_attention_forward(_problem(**changes), 4096, need, None) == 2, changes
         assert lib.texb_attention_backward(_problem(**changes), 4096, need, None) == 2, changes
         assert "softcap" in _native.last_error()
+
+
+def test_c_abi_rejects_scales_out_of_range():
+    """A scale whose factor in units of log2 leaves fp32 would turn scores of 0 into NaN."""
+    lib = _native.lib()
+    need = lib.texb_attention_workspace_bytes(10, 4, 2, 1)
+    for scale in (3e38, -3e38):
+        for call in (lib.texb_attention_forward, lib.texb_attention_backward):
+            assert call(_problem(scale=scale), 4096, need, None) == 2
+            assert "scale" in _native.last_error()

@@ -219,6 +219,8 @@ int check(const Problem& a, int dtype, bool backward) {
   if (!(a.cap >= 0.f && a.cap < INFINITY) || !(fabsf(a.scale) < INFINITY))
     return fail(TEXB_ERR_INVALID_ARGUMENT, "segment_attention: bad scale or softcap");
   // 0 times an infinite factor would be NaN, not a score of 0
+  if (a.cap == 0.f && !(fabsf(a.unit) < INFINITY))
+    return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: scale %g is out of range", a.scale);
   if (a.cap > 0.f && !(a.cap >= FLT_MIN && fabsf(a.bend_in) < INFINITY && a.bend_out < INFINITY))
     return fail(TEXB_ERR_UNSUPPORTED, "segment_attention: softcap %g is out of range for scale %g", a.cap, a.scale);
   if (a.n == 0) return TEXB_OK;
