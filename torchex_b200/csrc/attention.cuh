@@ -205,7 +205,7 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// 16 bytes to shared memory; `bytes` 0 writes zeros and reads nothing
+// 4 or 16 bytes to shared memory; `bytes` 0 writes zeros and reads nothing
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }

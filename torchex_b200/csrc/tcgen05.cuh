@@ -211,8 +211,5 @@ __device__ __forceinline__ void settle(uint32_t bar, bool issuer, int* counter) 
   atomicAdd(counter, 1);
 }
 
-template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 }  // namespace t5
 }  // namespace texb
