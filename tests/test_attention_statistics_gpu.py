@@ -17,7 +17,7 @@ def _forget(data):
 
 
 LENS = {"half tiles": [32 + 7 * i % 33 for i in range(40)], "tiles": [64] * 9, "short": [1 + 11 * i % 64 for i in range(50)],
-        "one": [50], "longer": [40, 65, 300]}
+        "one": [50], "longer": [40, 65, 300], "many": [32 + 7 * i % 33 for i in range(300)]}
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -241,8 +241,8 @@ int check(const Problem& a, int dtype, bool backward) {
 inline size_t blocks_of(int64_t n) { return size_t(ceil_div(n, kFlag)); }  // of flags
 
 // Segments short enough that a tile looks at the values of its keys itself instead of a pass of its own
-// doing it: at most three tiles of keys.  Either way the same blocks of positions decide, and the kernels are chosen by
-// `long_segments` alone: whether the host knows the longest segment yet does not show in the results.
+// doing it: at most three tiles of keys.  Either way the same blocks of positions decide, and the kernels are chosen
+// without it: whether the host knows the longest segment yet does not show in the results.
 constexpr int kShortSegment = 64;
 
 // Whether the 5th-generation tensor cores' kernels are used: where segments are long enough, on average, for tiles of
@@ -253,6 +253,14 @@ constexpr int kShortSegment = 64;
 inline bool long_segments(const Problem& a) {
   const int64_t average = a.dim <= 16 ? 768 : a.dim <= 32 ? 256 : 32;
   return a.n >= a.segments * average;
+}
+
+// The forward pass of short segments that do not fill the GPU is latency: tiles of 64 rows start sooner and are more.
+// Measured on segments of 32 to 64 rows (48 on average), general / long kernels in us, by rows times heads: dim 64, 1100:
+// 13 / 17, 3800: 15 / 25, 15 400: 17 / 27, 30 700: 27 / 27, 61 000: 46 / 44; dim 128, 1100: 17 / 21, 3800: 23 / 27,
+// 15 400: 27 / 31, 30 700: 44 / 31.
+inline bool long_forward(const Problem& a) {
+  return long_segments(a) && (a.n > a.segments * int64_t(64) || int64_t(a.n) * a.heads >= 24576);
 }
 
 }  // namespace
@@ -369,7 +377,7 @@ int attention_forward_impl(const texb_attention_problem* t, void* workspace, siz
   st = check(a, dtype, false);
   if (st != TEXB_OK || a.n == 0) return st;
   a.bad_v = nullptr;
-  const bool use_long = long_segments(a);
+  const bool use_long = long_forward(a);
   if (use_long || t->max_count < 0 || t->max_count > kShortSegment) {
     const Workspace w = carve(workspace, a.n, a.heads, a.kv_heads, false);
     if (!workspace || workspace_bytes < w.bytes)
