@@ -424,7 +424,8 @@ int texb_scatter_mean_max_backward(const float* g_mean, const float* g_max,
  *                No floating-point atomics: bit-reproducible run to run.
  * A token outside [0, vocab) reads nothing: its output row is 0, it takes no part
  * in the gradient, and it is counted (texb_device_status, bad_indices).
- * Limits: n and vocab < 2^31 - 65536. */
+ * Limits: n and vocab < 2^31 - 65536.  The workspace is sized for fp32 rows,
+ * whatever the dtype. */
 #define TEXB_FLOAT32 0
 #define TEXB_BFLOAT16 1
 #define TEXB_FLOAT16 2
@@ -469,7 +470,9 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
  * Scores, softmax statistics and sums are fp32; probabilities and the gradients of
  * scores are rounded to the tensors' type before they are multiplied, in fp16 after a
  * power of two has brought them into its range.  A row that a query
- * does not see has no influence on it, whatever it holds (NaN and infinities included).
+ * does not see has no influence on it, whatever it holds (NaN and infinities included);
+ * beside rows that are not finite results may differ in their last bits from what they
+ * are otherwise, and take much longer.
  * No atomics: bit-reproducible run to run.  Nothing synchronises.
  *   Limits: TEXB_BFLOAT16 or TEXB_FLOAT16; dim a multiple of 8 up to 128; pointers and
  *   strides (in values) such that rows start on 16-byte boundaries; heads a multiple of

@@ -249,7 +249,8 @@ constexpr int kShortSegment = 64;
 // 128 rows to be worth it.  Narrow rows are padded to 64 columns there, which takes longer segments to pay.
 // Measured on 16 384 rows, 8 heads, training step, general / long kernels in us: dim 128, average 32: 321 / 258,
 // 64: 383 / 241, 1024: 2543 / 709; dim 64, 32: 215 / 209, 64: 241 / 205; dim 32, 192: 238 / 221 (causal 169 / 189), 512: 449 / 323
-// (280 / 240); dim 16, 512: 311 / 314 (204 / 231), 1024: 562 / 497 (342 / 320).
+// (280 / 240); dim 16, 512: 311 / 314 (204 / 231), 1024: 562 / 497 (342 / 320).  An average does not see a long segment
+// among many short ones: such a batch takes the general kernels for all of its rows.
 inline bool long_segments(const Problem& a) {
   const int64_t average = a.dim <= 16 ? 768 : a.dim <= 32 ? 256 : 32;
   return a.n >= a.segments * average;

@@ -13,7 +13,10 @@
 // instructions add up whole tiles, so a NaN or an infinity in a row that a query must not see would
 // reach its result.  Rows are therefore looked over first (blocks of kFlag positions are flagged), and
 // a tile whose rows meet a flagged block is computed by the plain loops at the end of this file,
-// which touch visible rows only.
+// which touch visible rows only.  They add up in another order, with probabilities in 32 bits, so the rows of such a
+// tile may differ in the last bits from what they are without the flagged row.  They are also slow: 8192 rows of 16
+// heads of 128, segments up to 2048, take 8 (one such row) to 14 ms (all) forward instead of 0.1, and 30 to 35
+// backward instead of 0.3.
 #pragma once
 
 #include <climits>

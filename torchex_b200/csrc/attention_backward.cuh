@@ -12,7 +12,7 @@
 // In fp16 both are lifted first (attention.cuh), so that values far below its smallest normal number keep their bits.
 // A masked pair's dS is set to 0, not multiplied by 0: its g v may be infinite.
 // Bound as the forward kernel.  Measured: 20 000 rows, 8 heads of 16, segments up to 128: 31 us for the queries, 42
-// for the keys and values.
+// for the keys and values; 33 and 47 in fp16.
 #pragma once
 
 #include "attention.cuh"

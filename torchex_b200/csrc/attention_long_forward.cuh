@@ -12,10 +12,13 @@
 // While the softmax works on one buffer of scores, the products of the other one run (with one buffer of 128 columns
 // per query tile the softmax waited 1600 of every 4300 cycles for the products between two of its tiles).
 // The outputs are rescaled only when a row's maximum has grown by more than 2^8 (the sums carry the stale
-// maximum until then: probabilities up to 2^8 lose nothing in fp32 sums), which is rare after the first tiles.
-// Bound: exponentials.  128 x 128 of them take 1024 cycles of an SM, the two products of that many 512 at
-// the tensor cores' nominal rate.  Measured: 32 768 rows, 8 heads of 128, up to 4096 keys, causal, 205 us (a floor of
-// 105 for the products alone).
+// maximum until then: probabilities up to 2^8 lose nothing in fp32 sums), which is rare after the first tiles; the
+// technique is a published one.
+// Bound: products and exponentials together.  For 128 x 128 scores of 128 columns the products take some 1280 cycles of
+// an SM (768 for the scores, in tiles of 64 columns at three quarters of the full rate, 512 for the outputs), the
+// exponentials 1024.  Measured: 32 768 rows, 8 heads of 128, up to 4096 keys, causal, 206 us on the same inputs again
+// and again, 229 on new ones (a floor of 105 for the products alone); over the launch the tensor pipe is 46 % busy and
+// the special function pipe 50 %.
 #pragma once
 
 #include "attention_long.cuh"

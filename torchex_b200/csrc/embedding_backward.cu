@@ -13,8 +13,8 @@
 //      nobody asked for, so the larger part of a sparse gradient is written while the sort runs.
 //      More tokens take the plan builder's multi-launch sort, and a kernel that looks every row
 //      up in the sorted tokens clears the others.
-//   2. Tiles of consecutive sorted positions are walked by one group of lanes each, eight rows
-//      of g in flight whatever the lengths of the runs.  A run that begins and ends inside its
+//   2. Tiles of consecutive sorted positions are walked by one group of lanes each, three batches
+//      of eight rows of g (four of fp32) in flight whatever the lengths of the runs.  A run that begins and ends inside its
 //      tile is written at once; the parts of the others go to two slots per tile, in fp32.
 //   3. Where a run first crosses a tile boundary, one group adds its parts in order; runs of
 //      many tiles (padding that is not excluded, very frequent tokens) are added by all
