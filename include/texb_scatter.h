@@ -469,11 +469,12 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
  * Query heads share key / value heads in consecutive groups of heads / kv_heads.
  * Scores, softmax statistics and sums are fp32; probabilities and the gradients of
  * scores are rounded to the tensors' type before they are multiplied, in fp16 after a
- * power of two has brought them into its range.  A row that a query
- * does not see has no influence on it, whatever it holds (NaN and infinities included);
- * beside rows that are not finite results may differ in their last bits from what they
- * are otherwise, and take much longer.
- * No atomics: bit-reproducible run to run.  Nothing synchronises.
+ * power of two has brought them into its range.  A row that a query does not see has no
+ * influence on it, whatever it holds (NaN and infinities included), but for last bits:
+ * beside rows that are not finite sums are formed in another order (which takes much
+ * longer), and the powers of two of fp16 gradients go by the largest rows of v and g of
+ * the whole segment, later ones under `causal` included.
+ * No atomics whose order matters: bit-reproducible run to run.  Nothing synchronises.
  *   Limits: TEXB_BFLOAT16 or TEXB_FLOAT16; dim a multiple of 8 up to 128; pointers and
  *   strides (in values) such that rows start on 16-byte boundaries; heads a multiple of
  *   kv_heads; n < 2^31 - 65536; softcap 0 and scale times log2(e) finite in fp32, or
