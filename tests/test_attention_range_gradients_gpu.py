@@ -60,3 +60,60 @@ def test_large_gradients_in_other_segments(lens, dim):
     g[n:] = (g[n:].float() * 8192).clamp(-60000, 60000).half()
     q[n:], k[n:] = q[n:] / 64, k[n:] / 64
     _check(_step(q, k, v, g, data), _definition(q, k, v, g, [*lens, *lens], False, dim ** -0.5))
+
+
+@pytest.mark.parametrize("lens,dim", SHAPES)
+def test_zeros_and_infinities(lens, dim):
+    """No row has a largest value to go by: gradients are 0, not NaN."""
+    ids, data = _plan(lens + lens, False)
+    n = sum(lens)
+    q, k, v, g = _inputs(2 * n, 4, 2, dim, torch.float16, 3)
+    zero = torch.zeros_like
+    for got in (_step(q, k, v, zero(g), data), _step(q, k, v, g, data, scale=0.0)):
+        assert (got[1] == 0).all() and (got[2] == 0).all()
+    assert (_step(q, k, v, zero(g), data)[3] == 0).all()
+    got = _step(q, k, zero(v), g, data)
+    assert (got[0] == 0).all() and (got[1] == 0).all() and (got[2] == 0).all() and got[3].isfinite().all()
+
+
+@pytest.mark.parametrize("lens,dim", SHAPES)
+def test_infinities_in_other_segments(lens, dim):
+    ids, data = _plan(lens + lens, False)
+    n = sum(lens)
+    q, k, v, g = _inputs(2 * n, 2, 2, dim, torch.float16, 3)
+    g = (g.float() * 2.0 ** -10).half()
+    want = [(value[:n], bound[:n]) for value, bound in _definition(q, k, v, g, lens + lens, False, dim ** -0.5)]
+    for i in (2, 3):
+        ill = [q, k, v, g]
+        ill[i] = ill[i].clone()
+        ill[i][n:] = float("inf")
+        _check([x[:n] for x in _step(*ill, data)], want)
+
+
+def test_captured_and_on_another_stream():
+    lens = [70, 200, 33, 600]
+    ids, data = _plan(lens, True, 2)
+    inputs = _inputs(sum(lens), 4, 2, 64, torch.float16, 4)
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        held = [torch.zeros_like(x) for x in inputs]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = _step(*held, data, causal=True)
+        graphs.append((graph, held, outs))
+    for seed, power in ((4, 0), (5, -12), (6, 3)):
+        q, k, v, g = _inputs(sum(lens), 4, 2, 64, torch.float16, seed)
+        new = [q, k, v, (g.float() * 2.0 ** power).half()]
+        want = _step(*new, data, causal=True)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = _step(*new, data, causal=True)
+        torch.cuda.current_stream().wait_stream(side)
+        for graph, held, _ in graphs:
+            for a, b in zip(held, new):
+                a.copy_(b)
+            graph.replay()
+        torch.cuda.synchronize()
+        for got in (other, *(outs for _, _, outs in graphs)):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

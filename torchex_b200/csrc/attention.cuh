@@ -183,7 +183,7 @@ template <typename T> __device__ __forceinline__ uint32_t pack_lifted(float lo, 
 // small as the gradients, which is about g over the length of the segment: for g of 2^-10 and 2048 rows the unlifted
 // ones were off by 2 %.  A row has one factor for all that is added up for it, and its sum is divided by it.  Under
 // `causal` the largest rows may be ones that are not seen: 2^10 times larger than those that are, they leave fp16's
-// normal numbers for gradients down to some 2^-17 of their bound, and the factor is never below 1.
+// normal numbers for gradients down to 2^-18 of their bound, and the factor is never below 1.
 __device__ __forceinline__ int gradient_lift(const Problem& a, float g_square, float v_square) {
   const float bound = 2.f * fabsf(a.scale) * sqrtf(g_square) * sqrtf(v_square);
   return min(100, max(0, 14 - (int(__float_as_uint(bound) >> 23) - 127)));
