@@ -467,7 +467,9 @@ int texb_clip_grads(int count, const void* const* grads, const int64_t* sizes, c
  *          segment, in increasing row order);
  *   out_i = sum_j softmax_j(x_ij) v_j over the rows j of i's segment, up to i if causal.
  * Query heads share key / value heads in consecutive groups of heads / kv_heads.
- * Scores, softmax statistics and sums are fp32; probabilities and the gradients of
+ * Scores, softmax statistics and sums are fp32, so a probability of the backward pass,
+ * formed again from a score x, is off by some 2^-23 |x| of itself (outputs hold for
+ * scores of any size, gradients for scores far below 2^23); probabilities and the gradients of
  * scores are rounded to the tensors' type before they are multiplied, in fp16 after a
  * power of two has brought them into its range.  A row that a query does not see has no
  * influence on it, whatever it holds (NaN and infinities included), but for last bits:

@@ -92,3 +92,22 @@ def test_small_probabilities_reach_the_output(lens, dim, below):
     want = _definition(q, k, v, g, lens, False, 1.0)
     assert want[0][0].abs().max() > 2 ** -22
     _check([segment_attention(q, k, v, data, scale=1.0)], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,dim", [(300, 16), (20, 64), (300, 64), (300, 128)])
+@pytest.mark.parametrize("power", [10, 20, 24, 28, 32, 60])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size(dtype, n, dim, power, sign):
+    """One key is so far above the others that it takes all the weight: the output is its value, off by the roundings of
+    the weight and of the output."""
+    gen = torch.Generator(device=DEV).manual_seed(power)
+    q, k, v = (torch.zeros(n, 1, dim, device=DEV, dtype=dtype) for _ in range(3))
+    q[:, 0, 0] = 2.0 ** 15 * (1 + torch.rand(n, generator=gen, device=DEV) / 2).to(dtype)
+    k[:, 0, 0] = sign * (800 + 100 * torch.rand(n, generator=gen, device=DEV)).to(dtype)
+    k[n // 3, 0, 0] = 1100.0 if sign > 0 else -600.0
+    v[:, 0] = (torch.rand(n, dim, generator=gen, device=DEV) + 1).to(dtype)
+    ids, data = _plan([n], False)
+    out = segment_attention(q, k, v, data, scale=2.0 ** (power - 25))
+    want = v[n // 3].double()
+    assert ((out.double() - want).abs() <= (torch.finfo(dtype).eps + 2 ** -20) * want).all()

@@ -27,6 +27,11 @@ namespace texb {
 namespace attention {
 
 constexpr float kStale = 8.f;  // growth of a row's maximum, in units of log2, that is left unscaled
+// Scores, in the same units, beyond which a query tile is computed again by the plain loops.  `top` is a rounded product,
+// and one rounding of s unit - top leaves what that took from it: all weights of a row have it in common, but it is half
+// a step of the score, 1 at 2^24 and 64 at 2^30, and takes the lifted weights out of fp16, or those of bf16 out of fp32.
+// (A second rounding in the loop for such scores, behind a branch, took 216 us instead of 206 for all others.)
+template <typename T> constexpr float kLargeScore = kShortRange<T> ? 16777216.f : 1073741824.f;
 
 template <int DP>
 struct LongForwardMemory {
@@ -56,7 +61,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   constexpr int N = M::kKeys, S = M::kStages;
   unsigned char* smem = raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023);
   __shared__ uint32_t s_tmem;
-  __shared__ int s_dead;
+  __shared__ int s_dead, s_large;
   const uint32_t base = t5::smem_u32(smem);
   auto bar = [&](int i) { return base + M::kBarriers + i * 8; };
   // barriers by stage: keys full, keys empty, values full, values empty; by query tile and buffer: scores full,
@@ -66,7 +71,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   static_assert((kSettle + 2) * 8 <= 256, "room for the barriers");
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
   if (threadIdx.x == 0) {
-    s_dead = 0;
+    s_dead = s_large = 0;
     const int copiers = maps.used ? 1 : 4;
     t5::barrier_init(bar(kQueries), copiers);
     for (int s = 0; s < S; ++s) {
@@ -211,6 +216,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
       const int last = done - 1;  // products are done in order: the last one means all
       t5::warp_wait(bar(kDone + 2 * w + (last & 1)), (last >> 1) & 1, dead);
       const bool there = i < a.n;
+      if (MODE == kPlain && fabsf(top) > kLargeScore<T> && fabsf(top) < INFINITY) s_large = 1;
       const float total = sum.x + sum.y, factor = see.end > see.begin ? 1.f / total : 0.f;
       if (there && a.lse) a.lse[int64_t(head) * a.n + i] = see.end > see.begin ? top - kLift + log2f(total) : 0.f;
       T* to = row_at<T>(a, a.out, head, min(i, a.n - 1));
@@ -311,6 +317,7 @@ long_forward_kernel(const __grid_constant__ Problem a, const __grid_constant__ M
   __syncthreads();
   t5::fence_after_sync();
   if (warp == 12) t5::tmem_free(tmem, M::kColumns);
+  if (MODE == kPlain && s_large) plain_forward<T>(a, pos0, kLongRows, head);
 }
 
 template <typename T, int DP, int MODE>
