@@ -16,7 +16,7 @@
 // technique is a published one.
 // Bound: products and exponentials together.  For 128 x 128 scores of 128 columns the products take some 1280 cycles of
 // an SM (768 for the scores, in tiles of 64 columns at three quarters of the full rate, 512 for the outputs), the
-// exponentials 1024.  Measured: 32 768 rows, 8 heads of 128, up to 4096 keys, causal, 206 us on the same inputs again
+// exponentials 1024.  Measured: 32 768 rows, 8 heads of 128, up to 4096 keys, causal, 208 us on the same inputs again
 // and again, 229 on new ones (a floor of 105 for the products alone); over the launch the tensor pipe is 46 % busy and
 // the special function pipe 50 %.
 #pragma once
