@@ -200,8 +200,10 @@ look_over_kernel(const __grid_constant__ Problem a, Spread q_spread, Spread k_sp
         raise(word_of(a, keys, first_head + threadIdx.x, first), most);
       }
     } else {
-      for (int i = threadIdx.x; i < (end - pos0) * there; i += kThreads)
-        raise(word_of(a, keys, first_head + i % there, first_of(a, pos0 + i / there)), s_square[i / there * sp.heads + i % there]);
+      for (int i = threadIdx.x; i < (end - pos0) * there; i += kThreads) {
+        const int r = i / there, h = i % there;
+        raise(word_of(a, keys, first_head + h, first_of(a, pos0 + r)), s_square[r * sp.heads + h]);
+      }
     }
   }
 }

@@ -27,11 +27,12 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, data, s
 
     Differentiable once, by q, k and v.  Statistics and sums are fp32; probabilities and
     gradients of scores are rounded to the dtype of q before they are multiplied (float16: after a
-    power of two has brought them into its range, so that small gradients keep their bits).  Results are
-    bit-reproducible.  Rows that a query does not see have no influence on its results, whatever they
-    hold, but for last bits: beside rows that are not finite tiles are added up in another (slower)
-    way, and the powers of two of float16 gradients go by the largest rows of the whole segment.  A call that records a gradient keeps, beside q, k, v and the output, what
-    rounding took from the output, a tensor of the same size."""
+    power of two has brought them into its range, so that small gradients keep their bits).  Results
+    are bit-reproducible.  Rows that a query does not see have no influence on its results, whatever
+    they hold, but for last bits: beside rows that are not finite tiles are added up in another
+    (slower) way, and the powers of two of float16 gradients go by the largest rows of the whole
+    segment.  A call that records a gradient keeps, beside q, k, v and the output, what rounding took
+    from the output, a tensor of the same size."""
     if data._pending is not None:
         data._poll()
     if not isinstance(q, torch.Tensor) or q.ndim != 3:
